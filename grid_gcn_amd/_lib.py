@@ -58,6 +58,9 @@ EXPORTS = [
     "gridgcn_edge_geo_forward_workspace_bytes", "gridgcn_edge_geo_forward",
     "gridgcn_edge_lin0_backward_sparse_geo", "gridgcn_linear_fwd_direct_fin",
     "gridgcn_linear_fwd_direct_drop", "gridgcn_linear_dw_drop",
+    "gridgcn_act8_pack", "gridgcn_act8_unpack",
+    "gridgcn_group_norm_act_workspace_bytes", "gridgcn_group_norm_act_fwd", "gridgcn_group_norm_act_bwd",
+    "gridgcn_linear_act8_fwd", "gridgcn_linear_act8_bwd_workspace_bytes", "gridgcn_linear_act8_bwd",
 ]
 
 
@@ -324,6 +327,24 @@ def declare(lib, path="<library>"):
     lib.gridgcn_gridconv_forward.argtypes = [vp, vp, vp, ci, ci, ci, ci, ci, ci, ci, ci, ci,
                                              ctypes.POINTER(ConvLayer), ctypes.POINTER(ConvLayer),
                                              vp, vp]
+    lib.gridgcn_act8_pack.restype = ci
+    lib.gridgcn_act8_pack.argtypes = [vp, ci, ll, ci, ll, vp, vp, vp]
+    lib.gridgcn_act8_unpack.restype = ci
+    lib.gridgcn_act8_unpack.argtypes = [vp, vp, ll, ci, ci, vp, ll, vp]
+    lib.gridgcn_group_norm_act_workspace_bytes.restype = ci
+    lib.gridgcn_group_norm_act_workspace_bytes.argtypes = [ci, ll, ci, ci, ci, ci, ctypes.POINTER(cs)]
+    lib.gridgcn_group_norm_act_fwd.restype = ci
+    lib.gridgcn_group_norm_act_fwd.argtypes = [vp, ci, ci, ll, ci, ll, ll, ci, vp, vp, ci, vp, cf, ci, vp, vp, vp, vp,
+                                               vp, cs, vp]
+    lib.gridgcn_group_norm_act_bwd.restype = ci
+    lib.gridgcn_group_norm_act_bwd.argtypes = [vp, ll, ll, vp, ll, ll, vp, vp, ci, ci, ll, ci, ci, vp, vp, vp, ci, vp,
+                                               ci, vp, vp, vp, vp, cs, vp]
+    lib.gridgcn_linear_act8_fwd.restype = ci
+    lib.gridgcn_linear_act8_fwd.argtypes = [vp, ci, ll, ci, ll, vp, vp, ci, vp, vp, vp, vp]
+    lib.gridgcn_linear_act8_bwd_workspace_bytes.restype = ci
+    lib.gridgcn_linear_act8_bwd_workspace_bytes.argtypes = [ll, ci, ci, ctypes.POINTER(cs)]
+    lib.gridgcn_linear_act8_bwd.restype = ci
+    lib.gridgcn_linear_act8_bwd.argtypes = [vp, ci, ll, ci, ll, vp, ci, vp, vp, vp, vp, vp, vp, cs, vp]
     return lib
 
 

@@ -1,0 +1,819 @@
+// gridgcn_gnorm.hip -- group normalisation with an activation on channels-last rows, forward and backward.
+//
+//   x [B, N, C], G groups of cg = C / G channels, statistics of a (cloud, group) over its rows n < count_b and its channels:
+//     d = x - mean,  t = d * rstd * gamma_c + beta_c,  y = act(t);       rows n >= count_b: y = 0, dx = 0, never read
+//   backward, x^ = x or the 8-bit form the forward kept (gridgcn_act8.h), d = x^ - mean, xh = d * rstd:
+//     g = dy * act'(t);  dbeta_c = sum g;  dgamma_c = sum g xh;
+//     dx = rstd (gamma g - S1 - xh S2),  S1 = sum_group(gamma g) / M,  S2 = sum_group(gamma g xh) / M,  M = count_b * cg
+//
+// All of it is streaming: a thread keeps one column chunk of 16 bytes (its channels' constants sit in registers) and walks
+// rows.  The statistics are a reduction over a whole cloud, so a pass over the data has to end before the next begins: two
+// passes with a small launch between them that turns the workgroups' partial sums into statistics, or -- where the rows of a
+// few groups of one cloud fit a CU's caches -- ONE launch whose workgroup reads its rows twice.
+//
+// Numerics.  Sums of the statistics run in 64 bits on x - x[first row, first channel of the group] (64-bit vector adds run at
+// the rate of 32-bit ones here, the passes wait for memory): the variance needs no second look at the data even when the mean is
+// large against it.  The mean is subtracted as two floats, so d is x - mean to 32 bits whatever the mean.  Sums of the backward:
+// 32 bits over UNROLL rows, then 64.  The sign of t decides a whole gradient under ReLU: where |t| is within the rounding of
+// its two terms, it is formed again in 64 bits.  No atomics: every sum has one order.
+#include "../../include/gridgcn.h"
+#include "gridgcn_act8.h"
+#include <type_traits>
+
+namespace {
+constexpr int THREADS = 256;
+constexpr int UNROLL = 4;
+constexpr float SQRT1_2 = 0.70710678118654752f, INV_SQRT_2PI = 0.39894228040143268f;
+
+struct Lay { int nq, tpr, rpb; };          // chunks of a slab row, threads per row, rows per step
+Lay lay_of(int nq)
+{
+    Lay l;
+    l.nq = nq;
+    l.tpr = nq < THREADS ? nq : THREADS;
+    l.rpb = THREADS / l.tpr;
+    return l;
+}
+
+struct Args {
+    const void *x, *dy;
+    const uint8_t *codes, *scales;
+    uint8_t *codes_out, *scales_out;
+    void *y;                               // y or dx, contiguous [B, N, C]
+    long long N, xb, xn, gb, gn;           // strides of x and dy in elements
+    int B, C, G, cg, ptype;
+    const void *gamma, *beta;
+    void *dgamma, *dbeta;
+    const int *counts;
+    float eps;
+    double *stats;                         // [B, G, 2] mean, rstd
+    double *part;                          // [B, chunks, C, 2] partial sums of the workgroups
+    double *tot;                           // [B, C, 2] sums of g and g * xh
+    float2 *coef;                          // [B, G] S1, S2
+    long long rpc;                         // rows of a chunk
+    int chunks;
+};
+
+__device__ __forceinline__ long long count_of(const Args &a, int b)
+{
+    if (!a.counts) return a.N;
+    const long long n = a.counts[b];
+    return n < 0 ? 0 : (n < a.N ? n : a.N);
+}
+
+template <int ACT> __device__ __forceinline__ float act_of(float t)
+{
+    if constexpr (ACT == GRIDGCN_ACT_RELU) return t > 0.f ? t : (t != t ? t : 0.f);     // (NaN stays NaN)
+    if constexpr (ACT == GRIDGCN_ACT_SILU) return t / (1.f + __expf(-t));
+    if constexpr (ACT == GRIDGCN_ACT_GELU) return 0.5f * t * (1.f + erff(t * SQRT1_2));
+    return t;
+}
+template <int ACT> __device__ __forceinline__ float act_grad(float t)
+{
+    if constexpr (ACT == GRIDGCN_ACT_SILU) {
+        const float s = 1.f / (1.f + __expf(-t));
+        return s * (1.f + t * (1.f - s));
+    }
+    if constexpr (ACT == GRIDGCN_ACT_GELU)
+        return 0.5f * (1.f + erff(t * SQRT1_2)) + t * __expf(-0.5f * t * t) * INV_SQRT_2PI;
+    return 1.f;
+}
+
+// constants of one channel
+struct Chan { float mh, ml, a, beta, rstd, gamma; };
+__device__ __forceinline__ Chan chan_of(const Args &a, double mean, double rstd, int c)
+{
+    Chan k;
+    k.mh = (float)mean;
+    k.ml = (float)(mean - (double)k.mh);
+    k.rstd = (float)rstd;
+    k.gamma = gg_ld_param(a.gamma, a.ptype, c, 1.f);
+    k.beta = gg_ld_param(a.beta, a.ptype, c, 0.f);
+    k.a = (float)(rstd * (double)k.gamma);
+    return k;
+}
+// ... of the V channels of a thread, from the statistics in memory
+template <int V, class P> __device__ __forceinline__ void chans(const Args &a, const P &p, Chan (&k)[V])
+{
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const int c = p.c + i < a.C ? p.c + i : a.C - 1;
+        const double *st = a.stats + ((size_t)p.b * a.G + c / a.cg) * 2;
+        k[i] = chan_of(a, st[0], st[1], c);
+    }
+}
+__device__ __forceinline__ float dev_of(const Chan &k, float x) { return (x - k.mh) - k.ml; }
+
+// ReLU: is t = d a + beta > 0?  The float value is off by less than 2^-21 of |beta| where the two terms cancel.
+__device__ __forceinline__ bool positive(const Chan &k, float t, float x, const double *stat, const Args &a)
+{
+    if (__builtin_expect(fabsf(t) <= fabsf(k.beta) * 0x1p-20f, 0)) {
+        const double t64 = ((double)x - stat[0]) * stat[1] * (double)k.gamma + (double)k.beta;
+        return t64 > 0.0;
+    }
+    return t > 0.f;
+}
+
+// where the workgroup's threads stand
+template <int V> struct Pos {
+    int tr, q, c, b;
+    bool on;
+    __device__ __forceinline__ Pos(const Lay &l, int q0, int b_)
+    {
+        tr = (int)threadIdx.x / l.tpr;
+        q = q0 + (int)threadIdx.x % l.tpr;
+        c = q * V;
+        b = b_;
+        on = tr < l.rpb && q < q0 + l.tpr && q < l.nq;
+    }
+};
+
+// Sums s[V][2] of the threads of a column over the workgroup's row lanes: LDS red[rpb][tpr * V][2]; afterwards red[0] holds them.
+template <int V> __device__ __forceinline__ void reduce_rows(double *red, const Lay &l, int tr, int qi, const double (&s)[V][2])
+{
+    const int w = l.tpr * V * 2;
+    if (tr < l.rpb) {
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            red[(size_t)tr * w + (qi * V + i) * 2] = s[i][0];
+            red[(size_t)tr * w + (qi * V + i) * 2 + 1] = s[i][1];
+        }
+    }
+    __syncthreads();
+    for (int j = threadIdx.x; j < w; j += THREADS) {
+        double v = red[j];
+        for (int r = 1; r < l.rpb; r++) v += red[(size_t)r * w + j];
+        red[j] = v;                        // (entry j of row 0 is this thread's alone)
+    }
+    __syncthreads();
+}
+
+// first pass over the rows r0 <= n < r1 of cloud b: sums of x - base and its square per channel, and (SAVE8) the 8-bit form
+template <class T, bool SAVE8>
+__device__ __forceinline__ void rows_stats(const Args &a, const Lay &l, const Pos<GGRowT<T>::V> &p, long long r0, long long r1,
+                                           double (&s)[GGRowT<T>::V][2], double (&base)[GGRowT<T>::V])
+{
+    constexpr int V = GGRowT<T>::V;
+    const T *x = (const T *)a.x + (size_t)p.b * a.xb;
+    const int Cp = gg_a8_cp(a.C), nb = Cp / GG_A8_BLOCK;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        s[i][0] = s[i][1] = 0.0;
+        const int c = p.c + i < a.C ? p.c + i : a.C - 1;
+        base[i] = r1 > r0 ? (double)GGRowT<T>::get(x + (c / a.cg) * a.cg) : 0.0;      // (row 0 is valid where any row is)
+    }
+    for (long long n0 = r0; n0 < r1; n0 += (long long)l.rpb * UNROLL) {
+        float v[UNROLL][V];
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            const long long n = n0 + (long long)u * l.rpb + p.tr;
+            if (p.on && n < r1) {
+                gg_ld_chunk(x + (size_t)n * a.xn, p.c, a.C, v[u]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; i++) v[u][i] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            const long long n = n0 + (long long)u * l.rpb + p.tr;
+            const bool in = p.on && n < r1;
+            if (in) {
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    const double d = (double)v[u][i] - base[i];
+                    s[i][0] += d;
+                    s[i][1] = fma(d, d, s[i][1]);
+                }
+            }
+            if constexpr (SAVE8) {
+                const unsigned byte = gg_a8_block_byte<V>(v[u]);
+                unsigned w[V / 4];
+                gg_a8_encode<V>(v[u], byte, w);
+                if (in) {
+                    const size_t r = (size_t)p.b * a.N + n;
+                    gg_a8_st_codes<V>(a.codes_out + r * Cp + p.c, w);
+                    if (p.c % GG_A8_BLOCK == 0) a.scales_out[r * nb + p.c / GG_A8_BLOCK] = (uint8_t)byte;
+                }
+            }
+        }
+    }
+}
+
+// mean and rstd of a group from the sums of its channels (all on the same base)
+__device__ __forceinline__ void finish_stats(double s, double q, double base, double m, float eps, double *mean, double *rstd)
+{
+    m = m < 1.0 ? 1.0 : m;
+    const double e = s / m;
+    double var = q / m - e * e;
+    var = var < 0.0 ? 0.0 : var;           // (NaN stays NaN)
+    *mean = base + e;
+    *rstd = 1.0 / sqrt(var + (double)eps);
+}
+
+// second pass: y of the rows r0 <= n < r1; rows from `count` on are zero
+template <class T, int ACT>
+__device__ __forceinline__ void rows_apply(const Args &a, const Lay &l, const Pos<GGRowT<T>::V> &p, long long r0, long long r1,
+                                           long long count, const Chan (&k)[GGRowT<T>::V])
+{
+    constexpr int V = GGRowT<T>::V;
+    const T *x = (const T *)a.x + (size_t)p.b * a.xb;
+    T *y = (T *)a.y + (size_t)p.b * a.N * a.C;
+    if (!p.on) return;
+    for (long long n0 = r0 + p.tr; n0 < r1; n0 += (long long)l.rpb * UNROLL) {
+        float v[UNROLL][V];
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            const long long n = n0 + (long long)u * l.rpb;
+            if (n < count && n < r1) {
+                gg_ld_chunk(x + (size_t)n * a.xn, p.c, a.C, v[u]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; i++) v[u][i] = 0.f;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            const long long n = n0 + (long long)u * l.rpb;
+            float o[V];
+#pragma unroll
+            for (int i = 0; i < V; i++) o[i] = n < count ? act_of<ACT>(fmaf(dev_of(k[i], v[u][i]), k[i].a, k[i].beta)) : 0.f;
+            if (n < r1) gg_st_chunk(y + (size_t)n * a.C, p.c, a.C, o);
+        }
+    }
+}
+
+// x^ of one chunk: the input itself or its 8-bit form
+template <class T, bool Q8>
+__device__ __forceinline__ void ld_x(const Args &a, const Pos<GGRowT<T>::V> &p, long long n, float (&v)[GGRowT<T>::V])
+{
+    constexpr int V = GGRowT<T>::V;
+    if constexpr (Q8) {
+        const int Cp = gg_a8_cp(a.C);
+        const size_t r = (size_t)p.b * a.N + n;
+        gg_a8_ld<V>(a.codes + r * Cp + p.c, a.scales[r * (Cp / GG_A8_BLOCK) + p.c / GG_A8_BLOCK], v);
+    } else {
+        gg_ld_chunk((const T *)a.x + (size_t)p.b * a.xb + (size_t)n * a.xn, p.c, a.C, v);
+    }
+}
+
+// g = dy act'(t) of one value
+template <int ACT>
+__device__ __forceinline__ float gate(const Args &a, const Chan &k, float dy, float d, float x, const double *stat)
+{
+    if constexpr (ACT == GRIDGCN_ACT_NONE) return dy;
+    const float t = fmaf(d, k.a, k.beta);
+    if constexpr (ACT == GRIDGCN_ACT_RELU) return positive(k, t, x, stat, a) ? dy : 0.f;
+    return dy * act_grad<ACT>(t);
+}
+
+// backward, first pass over r0 <= n < r1 (all below count): s = sums of g and g * d per channel
+template <class T, int ACT, bool Q8>
+__device__ __forceinline__ void rows_bwd_sums(const Args &a, const Lay &l, const Pos<GGRowT<T>::V> &p, long long r0, long long r1,
+                                              const Chan (&k)[GGRowT<T>::V], double (&s)[GGRowT<T>::V][2])
+{
+    constexpr int V = GGRowT<T>::V;
+    const T *dy = (const T *)a.dy + (size_t)p.b * a.gb;
+    const double *stat = a.stats + (size_t)p.b * a.G * 2;
+#pragma unroll
+    for (int i = 0; i < V; i++) s[i][0] = s[i][1] = 0.0;
+    if (!p.on) return;
+    for (long long n0 = r0 + p.tr; n0 < r1; n0 += (long long)l.rpb * UNROLL) {
+        float v[UNROLL][V], e[UNROLL][V];
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            const long long n = n0 + (long long)u * l.rpb;
+            if (n < r1) {
+                gg_ld_chunk(dy + (size_t)n * a.gn, p.c, a.C, e[u]);
+                ld_x<T, Q8>(a, p, n, v[u]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; i++) { e[u][i] = 0.f; v[u][i] = k[i].mh; }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+            for (int u = 0; u < UNROLL; u++) {
+                const float d = dev_of(k[i], v[u][i]);
+                const int c = p.c + i < a.C ? p.c + i : a.C - 1;
+                const float g = gate<ACT>(a, k[i], e[u][i], d, v[u][i], stat + (c / a.cg) * 2);
+                s0 += g;
+                s1 = fmaf(g, d, s1);
+            }
+            s[i][0] += (double)s0;
+            s[i][1] += (double)s1;
+        }
+    }
+}
+
+// backward, second pass: dx of the rows r0 <= n < r1; rows from `count` on are zero
+template <class T, int ACT, bool Q8>
+__device__ __forceinline__ void rows_bwd_dx(const Args &a, const Lay &l, const Pos<GGRowT<T>::V> &p, long long r0, long long r1,
+                                            long long count, const Chan (&k)[GGRowT<T>::V], const float2 (&f)[GGRowT<T>::V])
+{
+    constexpr int V = GGRowT<T>::V;
+    const T *dy = (const T *)a.dy + (size_t)p.b * a.gb;
+    T *dx = (T *)a.y + (size_t)p.b * a.N * a.C;
+    const double *stat = a.stats + (size_t)p.b * a.G * 2;
+    if (!p.on) return;
+    for (long long n0 = r0 + p.tr; n0 < r1; n0 += (long long)l.rpb * UNROLL) {
+        float v[UNROLL][V], e[UNROLL][V];
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            const long long n = n0 + (long long)u * l.rpb;
+            if (n < count && n < r1) {
+                gg_ld_chunk(dy + (size_t)n * a.gn, p.c, a.C, e[u]);
+                ld_x<T, Q8>(a, p, n, v[u]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; i++) { e[u][i] = 0.f; v[u][i] = k[i].mh; }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            const long long n = n0 + (long long)u * l.rpb;
+            float o[V];
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const float d = dev_of(k[i], v[u][i]);
+                const int c = p.c + i < a.C ? p.c + i : a.C - 1;
+                const float g = gate<ACT>(a, k[i], e[u][i], d, v[u][i], stat + (c / a.cg) * 2);
+                // (gamma * g rounded on its own: in a group of one value it equals S1, and dx is 0)
+                const float h = k[i].gamma * g;
+                o[i] = n < count ? ((h - f[i].x) - (d * k[i].rstd) * f[i].y) * k[i].rstd : 0.f;
+            }
+            if (n < r1) gg_st_chunk(dx + (size_t)n * a.C, p.c, a.C, o);
+        }
+    }
+}
+
+// ---- many rows: pass, small launch, pass ----------------------------------------------------------------------------
+template <class T, bool SAVE8>
+__global__ __launch_bounds__(THREADS) void gg_k_gn_stats(Args a, Lay l)
+{
+    constexpr int V = GGRowT<T>::V;
+    __shared__ double red[THREADS * V * 2];
+    const Pos<V> p(l, blockIdx.y * l.tpr, blockIdx.z);
+    const long long count = count_of(a, p.b);
+    const long long r0 = (long long)blockIdx.x * a.rpc;
+    const long long r1 = r0 + a.rpc < count ? r0 + a.rpc : count;
+    double s[V][2], base[V];
+    rows_stats<T, SAVE8>(a, l, p, r0, r1, s, base);
+    reduce_rows<V>(red, l, p.tr, (int)threadIdx.x % l.tpr, s);
+    double *out = a.part + ((size_t)p.b * a.chunks + blockIdx.x) * a.C * 2;
+    const int c0 = blockIdx.y * l.tpr * V;
+    for (int j = threadIdx.x; j < l.tpr * V * 2; j += THREADS)
+        if (c0 + j / 2 < a.C) out[(size_t)c0 * 2 + j] = red[j];
+}
+
+// sums over the chunks of one cloud for the n channels from c0 on: f(channel, sum 0, sum 1), each channel once, by the thread
+// that owns it.  red: LDS [THREADS * 2].  Every thread calls.
+template <class F> __device__ __forceinline__ void sum_chunks(const Args &a, int b, int c0, int n, double *red, F f)
+{
+    const int cw = n < THREADS ? n : THREADS, nl = THREADS / cw;
+    const int cl = threadIdx.x % cw, kl = threadIdx.x / cw;
+    for (int o = 0; o < n; o += cw) {
+        double s0 = 0.0, s1 = 0.0;
+        if (kl < nl && o + cl < n) {
+            const double *p = a.part + ((size_t)b * a.chunks * a.C + c0 + o + cl) * 2;
+            for (int k = kl; k < a.chunks; k += nl) {
+                s0 += p[(size_t)k * a.C * 2];
+                s1 += p[(size_t)k * a.C * 2 + 1];
+            }
+        }
+        red[threadIdx.x * 2] = s0;
+        red[threadIdx.x * 2 + 1] = s1;
+        __syncthreads();
+        if ((int)threadIdx.x < cw && o + cl < n) {
+            for (int k = 1; k < nl; k++) {
+                s0 += red[(k * cw + cl) * 2];
+                s1 += red[(k * cw + cl) * 2 + 1];
+            }
+            f(c0 + o + cl, s0, s1);
+        }
+        __syncthreads();
+    }
+}
+
+// the workgroup's sums of (s, q), in one order; every thread calls, all get them
+__device__ __forceinline__ void sum_block(double *red, double &s, double &q)
+{
+    red[threadIdx.x * 2] = s;
+    red[threadIdx.x * 2 + 1] = q;
+    for (int d = THREADS / 2; d > 0; d /= 2) {
+        __syncthreads();
+        if ((int)threadIdx.x < d) {
+            red[threadIdx.x * 2] += red[(threadIdx.x + d) * 2];
+            red[threadIdx.x * 2 + 1] += red[(threadIdx.x + d) * 2 + 1];
+        }
+    }
+    __syncthreads();
+    s = red[0];
+    q = red[1];
+}
+
+// for each of ng groups of cg values in LDS: the sums of get(value index) -> (s, q), then done(group, s, q) by one thread.
+// Many channels: a wave per group; few: a thread per group.
+template <class G, class D> __device__ __forceinline__ void for_groups(int cg, int ng, G get, D done)
+{
+    if (cg >= 32) {
+        const int lane = threadIdx.x & 63;
+        for (int j = threadIdx.x >> 6; j < ng; j += THREADS / 64) {
+            double s = 0.0, q = 0.0;
+            for (int c = lane; c < cg; c += 64) get(j * cg + c, s, q);
+#pragma unroll
+            for (int d = 32; d > 0; d /= 2) {
+                s += __shfl_xor(s, d);
+                q += __shfl_xor(q, d);
+            }
+            if (lane == 0) done(j, s, q);
+        }
+    } else {
+        for (int j = threadIdx.x; j < ng; j += THREADS) {
+            double s = 0.0, q = 0.0;
+            for (int c = 0; c < cg; c++) get(j * cg + c, s, q);
+            done(j, s, q);
+        }
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(THREADS) void gg_k_gn_stats_fin(Args a)
+{
+    __shared__ double red[THREADS * 2];
+    const int g = blockIdx.x, b = blockIdx.y;
+    double s = 0.0, q = 0.0;
+    sum_chunks(a, b, g * a.cg, a.cg, red, [&](int, double s0, double s1) { s += s0; q += s1; });
+    sum_block(red, s, q);
+    if (threadIdx.x == 0) {
+        const long long count = count_of(a, b);
+        const double base = count > 0 ? (double)GGRowT<T>::get((const T *)a.x + (size_t)b * a.xb + g * a.cg) : 0.0;
+        double *o = a.stats + ((size_t)b * a.G + g) * 2;
+        finish_stats(s, q, base, (double)count * a.cg, a.eps, o, o + 1);
+    }
+}
+
+template <class T, int ACT>
+__global__ __launch_bounds__(THREADS) void gg_k_gn_apply(Args a, Lay l)
+{
+    constexpr int V = GGRowT<T>::V;
+    const Pos<V> p(l, blockIdx.y * l.tpr, a.B - 1 - (int)blockIdx.z);
+    // (last rows first: they are what the pass before left in the caches)
+    const long long r0 = (long long)(gridDim.x - 1 - blockIdx.x) * a.rpc;
+    const long long r1 = r0 + a.rpc < a.N ? r0 + a.rpc : a.N;
+    Chan k[V];
+    chans<V>(a, p, k);
+    rows_apply<T, ACT>(a, l, p, r0, r1, count_of(a, p.b), k);
+}
+
+template <class T, int ACT, bool Q8>
+__global__ __launch_bounds__(THREADS) void gg_k_gn_bwd_sums(Args a, Lay l)
+{
+    constexpr int V = GGRowT<T>::V;
+    __shared__ double red[THREADS * V * 2];
+    const Pos<V> p(l, blockIdx.y * l.tpr, blockIdx.z);
+    const long long count = count_of(a, p.b);
+    const long long r0 = (long long)blockIdx.x * a.rpc;
+    const long long r1 = r0 + a.rpc < count ? r0 + a.rpc : count;
+    Chan k[V];
+    chans<V>(a, p, k);
+    double s[V][2];
+    rows_bwd_sums<T, ACT, Q8>(a, l, p, r0, r1, k, s);
+    reduce_rows<V>(red, l, p.tr, (int)threadIdx.x % l.tpr, s);
+    double *out = a.part + ((size_t)p.b * a.chunks + blockIdx.x) * a.C * 2;
+    const int c0 = blockIdx.y * l.tpr * V;
+    for (int j = threadIdx.x; j < l.tpr * V * 2; j += THREADS)
+        if (c0 + j / 2 < a.C) out[(size_t)c0 * 2 + j] = red[j];
+}
+
+// S1, S2 of a group from the sums of gamma g and gamma g d over it
+__device__ __forceinline__ float2 coef_of(const Args &a, int b, int g, double s1, double s2)
+{
+    const long long count = count_of(a, b);
+    if (count < 1) return make_float2(0.f, 0.f);
+    const double m = (double)count * a.cg, rstd = a.stats[((size_t)b * a.G + g) * 2 + 1];
+    return make_float2((float)(s1 / m), (float)(s2 * rstd / m));
+}
+
+__global__ __launch_bounds__(THREADS) void gg_k_gn_bwd_fin(Args a)
+{
+    __shared__ double red[THREADS * 2];
+    const int g = blockIdx.x, b = blockIdx.y;
+    const double rstd = count_of(a, b) > 0 ? a.stats[((size_t)b * a.G + g) * 2 + 1] : 0.0;
+    double s = 0.0, q = 0.0;
+    sum_chunks(a, b, g * a.cg, a.cg, red, [&](int c, double s0, double s1) {
+        double *t = a.tot + ((size_t)b * a.C + c) * 2;
+        t[0] = s0;
+        t[1] = s1 * rstd;
+        const double w = (double)gg_ld_param(a.gamma, a.ptype, c, 1.f);
+        s += w * s0;
+        q += w * s1;
+    });
+    sum_block(red, s, q);
+    if (threadIdx.x == 0) a.coef[(size_t)b * a.G + g] = coef_of(a, b, g, s, q);
+}
+
+// dgamma, dbeta of a channel: the clouds' totals in order
+__device__ __forceinline__ void params_of(const Args &a, int c)
+{
+    double db = 0.0, dg = 0.0;
+    for (int b = 0; b < a.B; b++) {
+        const double *t = a.tot + ((size_t)b * a.C + c) * 2;
+        db += t[0];
+        dg += t[1];
+    }
+    if (a.dbeta) gg_st_param(a.dbeta, a.ptype, c, (float)db);
+    if (a.dgamma) gg_st_param(a.dgamma, a.ptype, c, (float)dg);
+}
+
+template <class T, int ACT, bool Q8>
+__global__ __launch_bounds__(THREADS) void gg_k_gn_bwd_dx(Args a, Lay l)
+{
+    constexpr int V = GGRowT<T>::V;
+    if (blockIdx.x == 0 && blockIdx.z == 0) {
+        const int c0 = blockIdx.y * l.tpr * V, c1 = c0 + l.tpr * V < a.C ? c0 + l.tpr * V : a.C;
+        for (int c = c0 + threadIdx.x; c < c1; c += THREADS) params_of(a, c);
+    }
+    if (!a.y) return;
+    const Pos<V> p(l, blockIdx.y * l.tpr, a.B - 1 - (int)blockIdx.z);
+    const long long r0 = (long long)(gridDim.x - 1 - blockIdx.x) * a.rpc;
+    const long long r1 = r0 + a.rpc < a.N ? r0 + a.rpc : a.N;
+    Chan k[V];
+    chans<V>(a, p, k);
+    float2 f[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const int c = p.c + i < a.C ? p.c + i : a.C - 1;
+        f[i] = a.coef[(size_t)p.b * a.G + c / a.cg];
+    }
+    rows_bwd_dx<T, ACT, Q8>(a, l, p, r0, r1, count_of(a, p.b), k, f);
+}
+
+__global__ __launch_bounds__(THREADS) void gg_k_gn_params(Args a)
+{
+    const int c = blockIdx.x * THREADS + threadIdx.x;
+    if (c < a.C) params_of(a, c);
+}
+
+// ---- few rows: one launch, a workgroup = whole groups of one cloud (l.nq chunks from channel slab * slab_c on) ---------
+template <class T, int ACT, bool SAVE8>
+__global__ __launch_bounds__(THREADS) void gg_k_gn_small(Args a, Lay l, int slab_c)
+{
+    constexpr int V = GGRowT<T>::V;
+    __shared__ double red[THREADS * V * 2];
+    __shared__ double grp[THREADS * V * 2];
+    const int c0 = blockIdx.x * slab_c, c1 = c0 + slab_c < a.C ? c0 + slab_c : a.C;
+    Pos<V> p(l, c0 / V, blockIdx.y);
+    p.on = p.tr < l.rpb && p.c < (SAVE8 ? (c1 == a.C ? gg_a8_cp(a.C) : c1) : c1);
+    const long long count = count_of(a, p.b);
+    double s[V][2], base[V];
+    rows_stats<T, SAVE8>(a, l, p, 0, count, s, base);
+    reduce_rows<V>(red, l, p.tr, (int)threadIdx.x % l.tpr, s);
+    for_groups(a.cg, (c1 - c0) / a.cg, [&](int c, double &t, double &q) { t += red[c * 2]; q += red[c * 2 + 1]; },
+               [&](int j, double t, double q) {
+        const int g = c0 / a.cg + j;
+        const double b0 = count > 0 ? (double)GGRowT<T>::get((const T *)a.x + (size_t)p.b * a.xb + g * a.cg) : 0.0;
+        finish_stats(t, q, b0, (double)count * a.cg, a.eps, grp + j * 2, grp + j * 2 + 1);
+        a.stats[((size_t)p.b * a.G + g) * 2] = grp[j * 2];
+        a.stats[((size_t)p.b * a.G + g) * 2 + 1] = grp[j * 2 + 1];
+    });
+    __syncthreads();
+    if (p.c >= c1) p.on = false;
+    Chan k[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const int c = p.c + i < c1 ? p.c + i : c1 - 1;
+        const double *st = grp + (c / a.cg - c0 / a.cg) * 2;
+        k[i] = chan_of(a, st[0], st[1], c);
+    }
+    rows_apply<T, ACT>(a, l, p, 0, a.N, count, k);
+}
+
+template <class T, int ACT, bool Q8>
+__global__ __launch_bounds__(THREADS) void gg_k_gn_small_bwd(Args a, Lay l, int slab_c)
+{
+    constexpr int V = GGRowT<T>::V;
+    __shared__ double red[THREADS * V * 2];
+    __shared__ float2 cf[THREADS * V];
+    const int c0 = blockIdx.x * slab_c, c1 = c0 + slab_c < a.C ? c0 + slab_c : a.C;
+    Pos<V> p(l, c0 / V, blockIdx.y);
+    p.on = p.tr < l.rpb && p.c < c1;
+    const long long count = count_of(a, p.b);
+    Chan k[V];
+    chans<V>(a, p, k);
+    double s[V][2];
+    rows_bwd_sums<T, ACT, Q8>(a, l, p, 0, count, k, s);
+    reduce_rows<V>(red, l, p.tr, (int)threadIdx.x % l.tpr, s);
+    for_groups(a.cg, (c1 - c0) / a.cg, [&](int c, double &t, double &q) {
+        const double w = (double)gg_ld_param(a.gamma, a.ptype, c0 + c, 1.f);
+        t += w * red[c * 2];
+        q += w * red[c * 2 + 1];
+    }, [&](int j, double t, double q) { cf[j] = coef_of(a, p.b, c0 / a.cg + j, t, q); });
+    for (int j = threadIdx.x; j < c1 - c0; j += THREADS) {
+        const int c = c0 + j;
+        const double db = red[j * 2], dg = count > 0 ? red[j * 2 + 1] * a.stats[((size_t)p.b * a.G + c / a.cg) * 2 + 1] : 0.0;
+        if (a.B == 1) {
+            if (a.dbeta) gg_st_param(a.dbeta, a.ptype, c, (float)db);
+            if (a.dgamma) gg_st_param(a.dgamma, a.ptype, c, (float)dg);
+        } else {
+            a.tot[((size_t)p.b * a.C + c) * 2] = db;
+            a.tot[((size_t)p.b * a.C + c) * 2 + 1] = dg;
+        }
+    }
+    __syncthreads();
+    if (!a.y) return;
+    float2 f[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const int c = p.c + i < c1 ? p.c + i : c1 - 1;
+        f[i] = cf[c / a.cg - c0 / a.cg];
+    }
+    rows_bwd_dx<T, ACT, Q8>(a, l, p, 0, a.N, count, k, f);
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------
+struct Plan {
+    bool small;
+    int slab_c, slabs;      // small: channels of a workgroup
+    Lay l;                  // of a pass (small: of a slab)
+    int nq;                 // chunks of a row
+    long long rpc;
+    int chunks;
+    size_t off_part, off_tot, off_coef, off_stats, bytes;
+};
+
+long long gcd_ll(long long a, long long b) { return b ? gcd_ll(b, a % b) : a; }
+
+// Values of a workgroup of the one-launch form (it reads them twice, the second time from the CU's caches and L2).
+// Measured both ways (forward + backward, fp32): see the table beside gridgcn_group_norm_act_fwd's description.
+constexpr long long SMALL_VALUES = 32768;
+
+Plan plan_of(int B, long long N, int C, int G, int dtype, bool save8)
+{
+    Plan p = {};
+    const int V = dtype == GRIDGCN_F32 ? 4 : 8, cg = C / G;
+    p.nq = save8 ? gg_a8_cp(C) / V : (C + V - 1) / V;
+    // whole groups, whole chunks (whole blocks of the 8-bit form), at least 64 bytes of a row
+    const long long unit = save8 ? GG_A8_BLOCK : V;
+    long long slab = (long long)cg / gcd_ll(cg, unit) * unit;
+    const long long least = 64 / (dtype == GRIDGCN_F32 ? 4 : 2);
+    if (slab < least) slab = (least + slab - 1) / slab * slab;
+    if (slab > C) slab = C;
+    const long long per = N * slab;
+    auto quads = [&](long long s) { return save8 ? (s + GG_A8_BLOCK - 1) / GG_A8_BLOCK * (GG_A8_BLOCK / V) : (s + V - 1) / V; };
+    p.small = per <= SMALL_VALUES && quads(slab) <= THREADS;
+    if (p.small) {
+        // short rows are taken whole: a workgroup for 16 channels of one row would be all start-up
+        while (slab < C && N * slab * 2 <= 2048 && quads(slab * 2) <= THREADS) slab *= 2;
+        if (slab > C) slab = C;
+        p.slab_c = (int)slab;
+        p.slabs = (int)((C + slab - 1) / slab);
+        p.l = lay_of((int)quads(slab));
+    }
+    if (!p.small) {
+        p.l = lay_of(p.nq);
+        const long long slabs = (p.nq + p.l.tpr - 1) / p.l.tpr, step = (long long)p.l.rpb * UNROLL;
+        long long want = (2048 + B * slabs - 1) / (B * slabs);      // workgroups: two generations of four per CU
+        long long chunks = (N + step - 1) / step;
+        if (chunks > want) chunks = want;
+        p.rpc = ((N + chunks - 1) / chunks + step - 1) / step * step;
+        p.chunks = (int)((N + p.rpc - 1) / p.rpc);
+    }
+    size_t o = 0;
+    auto take = [&o](size_t n) { const size_t at = o; o += (n + 255) & ~(size_t)255; return at; };
+    p.off_part = take(p.small ? 0 : (size_t)B * p.chunks * C * 16);
+    p.off_tot = take((size_t)B * C * 16);
+    p.off_coef = take((size_t)B * G * 8);
+    p.off_stats = take((size_t)B * G * 16);
+    p.bytes = o ? o : 256;
+    return p;
+}
+
+// f((T *)nullptr) for the type
+template <class F> int with_type(int dtype, F f)
+{
+    if (dtype == GRIDGCN_F32) { f((float *)nullptr); return 0; }
+    if (dtype == GRIDGCN_BF16) { f((gg_bf16 *)nullptr); return 0; }
+    if (dtype == GRIDGCN_F16) { f((gg_f16 *)nullptr); return 0; }
+    return GRIDGCN_EINVAL;
+}
+
+template <class T, int ACT, bool SAVE8> void launch_fwd(Args &a, const Plan &p, hipStream_t st)
+{
+    if (p.small) {
+        gg_k_gn_small<T, ACT, SAVE8><<<dim3(p.slabs, a.B), THREADS, 0, st>>>(a, p.l, p.slab_c);
+        return;
+    }
+    const unsigned slabs = (p.nq + p.l.tpr - 1) / p.l.tpr;
+    gg_k_gn_stats<T, SAVE8><<<dim3(p.chunks, slabs, a.B), THREADS, 0, st>>>(a, p.l);
+    gg_k_gn_stats_fin<T><<<dim3(a.G, a.B), THREADS, 0, st>>>(a);
+    const Lay l = lay_of((a.C + GGRowT<T>::V - 1) / GGRowT<T>::V);
+    const unsigned sl = (l.nq + l.tpr - 1) / l.tpr;
+    gg_k_gn_apply<T, ACT><<<dim3(p.chunks, sl, a.B), THREADS, 0, st>>>(a, l);
+}
+
+template <class T, int ACT, bool Q8> void launch_bwd(Args &a, const Plan &p, hipStream_t st)
+{
+    if (p.small) {
+        gg_k_gn_small_bwd<T, ACT, Q8><<<dim3(p.slabs, a.B), THREADS, 0, st>>>(a, p.l, p.slab_c);
+        if (a.B > 1 && (a.dgamma || a.dbeta)) gg_k_gn_params<<<dim3((a.C + THREADS - 1) / THREADS), THREADS, 0, st>>>(a);
+        return;
+    }
+    const unsigned slabs = (p.l.nq + p.l.tpr - 1) / p.l.tpr;
+    gg_k_gn_bwd_sums<T, ACT, Q8><<<dim3(p.chunks, slabs, a.B), THREADS, 0, st>>>(a, p.l);
+    gg_k_gn_bwd_fin<<<dim3(a.G, a.B), THREADS, 0, st>>>(a);
+    const unsigned gx = a.y ? (unsigned)p.chunks : 1u, gz = a.y ? (unsigned)a.B : 1u;
+    gg_k_gn_bwd_dx<T, ACT, Q8><<<dim3(gx, slabs, gz), THREADS, 0, st>>>(a, p.l);
+}
+
+template <class T, bool Q> void fwd_act(Args &a, const Plan &p, int act, hipStream_t st)
+{
+    if (act == GRIDGCN_ACT_NONE) launch_fwd<T, GRIDGCN_ACT_NONE, Q>(a, p, st);
+    else if (act == GRIDGCN_ACT_RELU) launch_fwd<T, GRIDGCN_ACT_RELU, Q>(a, p, st);
+    else if (act == GRIDGCN_ACT_SILU) launch_fwd<T, GRIDGCN_ACT_SILU, Q>(a, p, st);
+    else launch_fwd<T, GRIDGCN_ACT_GELU, Q>(a, p, st);
+}
+template <class T, bool Q> void bwd_act(Args &a, const Plan &p, int act, hipStream_t st)
+{
+    if (act == GRIDGCN_ACT_NONE) launch_bwd<T, GRIDGCN_ACT_NONE, Q>(a, p, st);
+    else if (act == GRIDGCN_ACT_RELU) launch_bwd<T, GRIDGCN_ACT_RELU, Q>(a, p, st);
+    else if (act == GRIDGCN_ACT_SILU) launch_bwd<T, GRIDGCN_ACT_SILU, Q>(a, p, st);
+    else launch_bwd<T, GRIDGCN_ACT_GELU, Q>(a, p, st);
+}
+
+bool sizes_ok(int B, long long N, int C, int G)
+{
+    // (grid.y and grid.z are 16-bit)
+    return B >= 1 && B <= 65535 && N >= 1 && C >= 1 && C <= GRIDGCN_GN_MAX_C && G >= 1 && G <= C && C % G == 0;
+}
+bool type_ok(int t) { return t == GRIDGCN_F32 || t == GRIDGCN_BF16 || t == GRIDGCN_F16; }
+}  // namespace
+
+extern "C" {
+
+int gridgcn_group_norm_act_workspace_bytes(int B, long long N, int C, int G, int dtype, int save8, size_t *bytes)
+{
+    if (!bytes || !sizes_ok(B, N, C, G) || !type_ok(dtype)) return GRIDGCN_EINVAL;
+    // (the backward's plan has no padded channels: take the larger of the two)
+    const Plan f = plan_of(B, N, C, G, dtype, save8 != 0), b = plan_of(B, N, C, G, dtype, false);
+    *bytes = f.bytes > b.bytes ? f.bytes : b.bytes;
+    return GRIDGCN_OK;
+}
+
+int gridgcn_group_norm_act_fwd(const void *x, int dtype, int B, long long N, int C, long long ldb, long long ldn, int G,
+                               const void *gamma, const void *beta, int ptype, const int32_t *counts, float eps, int act,
+                               void *y, double *stats, uint8_t *codes, uint8_t *scales, void *ws, size_t ws_bytes, void *stream)
+{
+    if (!x || !y || !sizes_ok(B, N, C, G) || !type_ok(dtype) || !type_ok(ptype) || ldn < C || (B > 1 && ldb < 0) ||
+        !(eps >= 0.f) || act < GRIDGCN_ACT_NONE || act > GRIDGCN_ACT_GELU || !codes != !scales || ((uintptr_t)codes & 15))
+        return GRIDGCN_EINVAL;
+    const Plan p = plan_of(B, N, C, G, dtype, codes != nullptr);
+    if (!ws || ws_bytes < p.bytes) return GRIDGCN_EWORKSPACE;
+    Args a = {};
+    a.x = x; a.y = y; a.N = N; a.xb = ldb; a.xn = ldn; a.B = B; a.C = C; a.G = G; a.cg = C / G; a.ptype = ptype;
+    a.gamma = gamma; a.beta = beta; a.counts = counts; a.eps = eps; a.codes_out = codes; a.scales_out = scales;
+    a.part = (double *)((char *)ws + p.off_part);
+    a.stats = stats ? stats : (double *)((char *)ws + p.off_stats);
+    a.rpc = p.rpc; a.chunks = p.chunks;
+    const hipStream_t st = (hipStream_t)stream;
+    const int rc = with_type(dtype, [&](auto *t) {
+        typedef typename std::remove_pointer<decltype(t)>::type T;
+        if (codes) fwd_act<T, true>(a, p, act, st);
+        else fwd_act<T, false>(a, p, act, st);
+    });
+    if (rc) return rc;
+    return hipGetLastError() == hipSuccess ? GRIDGCN_OK : GRIDGCN_ELAUNCH;
+}
+
+int gridgcn_group_norm_act_bwd(const void *dy, long long ldgb, long long ldgn, const void *x, long long ldb, long long ldn,
+                               const uint8_t *codes, const uint8_t *scales, int dtype, int B, long long N, int C, int G,
+                               const double *stats, const void *gamma, const void *beta, int ptype, const int32_t *counts,
+                               int act, void *dx, void *dgamma, void *dbeta, void *ws, size_t ws_bytes, void *stream)
+{
+    if (!dy || !stats || !codes != !scales || (!x && !codes) || !sizes_ok(B, N, C, G) || !type_ok(dtype) || !type_ok(ptype) ||
+        ldgn < C || (x && !codes && ldn < C) || act < GRIDGCN_ACT_NONE || act > GRIDGCN_ACT_GELU || ((uintptr_t)codes & 15))
+        return GRIDGCN_EINVAL;
+    if (!dx && !dgamma && !dbeta) return GRIDGCN_OK;
+    const Plan p = plan_of(B, N, C, G, dtype, false);
+    if (!ws || ws_bytes < p.bytes) return GRIDGCN_EWORKSPACE;
+    Args a = {};
+    a.dy = dy; a.gb = ldgb; a.gn = ldgn; a.x = x; a.xb = ldb; a.xn = ldn; a.codes = codes; a.scales = scales;
+    a.y = dx; a.N = N; a.B = B; a.C = C; a.G = G; a.cg = C / G; a.ptype = ptype; a.gamma = gamma; a.beta = beta;
+    a.dgamma = dgamma; a.dbeta = dbeta; a.counts = counts; a.stats = (double *)stats;
+    a.part = (double *)((char *)ws + p.off_part);
+    a.tot = (double *)((char *)ws + p.off_tot);
+    a.coef = (float2 *)((char *)ws + p.off_coef);
+    a.rpc = p.rpc; a.chunks = p.chunks;
+    const hipStream_t st = (hipStream_t)stream;
+    const int rc = with_type(dtype, [&](auto *t) {
+        typedef typename std::remove_pointer<decltype(t)>::type T;
+        if (codes) bwd_act<T, true>(a, p, act, st);
+        else bwd_act<T, false>(a, p, act, st);
+    });
+    if (rc) return rc;
+    return hipGetLastError() == hipSuccess ? GRIDGCN_OK : GRIDGCN_ELAUNCH;
+}
+
+}  // extern "C"

@@ -50,11 +50,60 @@ class ConvBNReLU(nn.Module):
         return w.contiguous(), b.contiguous()
 
 
-def mlp(cin, dims, bn_decay=0.9):
-    """mlp2d_c / mlp1d_c (utils/ops.py:236-260)."""
+class ConvGNAct(nn.Module):
+    """conv (kernel 1) + group normalisation + activation on channels-last input [B, ..., cin]: ConvBNReLU with statistics
+    of one sample instead of the batch (one cloud per GPU, ragged batches).  Not a layer of the reference.
+
+    Training on the GPU keeps the conv's input and the normalisation's input in 8 bits (ops.linear_act8,
+    ops.group_norm_act): 1.03 bytes a value instead of 4 between forward and backward.  On the CPU: stock PyTorch ops.
+    groups: default = the largest power of two <= 32 that leaves groups of at least 4 channels (1 where none does).
+    counts (forward): int32 [B] or [B, 1], valid rows of x [B, N, cin]."""
+
+    bn, use_relu = None, False          # (not a layer of the BatchNorm kernels: train/common.py: supported)
+
+    def __init__(self, cin, cout, groups=None, act="relu", eps=1e-5):
+        super().__init__()
+        if groups is None:
+            groups = next((g for g in (32, 16, 8, 4, 2) if cout % g == 0 and cout // g >= 4), 1)
+        self.lin = nn.Linear(cin, cout, bias=True)
+        nn.init.xavier_uniform_(self.lin.weight)
+        nn.init.zeros_(self.lin.bias)
+        self.norm = nn.GroupNorm(groups, cout, eps=eps)
+        if act not in ("none", "relu", "silu", "gelu"):
+            raise ValueError("act %r" % (act,))
+        self.act = act
+
+    def forward(self, x, counts=None):
+        g = self.norm
+        if x.is_cuda:
+            from . import ops
+            z = ops.linear_act8(x, self.lin.weight, self.lin.bias)
+            return ops.group_norm_act(z, g.weight, g.bias, g.num_groups, eps=g.eps, act=self.act, counts=counts, save8=True)
+        z = self.lin(x)
+        B, C = z.shape[0], z.shape[-1]
+        z3 = z.reshape(B, -1, g.num_groups, C // g.num_groups)
+        valid = None
+        if counts is not None:
+            valid = (torch.arange(z3.shape[1], device=z.device)[None] < counts.reshape(B, 1))[..., None, None]
+            z3 = torch.where(valid, z3, torch.zeros_like(z3))
+            m = (counts.reshape(B, 1, 1, 1).clamp(1, z3.shape[1]) * z3.shape[3]).to(z.dtype)
+        else:
+            m = float(z3.shape[1] * z3.shape[3])
+        mean = z3.sum((1, 3), keepdim=True) / m
+        d = z3 - mean if valid is None else (z3 - mean) * valid
+        t = d * torch.rsqrt((d * d).sum((1, 3), keepdim=True) / m + g.eps)
+        t = t.reshape(z.shape) * g.weight + g.bias
+        y = {"none": lambda v: v, "relu": F.relu, "silu": F.silu, "gelu": F.gelu}[self.act](t)
+        return y if valid is None else torch.where(valid[..., 0], y, torch.zeros_like(y))
+
+
+def mlp(cin, dims, bn_decay=0.9, norm="batch"):
+    """mlp2d_c / mlp1d_c (utils/ops.py:236-260).  norm: 'batch' (the reference's) or 'group' (ConvGNAct)."""
+    if norm not in ("batch", "group"):
+        raise ValueError("norm %r" % (norm,))
     layers = []
     for d in dims:
-        layers.append(ConvBNReLU(cin, d, bn_decay))
+        layers.append(ConvBNReLU(cin, d, bn_decay) if norm == "batch" else ConvGNAct(cin, d))
         cin = d
     return nn.Sequential(*layers)
 
@@ -79,7 +128,11 @@ def _warn_stock_fallback(layers, x):
 
 def run_mlp(layers, x, mfma=True):
     """A stack of ConvBNReLU layers.  Training on the GPU: one autograd op over the hand-written
-    kernels (tmlp.mlp_bn_relu_train); otherwise the stock PyTorch modules."""
+    kernels (tmlp.mlp_bn_relu_train); otherwise the stock PyTorch modules.  ConvGNAct layers have kernels of their own."""
+    if layers and all(isinstance(l, ConvGNAct) for l in layers):
+        for l in layers:
+            x = l(x)
+        return x
     if mfma and x.is_cuda and layers and layers[0].training and torch.is_grad_enabled():
         from .train import common as tcommon, evalpath as teval, mlp as tmlp
         if tcommon.supported(layers, x):
@@ -167,11 +220,12 @@ class SubGUpdate(nn.Module):
     pt_mlp     : per-edge feature MLP dims
     center_in  : channels of center_ori_feats (None: down layer)
     center_dim / out_dim : centre MLP and update MLP dims (up layers)
+    norm       : 'batch' or 'group' (every layer a ConvGNAct)
     """
 
     def __init__(self, in_feats, pt_mlp, localfdim=0, relu=True, center_in=None, center_dim=(),
                  out_dim=(), bn_decay=0.9, attfdim=10, aggtype="gcn", pool_type="max_pooling",
-                 att_full="", elevation=(), up_center_inte="concat", cntxt_mlp=None):
+                 att_full="", elevation=(), up_center_inte="concat", cntxt_mlp=None, norm="batch"):
         super().__init__()
         check_shipped_branches("segmentation", attfdim=attfdim, localfdim=localfdim,
                                aggtype=aggtype, pool_type=pool_type, att_full=att_full,
@@ -183,12 +237,12 @@ class SubGUpdate(nn.Module):
         cin = 3 if not self.has_feats else in_feats + (3 if localfdim != 0 else 0)
         self.cin = cin
         C = pt_mlp[-1]
-        self.pt_mlp = mlp(cin, pt_mlp, bn_decay)
-        self.att1 = mlp(10, [C // 4], bn_decay)          # update_att_mlp2d_frst (:141)
-        self.att2 = mlp(C // 4, [C], bn_decay)           # update_att_mlp2d_scnd (:152)
-        self.center_mlp = mlp(center_in, list(center_dim), bn_decay) if center_in else None
+        self.pt_mlp = mlp(cin, pt_mlp, bn_decay, norm)
+        self.att1 = mlp(10, [C // 4], bn_decay, norm)    # update_att_mlp2d_frst (:141)
+        self.att2 = mlp(C // 4, [C], bn_decay, norm)     # update_att_mlp2d_scnd (:152)
+        self.center_mlp = mlp(center_in, list(center_dim), bn_decay, norm) if center_in else None
         agg_c = C + (center_dim[-1] if (center_in and len(center_dim)) else (center_in or 0))
-        self.update_mlp = mlp(agg_c, list(out_dim), bn_decay) if len(out_dim) else None
+        self.update_mlp = mlp(agg_c, list(out_dim), bn_decay, norm) if len(out_dim) else None
         self.out_channels = out_dim[-1] if len(out_dim) else agg_c
 
     mfma_train = True   # training on the GPU: MLPs through csrc/gridgcn_train.hip

@@ -11,7 +11,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from . import ops, synth
-from .gridconv import ConvBNReLU, SubGUpdate, run_mlp
+from .gridconv import SubGUpdate, mlp, run_mlp
 
 # last linear layer + softmax cross-entropy on the hand-written kernels (GPU, float32)
 HEAD_KERNELS = True
@@ -135,13 +135,15 @@ class GGCNSeg(nn.Module):
         # int64 GPU scalar added to every sampling / dropout seed inside the kernels (None: off).
         # graph.GraphedTrainStep sets and bumps it so that replays of ONE captured step still redraw
         self.seed_dev = None
+        # cfg["norm"] = "group": every conv of the net normalised per cloud (gridconv.ConvGNAct) instead of per batch
+        norm = self.norm = cfg.get("norm", "batch")
         g = cfg["grid"]
         nd = len(g["down"])
         self.down = nn.ModuleList()
         feat_c = [0]                                   # channels (without the 4 loc dims) per level
         for i in range(nd):
             layer = SubGUpdate(cfg["inputDim"][i], cfg["pt_ele_dim"][i], cfg["localfdim"],
-                               cfg["relu"], bn_decay=cfg["bn_decay"])
+                               cfg["relu"], bn_decay=cfg["bn_decay"], norm=norm)
             self.down.append(layer)
             feat_c.append(layer.out_channels)
         self.up = nn.ModuleList()
@@ -150,11 +152,11 @@ class GGCNSeg(nn.Module):
             this_c = 4 + feat_c[nd - 1 - i]            # f_this_layer carries xyz,w too (:212)
             layer = SubGUpdate(last_c, cfg["up_pt_ele_dim"][i], cfg["localfdim"], cfg["relu"],
                                center_in=this_c, center_dim=cfg["up_center_dim"][i],
-                               out_dim=cfg["up_gcn_outDim"][i], bn_decay=cfg["bn_decay"])
+                               out_dim=cfg["up_gcn_outDim"][i], bn_decay=cfg["bn_decay"], norm=norm)
             self.up.append(layer)
             last_c = layer.out_channels
         # get_seg_head (:30-43)
-        self.fc1 = ConvBNReLU(last_c, 128, cfg["bn_decay"])
+        self.fc1 = mlp(last_c, [128], cfg["bn_decay"], norm)[0]
         # fc1 directly follows the last up layer's update MLP: one conv+BN+ReLU chain (see finish())
         self.fc2 = nn.Linear(128, cfg["num_classes"])
         nn.init.xavier_uniform_(self.fc2.weight)
@@ -173,7 +175,7 @@ class GGCNSeg(nn.Module):
         # the fused evaluation kernels return tensors without a grad_fn: eval() WITH grad enabled
         # (frozen-BatchNorm fine-tuning, saliency) must take the differentiable path
         return (self.fused and (not self.training) and (not torch.is_grad_enabled())
-                and _is_hip(self.ix))
+                and _is_hip(self.ix) and self.norm == "batch")
 
     def _seed(self, forward_no, call_no):
         if self.fixed_seed or not self.training:

@@ -550,3 +550,7 @@ def edge_inputs(src, nebidx, cent, *, has_feats, localfdim):
     _chk(nebidx, "nebidx", 3, torch.int32)
     _chk(cent, "cent", 3, torch.float32)
     return _EdgeInputs.apply(src, nebidx, cent, bool(has_feats), int(localfdim))
+
+
+# ---- batch-independent normalisation, 8-bit activation checkpoints (act8.py) ------------------------------------------
+from .act8 import act8_pack, act8_unpack, group_norm_act, linear_act8  # noqa: E402,F401

@@ -20,18 +20,20 @@ torch.compile / export:
     torch.ops.gridgcn.ball_knn(unknown, known, downnum, upnum, k=3, radius=0.1) -> idx
     torch.ops.gridgcn.knn(unknown, known, downnum, upnum, k=3) -> idx
     torch.ops.gridgcn.batch_take(data, index) -> out          (differentiable w.r.t. data)
+    torch.ops.gridgcn.act8_pack / act8_unpack / group_norm_act / linear_act8       (end of this file; not operators of
+                                                  the reference)
 
 Index ops have no autograd formula, as in the reference (gridify-inl.h:227-231, ball_k_nn.cc:60).
 GPU only: there is no CPU kernel (gridify.cc:28-39 is LOG(FATAL) in the reference as well).
 The reference's BallKNN/KNN leave rows >= upnum untouched in a caller-provided buffer; the
 functional ops return a fresh tensor whose untouched rows hold 0 (as grid_gcn_amd.ops does).
 """
-from typing import List, Tuple
+from typing import List, Optional, Tuple
 
 import torch
 from torch import Tensor
 
-from . import ops
+from . import act8, ops
 
 _lib_def = torch.library.custom_op
 
@@ -176,3 +178,138 @@ def _take_bwd(ctx, grad_out):
 
 
 batch_take.register_autograd(_take_bwd, setup_context=_take_setup)
+
+
+# ---- batch-independent normalisation and 8-bit activation checkpoints (act8.py) --------------------------------------
+#     torch.ops.gridgcn.act8_pack(x) -> (codes, scales)
+#     torch.ops.gridgcn.act8_unpack(codes, scales, C, dtype) -> x
+#     torch.ops.gridgcn.group_norm_act(x, weight, bias, groups, eps=1e-5, act="relu", counts=None, save8=False)
+#         -> (y, stats, codes, scales)         differentiable w.r.t. x, weight, bias through y; stats [B, groups, 2] f64
+#                                              (mean, rstd); codes, scales: empty without save8, rows >= counts unwritten
+#     torch.ops.gridgcn.linear_act8(x, weight, bias=None) -> (y, codes, scales)        differentiable through y
+@_lib_def("gridgcn::act8_pack", mutates_args=(), device_types="cuda")
+def act8_pack(x: Tensor) -> Tuple[Tensor, Tensor]:
+    return act8.act8_pack(x)
+
+
+@act8_pack.register_fake
+def _(x):
+    c, s = act8.act8_shapes(1, x.shape[-1])
+    return (x.new_empty(tuple(x.shape[:-1]) + c[1:], dtype=torch.uint8),
+            x.new_empty(tuple(x.shape[:-1]) + s[1:], dtype=torch.uint8))
+
+
+@_lib_def("gridgcn::act8_unpack", mutates_args=(), device_types="cuda")
+def act8_unpack(codes: Tensor, scales: Tensor, C: int, dtype: torch.dtype) -> Tensor:
+    return act8.act8_unpack(codes, scales, C, dtype)
+
+
+@act8_unpack.register_fake
+def _(codes, scales, C, dtype):
+    return codes.new_empty(tuple(codes.shape[:-1]) + (C,), dtype=dtype)
+
+
+@_lib_def("gridgcn::group_norm_act", mutates_args=(), device_types="cuda")
+def group_norm_act(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], groups: int, eps: float = 1e-5,
+                   act: str = "relu", counts: Optional[Tensor] = None,
+                   save8: bool = False) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    _, groups, ptype = act8._check_gn(x, weight, bias, groups, eps, act, counts)
+    act8._require(x.numel() > 0, "x must not be empty")
+    y, _, st, codes, scales = act8._gn_forward(x, weight, bias, groups, ptype, eps, act, counts, save8, True)
+    if not save8:
+        codes, scales = (torch.empty(0, dtype=torch.uint8, device=x.device) for _ in range(2))
+    return y, st, codes, scales
+
+
+@group_norm_act.register_fake
+def _(x, weight, bias, groups, eps=1e-5, act="relu", counts=None, save8=False):
+    c, s = act8.act8_shapes(x.numel() // x.shape[-1], x.shape[-1]) if save8 else ((0,), (0,))
+    return (torch.empty_like(x, memory_format=torch.contiguous_format),
+            x.new_empty((x.shape[0], groups, 2), dtype=torch.float64),
+            x.new_empty(c, dtype=torch.uint8), x.new_empty(s, dtype=torch.uint8))
+
+
+@_lib_def("gridgcn::group_norm_act_backward", mutates_args=(), device_types="cuda")
+def group_norm_act_backward(dy: Tensor, x: Optional[Tensor], codes: Optional[Tensor], scales: Optional[Tensor],
+                            stats: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], groups: int, act: str,
+                            counts: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
+    """(dx, dweight, dbias); the last two are empty where the parameter is None"""
+    _, groups, ptype = act8._check_gn(dy, weight, bias, groups, 0.0, act, counts)
+    B, C = dy.shape[0], dy.shape[-1]
+    act8._require(stats.dtype == torch.float64 and stats.is_contiguous() and tuple(stats.shape) == (B, groups, 2),
+                  "stats should be the contiguous float64 [B,groups,2] tensor of the forward")
+    if codes is not None:
+        act8._check_codes(codes, scales, dy.numel() // C, C)
+    else:
+        act8._require(x is not None and x.shape == dy.shape and x.dtype == dy.dtype, "x must have dy's shape and type")
+        x = act8._rows3(x, B)[0]
+    dx, dw, db = act8._gn_backward(dy, x, codes, scales, stats, weight, bias, tuple(dy.shape), groups, ptype, act, counts,
+                                   (True, weight is not None, bias is not None))
+    return dx, dy.new_empty(0) if dw is None else dw, dy.new_empty(0) if db is None else db
+
+
+@group_norm_act_backward.register_fake
+def _(dy, x, codes, scales, stats, weight, bias, groups, act, counts=None):
+    return (torch.empty_like(dy, memory_format=torch.contiguous_format),
+            dy.new_empty(0) if weight is None else torch.empty_like(weight), dy.new_empty(0) if bias is None else torch.empty_like(bias))
+
+
+def _gn_setup(ctx, inputs, output):
+    x, weight, bias, groups, eps, act, counts, save8 = inputs
+    _, st, codes, scales = output
+    ctx.save_for_backward(None if save8 else x, codes if save8 else None, scales if save8 else None, st, weight, bias, counts)
+    ctx.gn = (groups, act)
+
+
+def _gn_bwd(ctx, dy, *_):
+    x, codes, scales, st, weight, bias, counts = ctx.saved_tensors
+    dx, dw, db = torch.ops.gridgcn.group_norm_act_backward(dy, x, codes, scales, st, weight, bias, *ctx.gn, counts)
+    return dx, None if weight is None else dw, None if bias is None else db, None, None, None, None, None
+
+
+group_norm_act.register_autograd(_gn_bwd, setup_context=_gn_setup)
+
+
+@_lib_def("gridgcn::linear_act8", mutates_args=(), device_types="cuda")
+def linear_act8(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
+    act8._check_linear(x, weight, bias)
+    act8._require(x.numel() > 0, "x must not be empty")
+    return act8._linear_forward(x, weight, bias, True)
+
+
+@linear_act8.register_fake
+def _(x, weight, bias=None):
+    c, s = act8.act8_shapes(x.numel() // x.shape[-1], x.shape[-1])
+    return (x.new_empty(tuple(x.shape[:-1]) + (weight.shape[0],)), x.new_empty(c, dtype=torch.uint8),
+            x.new_empty(s, dtype=torch.uint8))
+
+
+@_lib_def("gridgcn::linear_act8_backward", mutates_args=(), device_types="cuda")
+def linear_act8_backward(dy: Tensor, weight: Tensor, codes: Tensor, scales: Tensor) -> Tuple[Tensor, Tensor, Tensor]:
+    """(dx, dweight, dbias)"""
+    act8._check_rows(dy, "dy")
+    N, K = weight.shape
+    act8._require(weight.dtype == dy.dtype and weight.device == dy.device and dy.shape[-1] == N, "weight should be [%d, K] of dy's type" % dy.shape[-1])
+    act8._check_codes(codes, scales, dy.numel() // N, K)
+    return act8._linear_backward(dy, weight, codes, scales, tuple(dy.shape[:-1]) + (K,), (True, True, True))
+
+
+@linear_act8_backward.register_fake
+def _(dy, weight, codes, scales):
+    return (dy.new_empty(tuple(dy.shape[:-1]) + (weight.shape[1],)), torch.empty_like(weight), dy.new_empty(weight.shape[0]))
+
+
+def _lin8_setup(ctx, inputs, output):
+    x, weight, bias = inputs
+    _, codes, scales = output
+    ctx.save_for_backward(weight, codes, scales)
+    ctx.has_bias = bias is not None
+
+
+def _lin8_bwd(ctx, dy, *_):
+    weight, codes, scales = ctx.saved_tensors
+    dx, dw, db = torch.ops.gridgcn.linear_act8_backward(dy, weight, codes, scales)
+    return dx, dw, db if ctx.has_bias else None
+
+
+linear_act8.register_autograd(_lin8_bwd, setup_context=_lin8_setup)

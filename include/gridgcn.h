@@ -831,6 +831,63 @@ int gridgcn_gridconv_forward(const float *src, const int32_t *nebidx, const floa
                              int has_feats, int localfdim, int npt, const gridgcn_conv_layer *pt,
                              const gridgcn_conv_layer *att, float *out, void *stream);
 
+/* ---- batch-independent normalisation and 8-bit activation checkpoints ---------------------------------------
+ * Rows of float32, bfloat16 or float16 (GRIDGCN_F32 / _BF16 / _F16), channels contiguous, any row stride in ELEMENTS
+ * >= the number of channels, aligned to an element.
+ *
+ * The 8-bit form of a row of C channels: Cp = C rounded up to 32; codes[Cp] (e4m3, zeros behind C) and scales[Cp / 32]:
+ *   32 consecutive channels share the power of two 2^(scale - 127), the smallest with max |x| <= 448 * 2^(scale - 127)
+ *   (finite values only; scale >= 10); a channel is the e4m3 number nearest to x / 2^(scale - 127), ties to even.
+ *   Infinities and NaN become NaN.  A value is exact in bf16, and in fp16 if x was fp16; a magnitude above 3.29e38
+ *   rounds to 2^128, which float32 and bf16 read as infinite.
+ * gridgcn_act8_pack / _unpack: x[R][ldx] -> codes[R][Cp], scales[R][Cp / 32], and back.  codes 16-byte aligned.
+ *
+ * gridgcn_group_norm_act_fwd: x[B][N][C] (strides ldb, ldn), G groups of C / G channels; per (b, group) mean and
+ *   variance over the rows n < counts[b] (clamped to [0, N]; NULL: all N) and the group's channels;
+ *     y[b][n][c] = act((x - mean) / sqrt(var + eps) * gamma[c] + beta[c]), contiguous;  0 in rows n >= counts[b], whose
+ *   x is not read.  gamma, beta (either may be NULL: 1 / 0): C values of type ptype.  stats (optional): fp64 [B][G][2]
+ *   mean, 1 / sqrt(var + eps).  codes, scales (both or neither): the 8-bit form of x, rows b * N + n; rows
+ *   n >= counts[b] are left as they were.
+ * gridgcn_group_norm_act_bwd: from dy[B][N][C] (strides ldgb, ldgn), the forward's stats and x -- or codes and scales in
+ *   its place, the statistics staying those of the forward: dx (contiguous, type of x), dgamma, dbeta (ptype); any of
+ *   the three may be NULL.  Rows n >= counts[b]: dx = 0, dy not read.
+ *
+ * gridgcn_linear_act8_fwd: y[R][N] = x[R][K] W[N][K]^T + bias[N] (bias may be NULL), all of one type, products summed in
+ *   fp32 (float32 operands: each as three bf16 numbers, six products: the error of an fp32 product; an infinite operand
+ *   gives NaN), and codes / scales (both or neither) the 8-bit form of x.
+ * gridgcn_linear_act8_bwd: dx[R][K] = dy W;  dW[N][K] = dy^T x^ with x^ the values of codes / scales;  dbias[N] = sum of
+ *   dy; any of them may be NULL (codes, scales only for dW; W only for dx).
+ * Sums have one order: the same call gives the same bits. */
+#define GRIDGCN_F32 0
+#define GRIDGCN_BF16 1
+#define GRIDGCN_F16 2
+#define GRIDGCN_ACT_NONE 0
+#define GRIDGCN_ACT_RELU 1
+#define GRIDGCN_ACT_SILU 2
+#define GRIDGCN_ACT_GELU 3       /* t/2 (1 + erf(t / sqrt 2)) */
+#define GRIDGCN_ACT8_MAX_C 65536 /* channels of a row in the 8-bit form */
+#define GRIDGCN_GN_MAX_C 8192    /* channels of gridgcn_group_norm_act_* */
+int gridgcn_act8_pack(const void *x, int dtype, long long R, int C, long long ldx, uint8_t *codes,
+                      uint8_t *scales, void *stream);
+int gridgcn_act8_unpack(const uint8_t *codes, const uint8_t *scales, long long R, int C, int dtype, void *x,
+                        long long ldx, void *stream);
+int gridgcn_group_norm_act_workspace_bytes(int B, long long N, int C, int G, int dtype, int save8, size_t *bytes);
+int gridgcn_group_norm_act_fwd(const void *x, int dtype, int B, long long N, int C, long long ldb, long long ldn,
+                               int G, const void *gamma, const void *beta, int ptype, const int32_t *counts,
+                               float eps, int act, void *y, double *stats, uint8_t *codes, uint8_t *scales,
+                               void *ws, size_t ws_bytes, void *stream);
+int gridgcn_group_norm_act_bwd(const void *dy, long long ldgb, long long ldgn, const void *x, long long ldb,
+                               long long ldn, const uint8_t *codes, const uint8_t *scales, int dtype, int B,
+                               long long N, int C, int G, const double *stats, const void *gamma,
+                               const void *beta, int ptype, const int32_t *counts, int act, void *dx,
+                               void *dgamma, void *dbeta, void *ws, size_t ws_bytes, void *stream);
+int gridgcn_linear_act8_fwd(const void *x, int dtype, long long R, int K, long long ldx, const void *W,
+                            const void *bias, int N, void *y, uint8_t *codes, uint8_t *scales, void *stream);
+int gridgcn_linear_act8_bwd_workspace_bytes(long long R, int K, int N, size_t *bytes);
+int gridgcn_linear_act8_bwd(const void *dy, int dtype, long long R, int N, long long ldy, const void *W, int K,
+                            const uint8_t *codes, const uint8_t *scales, void *dx, void *dW, void *dbias,
+                            void *ws, size_t ws_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

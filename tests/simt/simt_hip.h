@@ -552,6 +552,66 @@ template <class V> SIMT_NOSAN static SIMT_INL simt_f32x16 simt_mfma_f32_32x32x16
 }
 #define __builtin_amdgcn_mfma_f32_32x32x16_bf16 simt_mfma_f32_32x32x16_bf16
 
+// v_mfma_f32_32x32x16_f16: as the bf16 form, fp16 operands
+template <class V> SIMT_NOSAN static SIMT_INL simt_f32x16 simt_mfma_f32_32x32x16_f16(V a, V b, simt_f32x16 c, int, int, int)
+{
+    static_assert(sizeof(V) == 16, "fp16x8 operands");
+    memcpy(simt_cur->wide, &a, 16);
+    memcpy(simt_cur->wide + 2, &b, 16);
+    (void)simt_collective(SIMT_OP_XCHG, 0, 0, 64);
+    const int l = simt_cur->lane, col = l & 31, h = l >> 5;
+    _Float16 bk[16];
+    memcpy(bk, &simt_xchg_wide[col][2], 16);
+    memcpy(bk + 8, &simt_xchg_wide[col + 32][2], 16);
+    if (!simt_xchg_in[col] || !simt_xchg_in[col + 32]) simt_foreign_reads++;
+    for (int r = 0; r < 16; r++) {
+        const int row = (r & 3) + 8 * (r >> 2) + 4 * h;
+        _Float16 ak[16];
+        memcpy(ak, &simt_xchg_wide[row][0], 16);
+        memcpy(ak + 8, &simt_xchg_wide[row + 32][0], 16);
+        if (!simt_xchg_in[row] || !simt_xchg_in[row + 32]) simt_foreign_reads++;
+        float acc = c[r];
+        for (int k = 0; k < 16; k++) acc = __builtin_fmaf((float)ak[k], (float)bk[k], acc);
+        c[r] = acc;
+    }
+    return c;
+}
+#define __builtin_amdgcn_mfma_f32_32x32x16_f16 simt_mfma_f32_32x32x16_f16
+
+// e4m3 (no infinities; 0x7f / 0xff NaN): v_cvt_pk_fp8_f32 to nearest even, v_cvt_pk_f32_fp8
+static inline uint8_t simt_f32_to_e4m3(float x)
+{
+    const uint8_t sign = std::signbit(x) ? 0x80 : 0;
+    const double a = std::fabs((double)x);
+    if (!(a <= 448.0)) return sign | (a < 464.0 ? 0x7e : 0x7f);       // (464 = halfway to the number behind 448: even is NaN's code)
+    int e = -6;
+    if (a >= 0.015625) std::frexp(a, &e), e -= 1;
+    const double q = std::nearbyint(std::ldexp(a, 3 - e));              // in units of 2^(e - 3)
+    int m = (int)q;
+    if (m == 16) { m = 8; e++; }
+    return sign | (uint8_t)(m < 8 ? m : ((e + 7) << 3) | (m - 8));
+}
+static inline float simt_e4m3_to_f32(uint8_t b)
+{
+    const int e = (b >> 3) & 15, m = b & 7;
+    double v = (b & 0x7f) == 0x7f ? NAN : e == 0 ? std::ldexp((double)m, -9) : std::ldexp(8.0 + m, e - 10);
+    return (float)((b & 0x80) ? -v : v);
+}
+static inline int simt_cvt_pk_fp8_f32(float a, float b, int old, bool high)
+{
+    const unsigned w = simt_f32_to_e4m3(a) | ((unsigned)simt_f32_to_e4m3(b) << 8);
+    return (int)(high ? ((unsigned)old & 0xffffu) | (w << 16) : ((unsigned)old & 0xffff0000u) | w);
+}
+typedef float simt_f32x2 __attribute__((ext_vector_type(2)));
+static inline simt_f32x2 simt_cvt_pk_f32_fp8(int w, bool high)
+{
+    const unsigned u = high ? (unsigned)w >> 16 : (unsigned)w;
+    return simt_f32x2{simt_e4m3_to_f32((uint8_t)u), simt_e4m3_to_f32((uint8_t)(u >> 8))};
+}
+#define __builtin_amdgcn_cvt_pk_fp8_f32 simt_cvt_pk_fp8_f32
+#define __builtin_amdgcn_cvt_pk_f32_fp8 simt_cvt_pk_f32_fp8
+#define __expf expf                                                    // (the GPU's: exp2 of a rounded product)
+
 static inline float rsqrtf(float x) { return 1.0f / sqrtf(x); }   // (the GPU's is an approximation within 1 ulp)
 static inline int __popc(unsigned x) { return __builtin_popcount(x); }
 static inline int __popcll(unsigned long long x) { return __builtin_popcountll(x); }
