@@ -332,7 +332,7 @@ def declare(lib, path="<library>"):
     lib.gridgcn_act8_unpack.restype = ci
     lib.gridgcn_act8_unpack.argtypes = [vp, vp, ll, ci, ci, vp, ll, vp]
     lib.gridgcn_group_norm_act_workspace_bytes.restype = ci
-    lib.gridgcn_group_norm_act_workspace_bytes.argtypes = [ci, ll, ci, ci, ci, ci, ctypes.POINTER(cs)]
+    lib.gridgcn_group_norm_act_workspace_bytes.argtypes = [ci, ll, ci, ci, ci, ci, ci, ci, ctypes.POINTER(cs)]
     lib.gridgcn_group_norm_act_fwd.restype = ci
     lib.gridgcn_group_norm_act_fwd.argtypes = [vp, ci, ci, ll, ci, ll, ll, ci, vp, vp, ci, vp, cf, ci, vp, vp, vp, vp,
                                                vp, cs, vp]

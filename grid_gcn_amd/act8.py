@@ -8,7 +8,9 @@ forward and backward (csrc/gridgcn_act8.h, gridgcn_gnorm.hip, gridgcn_lin8.hip).
 
 Rows are float32, bfloat16 or float16 GPU tensors; the last axis (channels) must be contiguous, rows may be strided
 (columns of a wider buffer) -- anything else is copied first.  Errors raise RuntimeError, as in ops.py."""
+import contextlib
 import ctypes
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -20,6 +22,7 @@ ACTS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}                   # GRIDGCN_
 ACT8_BLOCK = 32
 ACT8_MAX_C = 65536
 GN_MAX_C = 8192
+MAX_LD = 1 << 24                  # row strides above it are copied together first (32-bit offsets inside a tile of rows)
 
 
 def _require(cond, msg):
@@ -27,12 +30,27 @@ def _require(cond, msg):
         raise RuntimeError(msg)
 
 
+# The host's share of a small call is most of it (a training step of 32 rows: 160 us, of which 20 on the GPU): no context
+# manager where the device is the current one, no stream object, no query of a size that was asked before.
 def _p(t):
     return t.data_ptr() if t is not None else None
 
 
 def _st(t):
-    return torch.cuda.current_stream(t.device).cuda_stream
+    i = t.device.index
+    return torch._C._cuda_getCurrentRawStream(i) if i is not None else torch.cuda.current_stream(t.device).cuda_stream
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(dev):
+    return _HERE if dev.index is None or dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _packed(t):
+    """a parameter as the kernels read it: contiguous (its pointer is all they get)"""
+    return t if t is None or t.is_contiguous() else t.detach().contiguous()
 
 
 def _check_rows(t, name, min_dim=1):
@@ -45,8 +63,9 @@ def _check_rows(t, name, min_dim=1):
 def _rows2(t):
     """[..., C] -> ([R, C] with contiguous channels and rows that do not overlap, row stride in elements)"""
     C = t.shape[-1]
-    t = t.reshape(-1, C)
-    if (C > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < C):
+    if t.dim() != 2:
+        t = t.reshape(-1, C)
+    if (C > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and not C <= t.stride(0) <= MAX_LD):
         t = t.contiguous()
     return t, (t.stride(0) if t.shape[0] > 1 else C)
 
@@ -54,9 +73,10 @@ def _rows2(t):
 def _rows3(t, B):
     """[B, ..., C] -> ([B, N, C], cloud stride, row stride), channels contiguous"""
     C = t.shape[-1]
-    t = t.reshape(B, -1, C)
+    if t.dim() != 3:
+        t = t.reshape(B, -1, C)
     N = t.shape[1]
-    if (C > 1 and t.stride(2) != 1) or (N > 1 and t.stride(1) < C):
+    if (C > 1 and t.stride(2) != 1) or (N > 1 and not C <= t.stride(1) <= MAX_LD):
         t = t.contiguous()
     return t, (t.stride(0) if B > 1 else 0), (t.stride(1) if N > 1 else C)
 
@@ -85,7 +105,7 @@ def act8_pack(x):
     R = x2.shape[0]
     codes, scales = _new_act8(R, C, x.device)
     if R:
-        with torch.cuda.device(x.device):
+        with _on(x.device):
             rc = _lib.load().gridgcn_act8_pack(_p(x2), _DTYPES[x.dtype], R, C, ld, _p(codes), _p(scales), _st(x))
         _lib.check(rc, "gridgcn_act8_pack")
     return codes.view(lead + (codes.shape[1],)), scales.view(lead + (scales.shape[1],))
@@ -103,7 +123,7 @@ def act8_unpack(codes, scales, C, dtype=torch.float32):
     x = torch.empty(lead + (C,), dtype=dtype, device=codes.device)
     R = x.numel() // C
     if R:
-        with torch.cuda.device(codes.device):
+        with _on(codes.device):
             rc = _lib.load().gridgcn_act8_unpack(_p(codes), _p(scales), R, C, _DTYPES[dtype], _p(x), C, _st(codes))
         _lib.check(rc, "gridgcn_act8_unpack")
     return x
@@ -121,6 +141,13 @@ def _check_codes(codes, scales, rows, C):
 
 
 # ---- group normalisation + activation -------------------------------------------------------------------------------
+def _check_param(t, name, x, C):
+    _require(isinstance(t, torch.Tensor) and t.device == x.device and t.dim() == 1 and t.shape[0] == C,
+             "%s should be a [%d] tensor on the device of x" % (name, C))
+    _require(t.dtype == torch.float32 or t.dtype == x.dtype, "%s must be float32 or of x's type" % name)
+    return t.dtype
+
+
 def _check_gn(x, weight, bias, groups, eps, act, counts):
     _check_rows(x, "x", 2)
     C = x.shape[-1]
@@ -128,30 +155,29 @@ def _check_gn(x, weight, bias, groups, eps, act, counts):
     _require(1 <= C <= GN_MAX_C, "x must have 1..%d channels" % GN_MAX_C)
     _require(x.shape[0] <= 65535, "x may have at most 65535 samples")
     _require(groups >= 1 and C % groups == 0, "%d channels cannot be cut into %d groups" % (C, groups))
-    _require(act in ACTS, "act must be one of %s" % ", ".join(ACTS))
-    _require(0.0 <= float(eps) < float("inf"), "eps must be finite and >= 0")
-    ptype = None
-    for t, name in ((weight, "weight"), (bias, "bias")):
-        if t is None:
-            continue
-        _require(isinstance(t, torch.Tensor) and t.device == x.device and tuple(t.shape) == (C,),
-                 "%s should be a [%d] tensor on the device of x" % (name, C))
-        _require(t.dtype == torch.float32 or t.dtype == x.dtype, "%s must be float32 or of x's type" % name)
-        _require(ptype is None or t.dtype == ptype, "weight and bias must have one type")
-        ptype = t.dtype
+    _require(act in ACTS, "act must be one of none, relu, silu, gelu")
+    _require(0.0 <= eps < float("inf"), "eps must be finite and >= 0")
+    ptype = torch.float32
+    if weight is not None:
+        ptype = _check_param(weight, "weight", x, C)
+    if bias is not None:
+        t = _check_param(bias, "bias", x, C)
+        _require(weight is None or t == ptype, "weight and bias must have one type")
+        ptype = t
     if counts is not None:
         _require(isinstance(counts, torch.Tensor) and counts.device == x.device and counts.dtype == torch.int32,
                  "counts must be an int32 tensor on the device of x")
         _require(x.dim() == 3, "counts need x as [B, N, C]")
         _require(counts.numel() == x.shape[0] and counts.is_contiguous(), "counts should be a [B,1] tensor")
-    return C, groups, _DTYPES[ptype if ptype is not None else torch.float32]
+    return C, groups, _DTYPES[ptype]
 
 
-def _gn_workspace(lib, B, N, C, groups, dt, save8, dev):
+@functools.lru_cache(maxsize=1024)
+def _gn_workspace_bytes(B, N, C, groups, dt, save8, stats, backward):
     nb = ctypes.c_size_t(0)
-    _lib.check(lib.gridgcn_group_norm_act_workspace_bytes(B, N, C, groups, dt, int(save8), ctypes.byref(nb)),
+    _lib.check(_lib.load().gridgcn_group_norm_act_workspace_bytes(B, N, C, groups, dt, save8, stats, backward, ctypes.byref(nb)),
                "gridgcn_group_norm_act_workspace_bytes")
-    return torch.empty(nb.value, dtype=torch.uint8, device=dev), nb.value
+    return nb.value
 
 
 def _gn_forward(x, weight, bias, groups, ptype, eps, act, counts, save8, stats):
@@ -160,15 +186,15 @@ def _gn_forward(x, weight, bias, groups, ptype, eps, act, counts, save8, stats):
     B, C = x.shape[0], x.shape[-1]
     x3, sb, sn = _rows3(x, B)
     N, dt = x3.shape[1], _DTYPES[x.dtype]
-    with torch.cuda.device(dev):
+    nb = _gn_workspace_bytes(B, N, C, groups, dt, int(save8), int(stats), 0)
+    with _on(dev):
         y = torch.empty(x.shape, dtype=x.dtype, device=dev)
         st = torch.empty((B, groups, 2), dtype=torch.float64, device=dev) if stats else None
         codes, scales = _new_act8(B * N, C, dev) if save8 else (None, None)
-        ws, nb = _gn_workspace(lib, B, N, C, groups, dt, save8, dev)
-        w = weight.detach().contiguous() if weight is not None else None
-        b = bias.detach().contiguous() if bias is not None else None
-        rc = lib.gridgcn_group_norm_act_fwd(_p(x3), dt, B, N, C, sb, sn, groups, _p(w), _p(b), ptype, _p(counts), float(eps),
-                                            ACTS[act], _p(y), _p(st), _p(codes), _p(scales), _p(ws), nb, _st(x))
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+        w, b = _packed(weight), _packed(bias)
+        rc = lib.gridgcn_group_norm_act_fwd(x3.data_ptr(), dt, B, N, C, sb, sn, groups, _p(w), _p(b), ptype, _p(counts), eps,
+                                            ACTS[act], y.data_ptr(), _p(st), _p(codes), _p(scales), _p(ws), nb, _st(x))
     _lib.check(rc, "gridgcn_group_norm_act_fwd")
     return y, x3, st, codes, scales
 
@@ -182,16 +208,16 @@ def _gn_backward(dy, x3, codes, scales, stats, weight, bias, shape, groups, ptyp
     xb = xn = 0
     if codes is None:
         xb, xn = (x3.stride(0) if B > 1 else 0), (x3.stride(1) if N > 1 else C)
-    with torch.cuda.device(dev):
+    nb = _gn_workspace_bytes(B, N, C, groups, dt, 0, 1, 1)
+    with _on(dev):
         dx = torch.empty(shape, dtype=dy.dtype, device=dev) if need[0] else None
         dw = torch.empty(C, dtype=weight.dtype, device=dev) if need[1] else None
         db = torch.empty(C, dtype=bias.dtype, device=dev) if need[2] else None
-        ws, nb = _gn_workspace(lib, B, N, C, groups, dt, False, dev)
-        w = weight.detach().contiguous() if weight is not None else None
-        b = bias.detach().contiguous() if bias is not None else None
-        rc = lib.gridgcn_group_norm_act_bwd(_p(g3), gb, gn, _p(x3), xb, xn, _p(codes), _p(scales), dt, B, N, C, groups,
-                                            _p(stats), _p(w), _p(b), ptype, _p(counts), ACTS[act], _p(dx), _p(dw), _p(db),
-                                            _p(ws), nb, _st(dy))
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+        w, b = _packed(weight), _packed(bias)
+        rc = lib.gridgcn_group_norm_act_bwd(g3.data_ptr(), gb, gn, _p(x3), xb, xn, _p(codes), _p(scales), dt, B, N, C, groups,
+                                            stats.data_ptr(), _p(w), _p(b), ptype, _p(counts), ACTS[act], _p(dx), _p(dw),
+                                            _p(db), _p(ws), nb, _st(dy))
     _lib.check(rc, "gridgcn_group_norm_act_bwd")
     return dx, dw, db
 
@@ -224,6 +250,7 @@ def group_norm_act(x, weight, bias, groups, eps=1e-5, act="relu", counts=None, s
     save8: keep x for the backward in 8 bits (act8_pack) instead of x itself: 1.03 bytes a value.  The gradients are then those of
     the formulas at the 8-bit values of x, with the statistics of x.
     Not differentiable twice."""
+    eps = float(eps)
     C, groups, ptype = _check_gn(x, weight, bias, groups, eps, act, counts)
     if x.numel() == 0:
         y = x * 0
@@ -232,7 +259,7 @@ def group_norm_act(x, weight, bias, groups, eps=1e-5, act="relu", counts=None, s
         return y
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad)):
-        return _GroupNormAct.apply(x, weight, bias, counts, groups, ptype, float(eps), act, bool(save8))
+        return _GroupNormAct.apply(x, weight, bias, counts, groups, ptype, eps, act, bool(save8))
     return _gn_forward(x, weight, bias, groups, ptype, eps, act, counts, False, False)[0]
 
 
@@ -256,14 +283,21 @@ def _linear_forward(x, weight, bias, save8):
     N, K = weight.shape
     x2, ld = _rows2(x)
     R = x2.shape[0]
-    with torch.cuda.device(dev):
+    with _on(dev):
         y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=dev)
         codes, scales = _new_act8(R, K, dev) if save8 else (None, None)
-        w = weight.detach().contiguous()
-        b = bias.detach().contiguous() if bias is not None else None
-        rc = lib.gridgcn_linear_act8_fwd(_p(x2), _DTYPES[x.dtype], R, K, ld, _p(w), _p(b), N, _p(y), _p(codes), _p(scales), _st(x))
+        w, b = _packed(weight), _packed(bias)
+        rc = lib.gridgcn_linear_act8_fwd(x2.data_ptr(), _DTYPES[x.dtype], R, K, ld, w.data_ptr(), _p(b), N, y.data_ptr(), _p(codes),
+                                         _p(scales), _st(x))
     _lib.check(rc, "gridgcn_linear_act8_fwd")
     return y, codes, scales
+
+
+@functools.lru_cache(maxsize=1024)
+def _linear_workspace_bytes(R, K, N):
+    nb = ctypes.c_size_t(0)
+    _lib.check(_lib.load().gridgcn_linear_act8_bwd_workspace_bytes(R, K, N, ctypes.byref(nb)), "gridgcn_linear_act8_bwd_workspace_bytes")
+    return nb.value
 
 
 def _linear_backward(dy, weight, codes, scales, x_shape, need):
@@ -272,19 +306,15 @@ def _linear_backward(dy, weight, codes, scales, x_shape, need):
     N, K = weight.shape
     g2, ld = _rows2(dy)
     R = g2.shape[0]
-    with torch.cuda.device(dev):
+    nb = _linear_workspace_bytes(R, K, N) if need[1] or need[2] else 0
+    with _on(dev):
         dx = torch.empty(x_shape, dtype=dy.dtype, device=dev) if need[0] else None
         dw = torch.empty((N, K), dtype=dy.dtype, device=dev) if need[1] else None
         db = torch.empty(N, dtype=dy.dtype, device=dev) if need[2] else None
-        ws, nb = None, 0
-        if need[1] or need[2]:
-            n = ctypes.c_size_t(0)
-            _lib.check(lib.gridgcn_linear_act8_bwd_workspace_bytes(R, K, N, ctypes.byref(n)), "gridgcn_linear_act8_bwd_workspace_bytes")
-            nb = n.value
-            ws = torch.empty(nb, dtype=torch.uint8, device=dev)
-        w = weight.detach().contiguous() if need[0] else None
-        rc = lib.gridgcn_linear_act8_bwd(_p(g2), _DTYPES[dy.dtype], R, N, ld, _p(w), K, _p(codes), _p(scales), _p(dx), _p(dw),
-                                         _p(db), _p(ws), nb, _st(dy))
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+        w = _packed(weight) if need[0] else None
+        rc = lib.gridgcn_linear_act8_bwd(g2.data_ptr(), _DTYPES[dy.dtype], R, N, ld, _p(w), K, _p(codes), _p(scales), _p(dx),
+                                         _p(dw), _p(db), _p(ws), nb, _st(dy))
     _lib.check(rc, "gridgcn_linear_act8_bwd")
     return dx, dw, db
 

@@ -29,6 +29,8 @@ typedef unsigned gg_u32x2 __attribute__((ext_vector_type(2)));
 typedef gg_u32x4 gg_u32x4_a4 __attribute__((aligned(4)));
 typedef gg_u32x4 gg_u32x4_a2 __attribute__((aligned(2)));
 typedef gg_u32x2 gg_u32x2_a2 __attribute__((aligned(2)));
+typedef gg_u32x2 gg_u32x2_a4 __attribute__((aligned(4)));
+typedef unsigned gg_u32_a2 __attribute__((aligned(2)));
 
 __device__ __forceinline__ float gg_lo16f(unsigned u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float gg_hi16f(unsigned u) { return __uint_as_float(u & 0xffff0000u); }
@@ -132,6 +134,37 @@ template <class T> __device__ __forceinline__ void gg_st_chunk(T *row, int c, in
     }
 }
 
+// the same chunk as it stands in memory: 4 registers until it is used
+template <class T> struct GGChunk {
+    gg_u32x4 w;
+    __device__ __forceinline__ void load(const T *row, int c, int C)
+    {
+        constexpr int V = GGRowT<T>::V;
+        if (c + V <= C) {
+            if constexpr (V == 4) w = *(const gg_u32x4_a4 *)(row + c);
+            else w = *(const gg_u32x4_a2 *)(row + c);
+        } else {
+            w = gg_u32x4{0u, 0u, 0u, 0u};
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                if (c + i >= C) continue;
+                if constexpr (V == 4) w[i] = ((const unsigned *)row)[c + i];
+                else w[i / 2] |= (unsigned)((const unsigned short *)row)[c + i] << (16 * (i & 1));
+            }
+        }
+    }
+    __device__ __forceinline__ void zero() { w = gg_u32x4{0u, 0u, 0u, 0u}; }
+    __device__ __forceinline__ void get(float (&v)[GGRowT<T>::V]) const
+    {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if constexpr (GGRowT<T>::id == GG_T_F32) v[i] = __uint_as_float(w[i]);
+            else if constexpr (GGRowT<T>::id == GG_T_BF16) { v[2 * i] = gg_lo16f(w[i]); v[2 * i + 1] = gg_hi16f(w[i]); }
+            else { v[2 * i] = gg_f16of(w[i], 0); v[2 * i + 1] = gg_f16of(w[i], 1); }
+        }
+    }
+};
+
 // a parameter vector of either type; none: the given value
 __device__ __forceinline__ float gg_ld_param(const void *p, int ptype, int i, float none)
 {
@@ -186,45 +219,85 @@ __device__ __forceinline__ void gg_a8_dec4(unsigned w, float &a, float &b, float
     a = lo[0]; b = lo[1]; c = hi[0]; d = hi[1];
 }
 
-// V channels of one block, the other 32 / V - 1 lanes of the block beside this one: encode them.  Every lane of the wave
-// takes part (lanes without data pass zeros).
-template <int V> __device__ __forceinline__ unsigned gg_a8_block_byte(const float (&v)[V])
+// V channels of one block, the other 32 / V - 1 lanes of the block beside this one: its scale byte.  Every lane of the wave
+// takes part (lanes without data pass zeros).  clean: no value of the WAVE is infinite or NaN, which saves the tests on each
+// (the largest bit pattern tells); where one is, all lanes look again at the finite ones only.
+template <int V> __device__ __forceinline__ unsigned gg_a8_block_max(unsigned m)
 {
-    unsigned m = 0;
-#pragma unroll
-    for (int i = 0; i < V; i++) {
-        const unsigned u = gg_a8_mag(v[i]);
-        m = m > u ? m : u;
-    }
 #pragma unroll
     for (int d = 1; d < GG_A8_BLOCK / V; d *= 2) {
         const unsigned o = (unsigned)__shfl_xor((int)m, d);
         m = m > o ? m : o;
     }
+    return m;
+}
+template <int V> __device__ __forceinline__ unsigned gg_a8_block_byte(const float (&v)[V], bool &clean)
+{
+    unsigned m = 0;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const unsigned u = __float_as_uint(v[i]) & 0x7fffffffu;
+        m = m > u ? m : u;
+    }
+    m = gg_a8_block_max<V>(m);
+    clean = !__any(m >= 0x7f800000u);
+    if (!clean) {
+        m = 0;
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const unsigned u = gg_a8_mag(v[i]);
+            m = m > u ? m : u;
+        }
+        m = gg_a8_block_max<V>(m);
+    }
     return gg_a8_byte(m);
 }
-template <int V> __device__ __forceinline__ void gg_a8_encode(const float (&v)[V], unsigned byte, unsigned (&w)[V / 4])
+template <int V> __device__ __forceinline__ void gg_a8_encode(const float (&v)[V], unsigned byte, bool clean, unsigned (&w)[V / 4])
 {
     const float s = gg_a8_unscale(byte);
+    if (clean) {
 #pragma unroll
-    for (int i = 0; i < V / 4; i++)
-        w[i] = gg_a8_enc4(gg_a8_ready(v[4 * i], s), gg_a8_ready(v[4 * i + 1], s), gg_a8_ready(v[4 * i + 2], s), gg_a8_ready(v[4 * i + 3], s));
+        for (int i = 0; i < V / 4; i++) w[i] = gg_a8_enc4(v[4 * i] * s, v[4 * i + 1] * s, v[4 * i + 2] * s, v[4 * i + 3] * s);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V / 4; i++)
+            w[i] = gg_a8_enc4(gg_a8_ready(v[4 * i], s), gg_a8_ready(v[4 * i + 1], s), gg_a8_ready(v[4 * i + 2], s), gg_a8_ready(v[4 * i + 3], s));
+    }
 }
 template <int V> __device__ __forceinline__ void gg_a8_st_codes(uint8_t *p, const unsigned (&w)[V / 4])
 {
     if constexpr (V == 4) *(unsigned *)p = w[0];
     else *(gg_u32x2 *)p = gg_u32x2{w[0], w[1]};
 }
-template <int V> __device__ __forceinline__ void gg_a8_ld(const uint8_t *codes, unsigned byte, float (&v)[V])
-{
-    unsigned w[V / 4];
-    if constexpr (V == 4) w[0] = *(const unsigned *)codes;
-    else { const gg_u32x2 u = *(const gg_u32x2 *)codes; w[0] = u[0]; w[1] = u[1]; }
-    const float s = gg_a8_scale(byte);
-#pragma unroll
-    for (int i = 0; i < V / 4; i++) {
-        float a, b, c, d;
-        gg_a8_dec4(w[i], a, b, c, d);
-        v[4 * i] = a * s; v[4 * i + 1] = b * s; v[4 * i + 2] = c * s; v[4 * i + 3] = d * s;
+// V channels of a block as they stand in memory
+template <int V> struct GGCodes {
+    unsigned w[V / 4], byte;
+    __device__ __forceinline__ void load(const uint8_t *codes, const uint8_t *scale)
+    {
+        if constexpr (V == 4) w[0] = *(const unsigned *)codes;
+        else { const gg_u32x2 u = *(const gg_u32x2 *)codes; w[0] = u[0]; w[1] = u[1]; }
+        byte = *scale;
     }
+    __device__ __forceinline__ void zero()
+    {
+#pragma unroll
+        for (int i = 0; i < V / 4; i++) w[i] = 0u;
+        byte = GG_A8_MIN_BYTE;
+    }
+    __device__ __forceinline__ void get(float (&v)[V]) const
+    {
+        const float s = gg_a8_scale(byte);
+#pragma unroll
+        for (int i = 0; i < V / 4; i++) {
+            float a, b, c, d;
+            gg_a8_dec4(w[i], a, b, c, d);
+            v[4 * i] = a * s; v[4 * i + 1] = b * s; v[4 * i + 2] = c * s; v[4 * i + 3] = d * s;
+        }
+    }
+};
+template <int V> __device__ __forceinline__ void gg_a8_ld(const uint8_t *codes, const uint8_t *scale, float (&v)[V])
+{
+    GGCodes<V> c;
+    c.load(codes, scale);
+    c.get(v);
 }

@@ -26,26 +26,25 @@ __global__ __launch_bounds__(THREADS) void gg_k_act8_pack(const T *__restrict__ 
     constexpr int V = GGRowT<T>::V;
     const int Cp = gg_a8_cp(C), nb = Cp / GG_A8_BLOCK;
     const int tr = threadIdx.x / l.tpr, q = blockIdx.y * l.tpr + threadIdx.x % l.tpr, c = q * V;
-    const bool on = tr < l.rpb && q < l.nq;
+    const bool on = tr < l.rpb && q < l.nq;     // (a chunk behind C: zeros)
     const long long step = (long long)gridDim.x * l.rpb * UNROLL;
     for (long long r0 = (long long)blockIdx.x * l.rpb * UNROLL; r0 < R; r0 += step) {
-        float v[UNROLL][V];
+        GGChunk<T> in[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) {
             const long long r = r0 + (long long)u * l.rpb + tr;
-            if (on && r < R) {
-                gg_ld_chunk(x + r * ldx, c, C, v[u]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; i++) v[u][i] = 0.f;
-            }
+            if (on && r < R) in[u].load(x + r * ldx, c, C);
+            else in[u].zero();
         }
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) {
             const long long r = r0 + (long long)u * l.rpb + tr;
-            const unsigned byte = gg_a8_block_byte<V>(v[u]);
+            float v[V];
+            in[u].get(v);
+            bool clean;
+            const unsigned byte = gg_a8_block_byte<V>(v, clean);
             unsigned w[V / 4];
-            gg_a8_encode<V>(v[u], byte, w);
+            gg_a8_encode<V>(v, byte, clean, w);
             if (on && r < R) {
                 gg_a8_st_codes<V>(codes + r * Cp + c, w);
                 if (c % GG_A8_BLOCK == 0) scales[r * nb + c / GG_A8_BLOCK] = (uint8_t)byte;
@@ -69,7 +68,7 @@ __global__ __launch_bounds__(THREADS) void gg_k_act8_unpack(const uint8_t *__res
         for (int u = 0; u < UNROLL; u++) {
             const long long r = r0 + (long long)u * l.rpb;
             const long long rr = r < R ? r : R - 1;
-            gg_a8_ld<V>(codes + rr * Cp + c, scales[rr * nb + c / GG_A8_BLOCK], v[u]);
+            gg_a8_ld<V>(codes + rr * Cp + c, scales + rr * nb + c / GG_A8_BLOCK, v[u]);
         }
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) {
@@ -104,7 +103,7 @@ extern "C" {
 
 int gridgcn_act8_pack(const void *x, int dtype, long long R, int C, long long ldx, uint8_t *codes, uint8_t *scales, void *stream)
 {
-    if (!x || !codes || !scales || R < 1 || C < 1 || C > GRIDGCN_ACT8_MAX_C || ldx < C || ((uintptr_t)codes & 15)) return GRIDGCN_EINVAL;
+    if (!x || !codes || !scales || R < 1 || C < 1 || C > GRIDGCN_ACT8_MAX_C || ldx < C || ldx > GRIDGCN_MAX_LD || ((uintptr_t)codes & 15)) return GRIDGCN_EINVAL;
     const hipStream_t st = (hipStream_t)stream;
     if (dtype == GRIDGCN_F32) pack<float>(x, R, C, ldx, codes, scales, st);
     else if (dtype == GRIDGCN_BF16) pack<gg_bf16>(x, R, C, ldx, codes, scales, st);
@@ -115,7 +114,7 @@ int gridgcn_act8_pack(const void *x, int dtype, long long R, int C, long long ld
 
 int gridgcn_act8_unpack(const uint8_t *codes, const uint8_t *scales, long long R, int C, int dtype, void *x, long long ldx, void *stream)
 {
-    if (!x || !codes || !scales || R < 1 || C < 1 || C > GRIDGCN_ACT8_MAX_C || ldx < C || ((uintptr_t)codes & 15)) return GRIDGCN_EINVAL;
+    if (!x || !codes || !scales || R < 1 || C < 1 || C > GRIDGCN_ACT8_MAX_C || ldx < C || ldx > GRIDGCN_MAX_LD || ((uintptr_t)codes & 15)) return GRIDGCN_EINVAL;
     const hipStream_t st = (hipStream_t)stream;
     if (dtype == GRIDGCN_F32) unpack<float>(codes, scales, R, C, x, ldx, st);
     else if (dtype == GRIDGCN_BF16) unpack<gg_bf16>(codes, scales, R, C, x, ldx, st);

@@ -9,7 +9,7 @@
 // All of it is streaming: a thread keeps one column chunk of 16 bytes (its channels' constants sit in registers) and walks
 // rows.  The statistics are a reduction over a whole cloud, so a pass over the data has to end before the next begins: two
 // passes with a small launch between them that turns the workgroups' partial sums into statistics, or -- where the rows of a
-// few groups of one cloud fit a CU's caches -- ONE launch whose workgroup reads its rows twice.
+// few groups of one cloud fit a workgroup's registers -- ONE launch that reads them once.
 //
 // Numerics.  Sums of the statistics run in 64 bits on x - x[first row, first channel of the group] (64-bit vector adds run at
 // the rate of 32-bit ones here, the passes wait for memory): the variance needs no second look at the data even when the mean is
@@ -23,15 +23,17 @@
 namespace {
 constexpr int THREADS = 256;
 constexpr int UNROLL = 4;
+constexpr int FEW = 512;                   // threads of the one-launch form, which keeps its values in registers
+template <class T> constexpr int KEEP = sizeof(T) == 4 ? 16 : 8;     // chunks a thread keeps
 constexpr float SQRT1_2 = 0.70710678118654752f, INV_SQRT_2PI = 0.39894228040143268f;
 
 struct Lay { int nq, tpr, rpb; };          // chunks of a slab row, threads per row, rows per step
-Lay lay_of(int nq)
+Lay lay_of(int nq, int threads = THREADS)
 {
     Lay l;
     l.nq = nq;
-    l.tpr = nq < THREADS ? nq : THREADS;
-    l.rpb = THREADS / l.tpr;
+    l.tpr = nq < threads ? nq : threads;
+    l.rpb = threads / l.tpr;
     return l;
 }
 
@@ -49,7 +51,7 @@ struct Args {
     double *stats;                         // [B, G, 2] mean, rstd
     double *part;                          // [B, chunks, C, 2] partial sums of the workgroups
     double *tot;                           // [B, C, 2] sums of g and g * xh
-    float2 *coef;                          // [B, G] S1, S2
+    float2 *coef;                          // [B, G] rstd S1, rstd^2 S2
     long long rpc;                         // rows of a chunk
     int chunks;
 };
@@ -61,35 +63,57 @@ __device__ __forceinline__ long long count_of(const Args &a, int b)
     return n < 0 ? 0 : (n < a.N ? n : a.N);
 }
 
+// Phi(t) = (1 + erf(t / sqrt 2)) / 2 and e = exp(-t^2 / 2), which its derivative wants as well.  erf by the rational
+// approximation 7.1.26 of Abramowitz and Stegun, whose one exponential is that same e: |error of Phi| < 7.5e-8, about half a step
+// of float32 at 1 (half the instructions of erff plus an exponential: a forward + backward of 67 M bf16 values by erff was
+// bound by arithmetic).
+__device__ __forceinline__ float normal_cdf(float t, float &e)
+{
+    const float a = fabsf(t), k = __builtin_amdgcn_rcpf(fmaf(a, 0.3275911f * SQRT1_2, 1.f));
+    e = __expf(-0.5f * t * t);
+    float q = fmaf(k, 1.061405429f, -1.453152027f);
+    q = fmaf(k, q, 1.421413741f);
+    q = fmaf(k, q, -0.284496736f);
+    q = fmaf(k, q, 0.254829592f);
+    q *= 0.5f * k * e;                      // Phi(-|t|): no cancellation on the side where it is small
+    return t < 0.f ? q : 1.f - q;
+}
+// (the reciprocal instruction is good to one step: far below the activation's own rounding budget)
+__device__ __forceinline__ float sigmoid(float t) { return __builtin_amdgcn_rcpf(1.f + __expf(-t)); }
+
 template <int ACT> __device__ __forceinline__ float act_of(float t)
 {
     if constexpr (ACT == GRIDGCN_ACT_RELU) return t > 0.f ? t : (t != t ? t : 0.f);     // (NaN stays NaN)
-    if constexpr (ACT == GRIDGCN_ACT_SILU) return t / (1.f + __expf(-t));
-    if constexpr (ACT == GRIDGCN_ACT_GELU) return 0.5f * t * (1.f + erff(t * SQRT1_2));
+    if constexpr (ACT == GRIDGCN_ACT_SILU) return t * sigmoid(t);
+    if constexpr (ACT == GRIDGCN_ACT_GELU) {
+        float e;
+        return t * normal_cdf(t, e);
+    }
     return t;
 }
 template <int ACT> __device__ __forceinline__ float act_grad(float t)
 {
     if constexpr (ACT == GRIDGCN_ACT_SILU) {
-        const float s = 1.f / (1.f + __expf(-t));
-        return s * (1.f + t * (1.f - s));
+        const float s = sigmoid(t);
+        return s * fmaf(t, 1.f - s, 1.f);
     }
-    if constexpr (ACT == GRIDGCN_ACT_GELU)
-        return 0.5f * (1.f + erff(t * SQRT1_2)) + t * __expf(-0.5f * t * t) * INV_SQRT_2PI;
+    if constexpr (ACT == GRIDGCN_ACT_GELU) {
+        float e;
+        const float c = normal_cdf(t, e);
+        return fmaf(t * INV_SQRT_2PI, e, c);
+    }
     return 1.f;
 }
 
 // constants of one channel
-struct Chan { float mh, ml, a, beta, rstd, gamma; };
+struct Chan { float mh, ml, a, beta; };     // mean in two parts, rstd * gamma, beta
 __device__ __forceinline__ Chan chan_of(const Args &a, double mean, double rstd, int c)
 {
     Chan k;
     k.mh = (float)mean;
     k.ml = (float)(mean - (double)k.mh);
-    k.rstd = (float)rstd;
-    k.gamma = gg_ld_param(a.gamma, a.ptype, c, 1.f);
     k.beta = gg_ld_param(a.beta, a.ptype, c, 0.f);
-    k.a = (float)(rstd * (double)k.gamma);
+    k.a = (float)(rstd * (double)gg_ld_param(a.gamma, a.ptype, c, 1.f));
     return k;
 }
 // ... of the V channels of a thread, from the statistics in memory
@@ -105,10 +129,11 @@ template <int V, class P> __device__ __forceinline__ void chans(const Args &a, c
 __device__ __forceinline__ float dev_of(const Chan &k, float x) { return (x - k.mh) - k.ml; }
 
 // ReLU: is t = d a + beta > 0?  The float value is off by less than 2^-21 of |beta| where the two terms cancel.
-__device__ __forceinline__ bool positive(const Chan &k, float t, float x, const double *stat, const Args &a)
+__device__ __forceinline__ bool positive(const Chan &k, float t, float x, const double *stat, const Args &a, int c)
 {
     if (__builtin_expect(fabsf(t) <= fabsf(k.beta) * 0x1p-20f, 0)) {
-        const double t64 = ((double)x - stat[0]) * stat[1] * (double)k.gamma + (double)k.beta;
+        const double *st = stat + (c / a.cg) * 2;
+        const double t64 = ((double)x - st[0]) * st[1] * (double)gg_ld_param(a.gamma, a.ptype, c, 1.f) + (double)k.beta;
         return t64 > 0.0;
     }
     return t > 0.f;
@@ -129,7 +154,7 @@ template <int V> struct Pos {
 };
 
 // Sums s[V][2] of the threads of a column over the workgroup's row lanes: LDS red[rpb][tpr * V][2]; afterwards red[0] holds them.
-template <int V> __device__ __forceinline__ void reduce_rows(double *red, const Lay &l, int tr, int qi, const double (&s)[V][2])
+template <int V, int NT> __device__ __forceinline__ void reduce_rows(double *red, const Lay &l, int tr, int qi, const double (&s)[V][2])
 {
     const int w = l.tpr * V * 2;
     if (tr < l.rpb) {
@@ -140,7 +165,7 @@ template <int V> __device__ __forceinline__ void reduce_rows(double *red, const 
         }
     }
     __syncthreads();
-    for (int j = threadIdx.x; j < w; j += THREADS) {
+    for (int j = threadIdx.x; j < w; j += NT) {
         double v = red[j];
         for (int r = 1; r < l.rpb; r++) v += red[(size_t)r * w + j];
         red[j] = v;                        // (entry j of row 0 is this thread's alone)
@@ -162,38 +187,38 @@ __device__ __forceinline__ void rows_stats(const Args &a, const Lay &l, const Po
         const int c = p.c + i < a.C ? p.c + i : a.C - 1;
         base[i] = r1 > r0 ? (double)GGRowT<T>::get(x + (c / a.cg) * a.cg) : 0.0;      // (row 0 is valid where any row is)
     }
-    for (long long n0 = r0; n0 < r1; n0 += (long long)l.rpb * UNROLL) {
-        float v[UNROLL][V];
+    constexpr int U = SAVE8 ? UNROLL : 2 * UNROLL;
+    for (long long n0 = r0; n0 < r1; n0 += (long long)l.rpb * U) {
+        GGChunk<T> r[U];
 #pragma unroll
-        for (int u = 0; u < UNROLL; u++) {
+        for (int u = 0; u < U; u++) {
             const long long n = n0 + (long long)u * l.rpb + p.tr;
-            if (p.on && n < r1) {
-                gg_ld_chunk(x + (size_t)n * a.xn, p.c, a.C, v[u]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; i++) v[u][i] = 0.f;
-            }
+            if (p.on && n < r1) r[u].load(x + (size_t)n * a.xn, p.c, a.C);
+            else r[u].zero();
         }
 #pragma unroll
-        for (int u = 0; u < UNROLL; u++) {
+        for (int u = 0; u < U; u++) {
             const long long n = n0 + (long long)u * l.rpb + p.tr;
             const bool in = p.on && n < r1;
+            float v[V];
+            r[u].get(v);
             if (in) {
 #pragma unroll
                 for (int i = 0; i < V; i++) {
-                    const double d = (double)v[u][i] - base[i];
+                    const double d = (double)v[i] - base[i];
                     s[i][0] += d;
                     s[i][1] = fma(d, d, s[i][1]);
                 }
             }
             if constexpr (SAVE8) {
-                const unsigned byte = gg_a8_block_byte<V>(v[u]);
+                bool clean;
+                const unsigned byte = gg_a8_block_byte<V>(v, clean);
                 unsigned w[V / 4];
-                gg_a8_encode<V>(v[u], byte, w);
+                gg_a8_encode<V>(v, byte, clean, w);
                 if (in) {
-                    const size_t r = (size_t)p.b * a.N + n;
-                    gg_a8_st_codes<V>(a.codes_out + r * Cp + p.c, w);
-                    if (p.c % GG_A8_BLOCK == 0) a.scales_out[r * nb + p.c / GG_A8_BLOCK] = (uint8_t)byte;
+                    const size_t row = (size_t)p.b * a.N + n;
+                    gg_a8_st_codes<V>(a.codes_out + row * Cp + p.c, w);
+                    if (p.c % GG_A8_BLOCK == 0) a.scales_out[row * nb + p.c / GG_A8_BLOCK] = (uint8_t)byte;
                 }
             }
         }
@@ -220,50 +245,54 @@ __device__ __forceinline__ void rows_apply(const Args &a, const Lay &l, const Po
     const T *x = (const T *)a.x + (size_t)p.b * a.xb;
     T *y = (T *)a.y + (size_t)p.b * a.N * a.C;
     if (!p.on) return;
-    for (long long n0 = r0 + p.tr; n0 < r1; n0 += (long long)l.rpb * UNROLL) {
-        float v[UNROLL][V];
+    const long long rv = r1 < count ? r1 : count;          // rows with values
+    long long n0 = r0 + p.tr;
+    for (; n0 < rv; n0 += (long long)l.rpb * UNROLL) {
+        GGChunk<T> r[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) {
             const long long n = n0 + (long long)u * l.rpb;
-            if (n < count && n < r1) {
-                gg_ld_chunk(x + (size_t)n * a.xn, p.c, a.C, v[u]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; i++) v[u][i] = 0.f;
-            }
+            r[u].load(x + (size_t)(n < rv ? n : n0) * a.xn, p.c, a.C);
         }
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) {
             const long long n = n0 + (long long)u * l.rpb;
-            float o[V];
+            if (n >= r1) continue;
+            float v[V], o[V];
+            r[u].get(v);
 #pragma unroll
-            for (int i = 0; i < V; i++) o[i] = n < count ? act_of<ACT>(fmaf(dev_of(k[i], v[u][i]), k[i].a, k[i].beta)) : 0.f;
-            if (n < r1) gg_st_chunk(y + (size_t)n * a.C, p.c, a.C, o);
+            for (int i = 0; i < V; i++) o[i] = n < rv ? act_of<ACT>(fmaf(dev_of(k[i], v[i]), k[i].a, k[i].beta)) : 0.f;
+            gg_st_chunk(y + (size_t)n * a.C, p.c, a.C, o);
         }
     }
+    float z[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) z[i] = 0.f;
+    for (; n0 < r1; n0 += l.rpb) gg_st_chunk(y + (size_t)n0 * a.C, p.c, a.C, z);
 }
 
-// x^ of one chunk: the input itself or its 8-bit form
-template <class T, bool Q8>
-__device__ __forceinline__ void ld_x(const Args &a, const Pos<GGRowT<T>::V> &p, long long n, float (&v)[GGRowT<T>::V])
-{
-    constexpr int V = GGRowT<T>::V;
-    if constexpr (Q8) {
-        const int Cp = gg_a8_cp(a.C);
-        const size_t r = (size_t)p.b * a.N + n;
-        gg_a8_ld<V>(a.codes + r * Cp + p.c, a.scales[r * (Cp / GG_A8_BLOCK) + p.c / GG_A8_BLOCK], v);
-    } else {
-        gg_ld_chunk((const T *)a.x + (size_t)p.b * a.xb + (size_t)n * a.xn, p.c, a.C, v);
+// x^ of one chunk as it stands in memory: the input itself or its 8-bit form
+template <class T, bool Q8> struct Xhat {
+    typename std::conditional<Q8, GGCodes<GGRowT<T>::V>, GGChunk<T>>::type r;
+    __device__ __forceinline__ void load(const Args &a, const Pos<GGRowT<T>::V> &p, long long n)
+    {
+        if constexpr (Q8) {
+            const int Cp = gg_a8_cp(a.C);
+            const size_t row = (size_t)p.b * a.N + n;
+            r.load(a.codes + row * Cp + p.c, a.scales + row * (Cp / GG_A8_BLOCK) + p.c / GG_A8_BLOCK);
+        } else {
+            r.load((const T *)a.x + (size_t)p.b * a.xb + (size_t)n * a.xn, p.c, a.C);
+        }
     }
-}
+};
 
-// g = dy act'(t) of one value
+// g = dy act'(t) of one value of channel c; stat: the cloud's statistics
 template <int ACT>
-__device__ __forceinline__ float gate(const Args &a, const Chan &k, float dy, float d, float x, const double *stat)
+__device__ __forceinline__ float gate(const Args &a, const Chan &k, float dy, float d, float x, const double *stat, int c)
 {
     if constexpr (ACT == GRIDGCN_ACT_NONE) return dy;
     const float t = fmaf(d, k.a, k.beta);
-    if constexpr (ACT == GRIDGCN_ACT_RELU) return positive(k, t, x, stat, a) ? dy : 0.f;
+    if constexpr (ACT == GRIDGCN_ACT_RELU) return positive(k, t, x, stat, a, c < a.C ? c : a.C - 1) ? dy : 0.f;
     return dy * act_grad<ACT>(t);
 }
 
@@ -279,31 +308,35 @@ __device__ __forceinline__ void rows_bwd_sums(const Args &a, const Lay &l, const
     for (int i = 0; i < V; i++) s[i][0] = s[i][1] = 0.0;
     if (!p.on) return;
     for (long long n0 = r0 + p.tr; n0 < r1; n0 += (long long)l.rpb * UNROLL) {
-        float v[UNROLL][V], e[UNROLL][V];
+        GGChunk<T> re[UNROLL];
+        Xhat<T, Q8> rx[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) {
-            const long long n = n0 + (long long)u * l.rpb;
-            if (n < r1) {
-                gg_ld_chunk(dy + (size_t)n * a.gn, p.c, a.C, e[u]);
-                ld_x<T, Q8>(a, p, n, v[u]);
-            } else {
+            const long long n = n0 + (long long)u * l.rpb, nn = n < r1 ? n : n0;
+            re[u].load(dy + (size_t)nn * a.gn, p.c, a.C);
+            rx[u].load(a, p, nn);
+        }
+        float s0[V], s1[V];
 #pragma unroll
-                for (int i = 0; i < V; i++) { e[u][i] = 0.f; v[u][i] = k[i].mh; }
+        for (int i = 0; i < V; i++) s0[i] = s1[i] = 0.f;
+#pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            if (n0 + (long long)u * l.rpb >= r1) continue;
+            float e[V], v[V];
+            re[u].get(e);
+            rx[u].r.get(v);
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const float d = dev_of(k[i], v[i]);
+                const float g = gate<ACT>(a, k[i], e[i], d, v[i], stat, p.c + i);
+                s0[i] += g;
+                s1[i] = fmaf(g, d, s1[i]);
             }
         }
 #pragma unroll
         for (int i = 0; i < V; i++) {
-            float s0 = 0.f, s1 = 0.f;
-#pragma unroll
-            for (int u = 0; u < UNROLL; u++) {
-                const float d = dev_of(k[i], v[u][i]);
-                const int c = p.c + i < a.C ? p.c + i : a.C - 1;
-                const float g = gate<ACT>(a, k[i], e[u][i], d, v[u][i], stat + (c / a.cg) * 2);
-                s0 += g;
-                s1 = fmaf(g, d, s1);
-            }
-            s[i][0] += (double)s0;
-            s[i][1] += (double)s1;
+            s[i][0] += (double)s0[i];
+            s[i][1] += (double)s1[i];
         }
     }
 }
@@ -318,40 +351,42 @@ __device__ __forceinline__ void rows_bwd_dx(const Args &a, const Lay &l, const P
     T *dx = (T *)a.y + (size_t)p.b * a.N * a.C;
     const double *stat = a.stats + (size_t)p.b * a.G * 2;
     if (!p.on) return;
-    for (long long n0 = r0 + p.tr; n0 < r1; n0 += (long long)l.rpb * UNROLL) {
-        float v[UNROLL][V], e[UNROLL][V];
+    const long long rv = r1 < count ? r1 : count;          // rows with values
+    long long n0 = r0 + p.tr;
+    for (; n0 < rv; n0 += (long long)l.rpb * UNROLL) {
+        GGChunk<T> re[UNROLL];
+        Xhat<T, Q8> rx[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) {
-            const long long n = n0 + (long long)u * l.rpb;
-            if (n < count && n < r1) {
-                gg_ld_chunk(dy + (size_t)n * a.gn, p.c, a.C, e[u]);
-                ld_x<T, Q8>(a, p, n, v[u]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < V; i++) { e[u][i] = 0.f; v[u][i] = k[i].mh; }
-            }
+            const long long n = n0 + (long long)u * l.rpb, nn = n < rv ? n : n0;
+            re[u].load(dy + (size_t)nn * a.gn, p.c, a.C);
+            rx[u].load(a, p, nn);
         }
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) {
             const long long n = n0 + (long long)u * l.rpb;
-            float o[V];
+            if (n >= r1) continue;
+            float e[V], v[V], o[V];
+            re[u].get(e);
+            rx[u].r.get(v);
 #pragma unroll
             for (int i = 0; i < V; i++) {
-                const float d = dev_of(k[i], v[u][i]);
-                const int c = p.c + i < a.C ? p.c + i : a.C - 1;
-                const float g = gate<ACT>(a, k[i], e[u][i], d, v[u][i], stat + (c / a.cg) * 2);
-                // (gamma * g rounded on its own: in a group of one value it equals S1, and dx is 0)
-                const float h = k[i].gamma * g;
-                o[i] = n < count ? ((h - f[i].x) - (d * k[i].rstd) * f[i].y) * k[i].rstd : 0.f;
+                const float d = dev_of(k[i], v[i]);
+                const float g = gate<ACT>(a, k[i], e[i], d, v[i], stat, p.c + i);
+                o[i] = n < rv ? fmaf(k[i].a, g, -fmaf(d, f[i].y, f[i].x)) : 0.f;
             }
-            if (n < r1) gg_st_chunk(dx + (size_t)n * a.C, p.c, a.C, o);
+            gg_st_chunk(dx + (size_t)n * a.C, p.c, a.C, o);
         }
     }
+    float z[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) z[i] = 0.f;
+    for (; n0 < r1; n0 += l.rpb) gg_st_chunk(dx + (size_t)n0 * a.C, p.c, a.C, z);
 }
 
 // ---- many rows: pass, small launch, pass ----------------------------------------------------------------------------
 template <class T, bool SAVE8>
-__global__ __launch_bounds__(THREADS) void gg_k_gn_stats(Args a, Lay l)
+__global__ __launch_bounds__(THREADS, 4) void gg_k_gn_stats(Args a, Lay l)
 {
     constexpr int V = GGRowT<T>::V;
     __shared__ double red[THREADS * V * 2];
@@ -361,7 +396,7 @@ __global__ __launch_bounds__(THREADS) void gg_k_gn_stats(Args a, Lay l)
     const long long r1 = r0 + a.rpc < count ? r0 + a.rpc : count;
     double s[V][2], base[V];
     rows_stats<T, SAVE8>(a, l, p, r0, r1, s, base);
-    reduce_rows<V>(red, l, p.tr, (int)threadIdx.x % l.tpr, s);
+    reduce_rows<V, THREADS>(red, l, p.tr, (int)threadIdx.x % l.tpr, s);
     double *out = a.part + ((size_t)p.b * a.chunks + blockIdx.x) * a.C * 2;
     const int c0 = blockIdx.y * l.tpr * V;
     for (int j = threadIdx.x; j < l.tpr * V * 2; j += THREADS)
@@ -373,7 +408,7 @@ __global__ __launch_bounds__(THREADS) void gg_k_gn_stats(Args a, Lay l)
 template <class F> __device__ __forceinline__ void sum_chunks(const Args &a, int b, int c0, int n, double *red, F f)
 {
     const int cw = n < THREADS ? n : THREADS, nl = THREADS / cw;
-    const int cl = threadIdx.x % cw, kl = threadIdx.x / cw;
+    const int cl = threadIdx.x % cw, kl = threadIdx.x / cw;       // (kl >= nl: idle)
     for (int o = 0; o < n; o += cw) {
         double s0 = 0.0, s1 = 0.0;
         if (kl < nl && o + cl < n) {
@@ -385,14 +420,17 @@ template <class F> __device__ __forceinline__ void sum_chunks(const Args &a, int
         }
         red[threadIdx.x * 2] = s0;
         red[threadIdx.x * 2 + 1] = s1;
-        __syncthreads();
-        if ((int)threadIdx.x < cw && o + cl < n) {
-            for (int k = 1; k < nl; k++) {
-                s0 += red[(k * cw + cl) * 2];
-                s1 += red[(k * cw + cl) * 2 + 1];
+        for (int d = 128; d > 0; d /= 2) {          // (nl <= 256)
+            if (d >= nl) continue;
+            __syncthreads();
+            if (kl < d && kl + d < nl) {
+                s0 += red[(threadIdx.x + d * cw) * 2];
+                s1 += red[(threadIdx.x + d * cw) * 2 + 1];
+                red[threadIdx.x * 2] = s0;
+                red[threadIdx.x * 2 + 1] = s1;
             }
-            f(c0 + o + cl, s0, s1);
         }
+        if (kl == 0 && o + cl < n) f(c0 + o + cl, s0, s1);
         __syncthreads();
     }
 }
@@ -416,11 +454,11 @@ __device__ __forceinline__ void sum_block(double *red, double &s, double &q)
 
 // for each of ng groups of cg values in LDS: the sums of get(value index) -> (s, q), then done(group, s, q) by one thread.
 // Many channels: a wave per group; few: a thread per group.
-template <class G, class D> __device__ __forceinline__ void for_groups(int cg, int ng, G get, D done)
+template <int NT, class G, class D> __device__ __forceinline__ void for_groups(int cg, int ng, G get, D done)
 {
     if (cg >= 32) {
         const int lane = threadIdx.x & 63;
-        for (int j = threadIdx.x >> 6; j < ng; j += THREADS / 64) {
+        for (int j = threadIdx.x >> 6; j < ng; j += NT / 64) {
             double s = 0.0, q = 0.0;
             for (int c = lane; c < cg; c += 64) get(j * cg + c, s, q);
 #pragma unroll
@@ -431,7 +469,7 @@ template <class G, class D> __device__ __forceinline__ void for_groups(int cg, i
             if (lane == 0) done(j, s, q);
         }
     } else {
-        for (int j = threadIdx.x; j < ng; j += THREADS) {
+        for (int j = threadIdx.x; j < ng; j += NT) {
             double s = 0.0, q = 0.0;
             for (int c = 0; c < cg; c++) get(j * cg + c, s, q);
             done(j, s, q);
@@ -469,7 +507,7 @@ __global__ __launch_bounds__(THREADS) void gg_k_gn_apply(Args a, Lay l)
 }
 
 template <class T, int ACT, bool Q8>
-__global__ __launch_bounds__(THREADS) void gg_k_gn_bwd_sums(Args a, Lay l)
+__global__ __launch_bounds__(THREADS, 4) void gg_k_gn_bwd_sums(Args a, Lay l)
 {
     constexpr int V = GGRowT<T>::V;
     __shared__ double red[THREADS * V * 2];
@@ -481,20 +519,20 @@ __global__ __launch_bounds__(THREADS) void gg_k_gn_bwd_sums(Args a, Lay l)
     chans<V>(a, p, k);
     double s[V][2];
     rows_bwd_sums<T, ACT, Q8>(a, l, p, r0, r1, k, s);
-    reduce_rows<V>(red, l, p.tr, (int)threadIdx.x % l.tpr, s);
+    reduce_rows<V, THREADS>(red, l, p.tr, (int)threadIdx.x % l.tpr, s);
     double *out = a.part + ((size_t)p.b * a.chunks + blockIdx.x) * a.C * 2;
     const int c0 = blockIdx.y * l.tpr * V;
     for (int j = threadIdx.x; j < l.tpr * V * 2; j += THREADS)
         if (c0 + j / 2 < a.C) out[(size_t)c0 * 2 + j] = red[j];
 }
 
-// S1, S2 of a group from the sums of gamma g and gamma g d over it
+// What dx needs of a group, from the sums of gamma g and gamma g d over it:  dx = (rstd gamma) g - (rstd S1 + d rstd^2 S2)
 __device__ __forceinline__ float2 coef_of(const Args &a, int b, int g, double s1, double s2)
 {
     const long long count = count_of(a, b);
     if (count < 1) return make_float2(0.f, 0.f);
     const double m = (double)count * a.cg, rstd = a.stats[((size_t)b * a.G + g) * 2 + 1];
-    return make_float2((float)(s1 / m), (float)(s2 * rstd / m));
+    return make_float2((float)(rstd * s1 / m), (float)(rstd * rstd * (s2 * rstd) / m));
 }
 
 __global__ __launch_bounds__(THREADS) void gg_k_gn_bwd_fin(Args a)
@@ -529,7 +567,7 @@ __device__ __forceinline__ void params_of(const Args &a, int c)
 }
 
 template <class T, int ACT, bool Q8>
-__global__ __launch_bounds__(THREADS) void gg_k_gn_bwd_dx(Args a, Lay l)
+__global__ __launch_bounds__(THREADS, 4) void gg_k_gn_bwd_dx(Args a, Lay l)
 {
     constexpr int V = GGRowT<T>::V;
     if (blockIdx.x == 0 && blockIdx.z == 0) {
@@ -557,63 +595,147 @@ __global__ __launch_bounds__(THREADS) void gg_k_gn_params(Args a)
     if (c < a.C) params_of(a, c);
 }
 
-// ---- few rows: one launch, a workgroup = whole groups of one cloud (l.nq chunks from channel slab * slab_c on) ---------
+// ---- few rows: one launch, a workgroup = whole groups of one cloud (l.nq chunks from channel slab * slab_c on), every value read
+// once and kept in registers: the time is one trip to memory, a reduction and the stores --------------------------------------
 template <class T, int ACT, bool SAVE8>
-__global__ __launch_bounds__(THREADS) void gg_k_gn_small(Args a, Lay l, int slab_c)
+__global__ __launch_bounds__(FEW) void gg_k_gn_small(Args a, Lay l, int slab_c)
 {
-    constexpr int V = GGRowT<T>::V;
-    __shared__ double red[THREADS * V * 2];
-    __shared__ double grp[THREADS * V * 2];
+    constexpr int V = GGRowT<T>::V, K = KEEP<T>;
+    __shared__ double red[FEW * V * 2];
     const int c0 = blockIdx.x * slab_c, c1 = c0 + slab_c < a.C ? c0 + slab_c : a.C;
     Pos<V> p(l, c0 / V, blockIdx.y);
-    p.on = p.tr < l.rpb && p.c < (SAVE8 ? (c1 == a.C ? gg_a8_cp(a.C) : c1) : c1);
+    p.on = p.tr < l.rpb && p.c < (SAVE8 && c1 == a.C ? gg_a8_cp(a.C) : c1);
     const long long count = count_of(a, p.b);
+    const T *x = (const T *)a.x + (size_t)p.b * a.xb;
+    GGChunk<T> r[K];
+#pragma unroll
+    for (int u = 0; u < K; u++) {
+        const long long n = (long long)u * l.rpb + p.tr;
+        if (p.on && n < count) r[u].load(x + (size_t)n * a.xn, p.c, a.C);
+        else r[u].zero();
+    }
     double s[V][2], base[V];
-    rows_stats<T, SAVE8>(a, l, p, 0, count, s, base);
-    reduce_rows<V>(red, l, p.tr, (int)threadIdx.x % l.tpr, s);
-    for_groups(a.cg, (c1 - c0) / a.cg, [&](int c, double &t, double &q) { t += red[c * 2]; q += red[c * 2 + 1]; },
-               [&](int j, double t, double q) {
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        s[i][0] = s[i][1] = 0.0;
+        const int c = p.c + i < a.C ? p.c + i : a.C - 1;
+        base[i] = count > 0 ? (double)GGRowT<T>::get(x + (c / a.cg) * a.cg) : 0.0;
+    }
+    const int Cp = gg_a8_cp(a.C), nb = Cp / GG_A8_BLOCK;
+#pragma unroll
+    for (int u = 0; u < K; u++) {
+        const long long n = (long long)u * l.rpb + p.tr;
+        const bool in = p.on && n < count;
+        if ((long long)u * l.rpb >= a.N) continue;
+        float v[V];
+        r[u].get(v);
+        if (in) {
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const double d = (double)v[i] - base[i];
+                s[i][0] += d;
+                s[i][1] = fma(d, d, s[i][1]);
+            }
+        }
+        if constexpr (SAVE8) {
+            bool clean;
+            const unsigned byte = gg_a8_block_byte<V>(v, clean);
+            unsigned w[V / 4];
+            gg_a8_encode<V>(v, byte, clean, w);
+            if (in) {
+                const size_t row = (size_t)p.b * a.N + n;
+                gg_a8_st_codes<V>(a.codes_out + row * Cp + p.c, w);
+                if (p.c % GG_A8_BLOCK == 0) a.scales_out[row * nb + p.c / GG_A8_BLOCK] = (uint8_t)byte;
+            }
+        }
+    }
+    reduce_rows<V, FEW>(red, l, p.tr, (int)threadIdx.x % l.tpr, s);
+    // (a group's statistics take the place of its first channel's sums, once the group is summed)
+    for_groups<FEW>(a.cg, (c1 - c0) / a.cg, [&](int c, double &t, double &q) { t += red[c * 2]; q += red[c * 2 + 1]; },
+                    [&](int j, double t, double q) {
         const int g = c0 / a.cg + j;
-        const double b0 = count > 0 ? (double)GGRowT<T>::get((const T *)a.x + (size_t)p.b * a.xb + g * a.cg) : 0.0;
-        finish_stats(t, q, b0, (double)count * a.cg, a.eps, grp + j * 2, grp + j * 2 + 1);
-        a.stats[((size_t)p.b * a.G + g) * 2] = grp[j * 2];
-        a.stats[((size_t)p.b * a.G + g) * 2 + 1] = grp[j * 2 + 1];
+        const double b0 = count > 0 ? (double)GGRowT<T>::get(x + g * a.cg) : 0.0;
+        double mean, rstd;
+        finish_stats(t, q, b0, (double)count * a.cg, a.eps, &mean, &rstd);
+        red[j * a.cg * 2] = mean;
+        red[j * a.cg * 2 + 1] = rstd;
+        if (a.stats) {
+            a.stats[((size_t)p.b * a.G + g) * 2] = mean;
+            a.stats[((size_t)p.b * a.G + g) * 2 + 1] = rstd;
+        }
     });
     __syncthreads();
-    if (p.c >= c1) p.on = false;
+    if (!p.on || p.c >= c1) return;
     Chan k[V];
 #pragma unroll
     for (int i = 0; i < V; i++) {
         const int c = p.c + i < c1 ? p.c + i : c1 - 1;
-        const double *st = grp + (c / a.cg - c0 / a.cg) * 2;
+        const double *st = red + ((c - c0) / a.cg) * a.cg * 2;
         k[i] = chan_of(a, st[0], st[1], c);
     }
-    rows_apply<T, ACT>(a, l, p, 0, a.N, count, k);
+    T *y = (T *)a.y + (size_t)p.b * a.N * a.C;
+#pragma unroll
+    for (int u = 0; u < K; u++) {
+        const long long n = (long long)u * l.rpb + p.tr;
+        if (n >= a.N) continue;
+        float v[V], o[V];
+        r[u].get(v);
+#pragma unroll
+        for (int i = 0; i < V; i++) o[i] = n < count ? act_of<ACT>(fmaf(dev_of(k[i], v[i]), k[i].a, k[i].beta)) : 0.f;
+        gg_st_chunk(y + (size_t)n * a.C, p.c, a.C, o);
+    }
 }
 
 template <class T, int ACT, bool Q8>
-__global__ __launch_bounds__(THREADS) void gg_k_gn_small_bwd(Args a, Lay l, int slab_c)
+__global__ __launch_bounds__(FEW) void gg_k_gn_small_bwd(Args a, Lay l, int slab_c)
 {
-    constexpr int V = GGRowT<T>::V;
-    __shared__ double red[THREADS * V * 2];
-    __shared__ float2 cf[THREADS * V];
+    constexpr int V = GGRowT<T>::V, K = KEEP<T>;
+    __shared__ double red[FEW * V * 2];
     const int c0 = blockIdx.x * slab_c, c1 = c0 + slab_c < a.C ? c0 + slab_c : a.C;
     Pos<V> p(l, c0 / V, blockIdx.y);
     p.on = p.tr < l.rpb && p.c < c1;
     const long long count = count_of(a, p.b);
+    const T *dy = (const T *)a.dy + (size_t)p.b * a.gb;
+    const double *stat = a.stats + (size_t)p.b * a.G * 2;
+    const int Cp = gg_a8_cp(a.C), nb = Cp / GG_A8_BLOCK;
+    GGChunk<T> rg[K];
+    typename std::conditional<Q8, GGCodes<V>, GGChunk<T>>::type rx[K];
+#pragma unroll
+    for (int u = 0; u < K; u++) {
+        const long long n = (long long)u * l.rpb + p.tr;
+        if (p.on && n < count) {
+            rg[u].load(dy + (size_t)n * a.gn, p.c, a.C);
+            const size_t row = (size_t)p.b * a.N + n;
+            if constexpr (Q8) rx[u].load(a.codes + row * Cp + p.c, a.scales + row * nb + p.c / GG_A8_BLOCK);
+            else rx[u].load((const T *)a.x + (size_t)p.b * a.xb + (size_t)n * a.xn, p.c, a.C);
+        } else {
+            rg[u].zero();
+            rx[u].zero();
+        }
+    }
     Chan k[V];
     chans<V>(a, p, k);
     double s[V][2];
-    rows_bwd_sums<T, ACT, Q8>(a, l, p, 0, count, k, s);
-    reduce_rows<V>(red, l, p.tr, (int)threadIdx.x % l.tpr, s);
-    for_groups(a.cg, (c1 - c0) / a.cg, [&](int c, double &t, double &q) {
-        const double w = (double)gg_ld_param(a.gamma, a.ptype, c0 + c, 1.f);
-        t += w * red[c * 2];
-        q += w * red[c * 2 + 1];
-    }, [&](int j, double t, double q) { cf[j] = coef_of(a, p.b, c0 / a.cg + j, t, q); });
-    for (int j = threadIdx.x; j < c1 - c0; j += THREADS) {
+#pragma unroll
+    for (int i = 0; i < V; i++) s[i][0] = s[i][1] = 0.0;
+#pragma unroll
+    for (int u = 0; u < K; u++) {
+        if (!(p.on && (long long)u * l.rpb + p.tr < count)) continue;
+        float e[V], v[V];
+        rg[u].get(e);
+        rx[u].get(v);
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const float d = dev_of(k[i], v[i]);
+            const float g = gate<ACT>(a, k[i], e[i], d, v[i], stat, p.c + i);
+            s[i][0] += (double)g;
+            s[i][1] = fma((double)g, (double)d, s[i][1]);
+        }
+    }
+    reduce_rows<V, FEW>(red, l, p.tr, (int)threadIdx.x % l.tpr, s);
+    for (int j = threadIdx.x; j < c1 - c0; j += FEW) {
         const int c = c0 + j;
-        const double db = red[j * 2], dg = count > 0 ? red[j * 2 + 1] * a.stats[((size_t)p.b * a.G + c / a.cg) * 2 + 1] : 0.0;
+        const double db = red[j * 2], dg = count > 0 ? red[j * 2 + 1] * stat[(c / a.cg) * 2 + 1] : 0.0;
         if (a.B == 1) {
             if (a.dbeta) gg_st_param(a.dbeta, a.ptype, c, (float)db);
             if (a.dgamma) gg_st_param(a.dgamma, a.ptype, c, (float)dg);
@@ -622,15 +744,43 @@ __global__ __launch_bounds__(THREADS) void gg_k_gn_small_bwd(Args a, Lay l, int 
             a.tot[((size_t)p.b * a.C + c) * 2 + 1] = dg;
         }
     }
-    __syncthreads();
     if (!a.y) return;
+    __syncthreads();
+    // (a group's coefficients take the place of its first channel's sums)
+    for_groups<FEW>(a.cg, (c1 - c0) / a.cg, [&](int c, double &t, double &q) {
+        const double w = (double)gg_ld_param(a.gamma, a.ptype, c0 + c, 1.f);
+        t += w * red[c * 2];
+        q += w * red[c * 2 + 1];
+    }, [&](int j, double t, double q) {
+        const float2 f = coef_of(a, p.b, c0 / a.cg + j, t, q);
+        red[j * a.cg * 2] = (double)f.x;
+        red[j * a.cg * 2 + 1] = (double)f.y;
+    });
+    __syncthreads();
+    if (!p.on) return;
     float2 f[V];
 #pragma unroll
     for (int i = 0; i < V; i++) {
         const int c = p.c + i < c1 ? p.c + i : c1 - 1;
-        f[i] = cf[c / a.cg - c0 / a.cg];
+        const double *q = red + ((c - c0) / a.cg) * a.cg * 2;
+        f[i] = make_float2((float)q[0], (float)q[1]);
     }
-    rows_bwd_dx<T, ACT, Q8>(a, l, p, 0, a.N, count, k, f);
+    T *dx = (T *)a.y + (size_t)p.b * a.N * a.C;
+#pragma unroll
+    for (int u = 0; u < K; u++) {
+        const long long n = (long long)u * l.rpb + p.tr;
+        if (n >= a.N) continue;
+        float e[V], v[V], o[V];
+        rg[u].get(e);
+        rx[u].get(v);
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const float d = dev_of(k[i], v[i]);
+            const float g = gate<ACT>(a, k[i], e[i], d, v[i], stat, p.c + i);
+            o[i] = n < count ? fmaf(k[i].a, g, -fmaf(d, f[i].y, f[i].x)) : 0.f;
+        }
+        gg_st_chunk(dx + (size_t)n * a.C, p.c, a.C, o);
+    }
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
@@ -646,33 +796,30 @@ struct Plan {
 
 long long gcd_ll(long long a, long long b) { return b ? gcd_ll(b, a % b) : a; }
 
-// Values of a workgroup of the one-launch form (it reads them twice, the second time from the CU's caches and L2).
-// Measured both ways (forward + backward, fp32): see the table beside gridgcn_group_norm_act_fwd's description.
-constexpr long long SMALL_VALUES = 32768;
-
-Plan plan_of(int B, long long N, int C, int G, int dtype, bool save8)
+// One launch wherever a workgroup's registers hold the rows of at least 64 bytes' worth of whole groups (32768 values);
+// rows beyond that: two passes.
+Plan plan_of(int B, long long N, int C, int G, int dtype, bool save8, bool stats, bool backward)
 {
     Plan p = {};
-    const int V = dtype == GRIDGCN_F32 ? 4 : 8, cg = C / G;
+    const int V = dtype == GRIDGCN_F32 ? 4 : 8, cg = C / G, keep = dtype == GRIDGCN_F32 ? KEEP<float> : KEEP<gg_bf16>;
     p.nq = save8 ? gg_a8_cp(C) / V : (C + V - 1) / V;
-    // whole groups, whole chunks (whole blocks of the 8-bit form), at least 64 bytes of a row
+    // whole groups, whole chunks (whole blocks of the 8-bit form)
     const long long unit = save8 ? GG_A8_BLOCK : V;
     long long slab = (long long)cg / gcd_ll(cg, unit) * unit;
     const long long least = 64 / (dtype == GRIDGCN_F32 ? 4 : 2);
     if (slab < least) slab = (least + slab - 1) / slab * slab;
     if (slab > C) slab = C;
-    const long long per = N * slab;
     auto quads = [&](long long s) { return save8 ? (s + GG_A8_BLOCK - 1) / GG_A8_BLOCK * (GG_A8_BLOCK / V) : (s + V - 1) / V; };
-    p.small = per <= SMALL_VALUES && quads(slab) <= THREADS;
+    auto fits = [&](long long s) { return quads(s) <= FEW && N <= (long long)keep * (FEW / quads(s)); };
+    p.small = fits(slab);
     if (p.small) {
         // short rows are taken whole: a workgroup for 16 channels of one row would be all start-up
-        while (slab < C && N * slab * 2 <= 2048 && quads(slab * 2) <= THREADS) slab *= 2;
+        while (slab < C && N * slab * 2 <= 2048 && fits(slab * 2)) slab *= 2;
         if (slab > C) slab = C;
         p.slab_c = (int)slab;
         p.slabs = (int)((C + slab - 1) / slab);
-        p.l = lay_of((int)quads(slab));
-    }
-    if (!p.small) {
+        p.l = lay_of((int)quads(slab), FEW);
+    } else {
         p.l = lay_of(p.nq);
         const long long slabs = (p.nq + p.l.tpr - 1) / p.l.tpr, step = (long long)p.l.rpb * UNROLL;
         long long want = (2048 + B * slabs - 1) / (B * slabs);      // workgroups: two generations of four per CU
@@ -684,10 +831,10 @@ Plan plan_of(int B, long long N, int C, int G, int dtype, bool save8)
     size_t o = 0;
     auto take = [&o](size_t n) { const size_t at = o; o += (n + 255) & ~(size_t)255; return at; };
     p.off_part = take(p.small ? 0 : (size_t)B * p.chunks * C * 16);
-    p.off_tot = take((size_t)B * C * 16);
-    p.off_coef = take((size_t)B * G * 8);
-    p.off_stats = take((size_t)B * G * 16);
-    p.bytes = o ? o : 256;
+    p.off_tot = take(backward && (!p.small || B > 1) ? (size_t)B * C * 16 : 0);
+    p.off_coef = take(backward && !p.small ? (size_t)B * G * 8 : 0);
+    p.off_stats = take(backward || stats || p.small ? 0 : (size_t)B * G * 16);
+    p.bytes = o;
     return p;
 }
 
@@ -703,7 +850,7 @@ template <class F> int with_type(int dtype, F f)
 template <class T, int ACT, bool SAVE8> void launch_fwd(Args &a, const Plan &p, hipStream_t st)
 {
     if (p.small) {
-        gg_k_gn_small<T, ACT, SAVE8><<<dim3(p.slabs, a.B), THREADS, 0, st>>>(a, p.l, p.slab_c);
+        gg_k_gn_small<T, ACT, SAVE8><<<dim3(p.slabs, a.B), FEW, 0, st>>>(a, p.l, p.slab_c);
         return;
     }
     const unsigned slabs = (p.nq + p.l.tpr - 1) / p.l.tpr;
@@ -717,7 +864,7 @@ template <class T, int ACT, bool SAVE8> void launch_fwd(Args &a, const Plan &p, 
 template <class T, int ACT, bool Q8> void launch_bwd(Args &a, const Plan &p, hipStream_t st)
 {
     if (p.small) {
-        gg_k_gn_small_bwd<T, ACT, Q8><<<dim3(p.slabs, a.B), THREADS, 0, st>>>(a, p.l, p.slab_c);
+        gg_k_gn_small_bwd<T, ACT, Q8><<<dim3(p.slabs, a.B), FEW, 0, st>>>(a, p.l, p.slab_c);
         if (a.B > 1 && (a.dgamma || a.dbeta)) gg_k_gn_params<<<dim3((a.C + THREADS - 1) / THREADS), THREADS, 0, st>>>(a);
         return;
     }
@@ -753,12 +900,11 @@ bool type_ok(int t) { return t == GRIDGCN_F32 || t == GRIDGCN_BF16 || t == GRIDG
 
 extern "C" {
 
-int gridgcn_group_norm_act_workspace_bytes(int B, long long N, int C, int G, int dtype, int save8, size_t *bytes)
+int gridgcn_group_norm_act_workspace_bytes(int B, long long N, int C, int G, int dtype, int save8, int stats, int backward,
+                                           size_t *bytes)
 {
     if (!bytes || !sizes_ok(B, N, C, G) || !type_ok(dtype)) return GRIDGCN_EINVAL;
-    // (the backward's plan has no padded channels: take the larger of the two)
-    const Plan f = plan_of(B, N, C, G, dtype, save8 != 0), b = plan_of(B, N, C, G, dtype, false);
-    *bytes = f.bytes > b.bytes ? f.bytes : b.bytes;
+    *bytes = plan_of(B, N, C, G, dtype, save8 && !backward, stats != 0, backward != 0).bytes;
     return GRIDGCN_OK;
 }
 
@@ -766,16 +912,16 @@ int gridgcn_group_norm_act_fwd(const void *x, int dtype, int B, long long N, int
                                const void *gamma, const void *beta, int ptype, const int32_t *counts, float eps, int act,
                                void *y, double *stats, uint8_t *codes, uint8_t *scales, void *ws, size_t ws_bytes, void *stream)
 {
-    if (!x || !y || !sizes_ok(B, N, C, G) || !type_ok(dtype) || !type_ok(ptype) || ldn < C || (B > 1 && ldb < 0) ||
+    if (!x || !y || !sizes_ok(B, N, C, G) || !type_ok(dtype) || !type_ok(ptype) || ldn < C || ldn > GRIDGCN_MAX_LD || (B > 1 && ldb < 0) ||
         !(eps >= 0.f) || act < GRIDGCN_ACT_NONE || act > GRIDGCN_ACT_GELU || !codes != !scales || ((uintptr_t)codes & 15))
         return GRIDGCN_EINVAL;
-    const Plan p = plan_of(B, N, C, G, dtype, codes != nullptr);
-    if (!ws || ws_bytes < p.bytes) return GRIDGCN_EWORKSPACE;
+    const Plan p = plan_of(B, N, C, G, dtype, codes != nullptr, stats != nullptr, false);
+    if (p.bytes && (!ws || ws_bytes < p.bytes)) return GRIDGCN_EWORKSPACE;
     Args a = {};
     a.x = x; a.y = y; a.N = N; a.xb = ldb; a.xn = ldn; a.B = B; a.C = C; a.G = G; a.cg = C / G; a.ptype = ptype;
     a.gamma = gamma; a.beta = beta; a.counts = counts; a.eps = eps; a.codes_out = codes; a.scales_out = scales;
     a.part = (double *)((char *)ws + p.off_part);
-    a.stats = stats ? stats : (double *)((char *)ws + p.off_stats);
+    a.stats = stats || p.small ? stats : (double *)((char *)ws + p.off_stats);
     a.rpc = p.rpc; a.chunks = p.chunks;
     const hipStream_t st = (hipStream_t)stream;
     const int rc = with_type(dtype, [&](auto *t) {
@@ -793,11 +939,12 @@ int gridgcn_group_norm_act_bwd(const void *dy, long long ldgb, long long ldgn, c
                                int act, void *dx, void *dgamma, void *dbeta, void *ws, size_t ws_bytes, void *stream)
 {
     if (!dy || !stats || !codes != !scales || (!x && !codes) || !sizes_ok(B, N, C, G) || !type_ok(dtype) || !type_ok(ptype) ||
-        ldgn < C || (x && !codes && ldn < C) || act < GRIDGCN_ACT_NONE || act > GRIDGCN_ACT_GELU || ((uintptr_t)codes & 15))
+        ldgn < C || ldgn > GRIDGCN_MAX_LD || (B > 1 && ldgb < 0) ||
+        (x && !codes && (ldn < C || ldn > GRIDGCN_MAX_LD || (B > 1 && ldb < 0))) || act < GRIDGCN_ACT_NONE || act > GRIDGCN_ACT_GELU || ((uintptr_t)codes & 15))
         return GRIDGCN_EINVAL;
     if (!dx && !dgamma && !dbeta) return GRIDGCN_OK;
-    const Plan p = plan_of(B, N, C, G, dtype, false);
-    if (!ws || ws_bytes < p.bytes) return GRIDGCN_EWORKSPACE;
+    const Plan p = plan_of(B, N, C, G, dtype, false, true, true);
+    if (p.bytes && (!ws || ws_bytes < p.bytes)) return GRIDGCN_EWORKSPACE;
     Args a = {};
     a.dy = dy; a.gb = ldgb; a.gn = ldgn; a.x = x; a.xb = ldb; a.xn = ldn; a.codes = codes; a.scales = scales;
     a.y = dx; a.N = N; a.B = B; a.C = C; a.G = G; a.cg = C / G; a.ptype = ptype; a.gamma = gamma; a.beta = beta;

@@ -42,6 +42,12 @@ __device__ __forceinline__ F16 zero16()
     return z;
 }
 
+// the low (c = 0) or high 16 bits of two registers as one
+__device__ __forceinline__ unsigned gg_pair16(unsigned a, unsigned b, int c)
+{
+    return (unsigned)__builtin_amdgcn_perm(b, a, c ? 0x07060302u : 0x05040100u);
+}
+
 // two floats as three bf16 pairs
 __device__ __forceinline__ void split2(float a, float b, unsigned &h, unsigned &m, unsigned &l)
 {
@@ -52,54 +58,44 @@ __device__ __forceinline__ void split2(float a, float b, unsigned &h, unsigned &
     l = gg_cvt_bf16(a, b);
 }
 
-// acc += A B from the pieces of both, the smallest partial products first
-template <class T, int PA, int PB>
-__device__ __forceinline__ F16 mul(const gg_u32x4 (&a)[PA], const gg_u32x4 (&b)[PB], F16 c)
+// acc[t] += A B[t] from the pieces of both, the smallest partial products first; neighbouring instructions on different tiles
+template <class T, int NT, int PA, int PB>
+__device__ __forceinline__ void mul(const gg_u32x4 (&a)[PA], const gg_u32x4 (&b)[NT][PB], F16 (&c)[NT])
 {
-    if constexpr (PA == 3 && PB == 3) {
-        c = Ty<T>::mfma(a[2], b[0], c);
-        c = Ty<T>::mfma(a[1], b[1], c);
-        c = Ty<T>::mfma(a[0], b[2], c);
-        c = Ty<T>::mfma(a[1], b[0], c);
-        c = Ty<T>::mfma(a[0], b[1], c);
-        return Ty<T>::mfma(a[0], b[0], c);
-    } else if constexpr (PA == 3) {
-        c = Ty<T>::mfma(a[2], b[0], c);
-        c = Ty<T>::mfma(a[1], b[0], c);
-        return Ty<T>::mfma(a[0], b[0], c);
-    } else {
-        return Ty<T>::mfma(a[0], b[0], c);
-    }
+    auto one = [&](int i, int j) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) c[t] = Ty<T>::mfma(a[i], b[t][j], c[t]);
+    };
+    if constexpr (PA == 3 && PB == 3) { one(2, 0); one(1, 1); one(0, 2); one(1, 0); one(0, 1); }
+    else if constexpr (PA == 3) { one(2, 0); one(1, 0); }
+    one(0, 0);
 }
 
-// ---- 32 consecutive channels of a row: a lane's share of a contraction step of 64 -----------------------------------
+// ---- 64 bytes of a row: a lane's share of a contraction step.  A step is KS channels (128 bytes of a row: a line), the half-wave h
+// takes the KS / 2 from KS / 2 * h on -- any order serves a contraction, as long as both operands have it -- so a lane's loads are
+// neighbours and the two halves share a line. ----------------------------------------------------------------------------
+template <class T> constexpr int KS = 128 / (int)sizeof(T);
+template <class T> constexpr int SS = KS<T> / 16;        // matrix instructions of a step: 8 channels of each half
 template <class T> struct Block {
-    static constexpr int NW = 2 * (int)sizeof(T);    // 16-byte words
-    static constexpr int VW = 16 / (int)sizeof(T);
-    gg_u32x4 w[NW];
+    static constexpr int VW = 16 / (int)sizeof(T), CH = 4 * VW;
+    gg_u32x4 w[4];
+    __device__ __forceinline__ void load_full(const T *q)
+    {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if constexpr (sizeof(T) == 4) w[i] = *(const gg_u32x4_a4 *)(q + i * VW);
+            else w[i] = *(const gg_u32x4_a2 *)(q + i * VW);
+        }
+    }
+    // channels k0 .. k0 + CH - 1 of a row of K, zeros behind it
     __device__ __forceinline__ void load(const T *row, int k0, int K)
     {
 #pragma unroll
-        for (int i = 0; i < NW; i++) {
-            const int k = k0 + i * VW;
-            if (k + VW <= K) {
-                if constexpr (sizeof(T) == 4) w[i] = *(const gg_u32x4_a4 *)(row + k);
-                else w[i] = *(const gg_u32x4_a2 *)(row + k);
-            } else {
-                gg_u32x4 u = {0u, 0u, 0u, 0u};
-                if (k < K) {
-                    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-                        for (int j = 0; j < 4; j++)
-                            if (k + j < K) u[j] = ((const unsigned *)row)[k + j];
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 8; j++)
-                            if (k + j < K) u[j / 2] |= (unsigned)((const unsigned short *)row)[k + j] << (16 * (j & 1));
-                    }
-                }
-                w[i] = u;
-            }
+        for (int i = 0; i < 4; i++) {
+            GGChunk<T> c;
+            c.zero();
+            if (k0 + i * VW < K) c.load(row, k0 + i * VW, K);
+            w[i] = c.w;
         }
     }
     // channels 8 s .. 8 s + 7 as a matrix operand
@@ -122,28 +118,47 @@ template <class T> struct Block {
         else if constexpr (std::is_same<T, gg_bf16>::value) return (i & 1) ? gg_hi16f(w[i / 8][(i % 8) / 2]) : gg_lo16f(w[i / 8][(i % 8) / 2]);
         else return gg_f16of(w[i / 8][(i % 8) / 2], i & 1);
     }
-    // the 8-bit form of the 32: the lane holds the whole block, no lane is asked
-    __device__ __forceinline__ void save(uint8_t *codes, uint8_t *scale) const
+    // the 8-bit form: 16-bit rows, the lane holds a block of 32; 32-bit rows, the two halves hold one together (every lane of
+    // the wave calls; `on`: this lane stores).  k: first channel of the lane's share, in a row of Cp padded channels
+    __device__ __forceinline__ void save(uint8_t *codes, uint8_t *scales, int k, bool on) const
     {
-        unsigned m = 0;
+        auto top = [&](bool finite) {
+            unsigned m = 0;
 #pragma unroll
-        for (int i = 0; i < 32; i++) {
-            const unsigned u = gg_a8_mag(get(i));
-            m = m > u ? m : u;
-        }
+            for (int i = 0; i < CH; i++) {
+                const unsigned u = finite ? gg_a8_mag(get(i)) : __float_as_uint(get(i)) & 0x7fffffffu;
+                m = m > u ? m : u;
+            }
+            if constexpr (CH == 16) {
+                const unsigned o = (unsigned)__shfl_xor((int)m, 32);
+                m = m > o ? m : o;
+            }
+            return m;
+        };
+        unsigned m = top(false);
+        const bool clean = !__any(m >= 0x7f800000u);                  // (as gg_a8_block_byte)
+        if (!clean) m = top(true);
         const unsigned byte = gg_a8_byte(m);
         const float s = gg_a8_unscale(byte);
+        Block b = *this;
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < 4; i++) asm volatile("" : "+v"(b.w[i]));  // (16-bit rows: unpacked again, not held unpacked)
+        if (!on) return;
+#pragma unroll
+        for (int i = 0; i < CH / 16; i++) {
             gg_u32x4 o;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const int e = 16 * i + 4 * j;
-                o[j] = gg_a8_enc4(gg_a8_ready(get(e), s), gg_a8_ready(get(e + 1), s), gg_a8_ready(get(e + 2), s), gg_a8_ready(get(e + 3), s));
+                float v[4];
+                unsigned w[1];
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = b.get(16 * i + 4 * j + e);
+                gg_a8_encode<4>(v, byte, clean, w);
+                o[j] = w[0];
             }
-            *(gg_u32x4 *)(codes + 16 * i) = o;
+            *(gg_u32x4 *)(codes + k + 16 * i) = o;
         }
-        *scale = (uint8_t)byte;
+        if (k % 32 == 0) scales[k / 32] = (uint8_t)byte;
     }
 };
 
@@ -170,74 +185,85 @@ __device__ __forceinline__ bool place(const Mm &p, unsigned &row, unsigned &col)
 }
 unsigned place_grid(unsigned nrow, unsigned ncol) { return (nrow + 7) / 8 * 8 * ncol; }
 
-// W of a contraction step (64 channels) in LDS, in operand order: [tile of 32 columns][s of 4][piece][lane], 16 bytes each; the
-// lanes 32.. start one slot later so that the eight k-groups of a column land on different banks when they are written.
+// W of a contraction step in LDS, in operand order: [tile of 32 columns][s][piece][lane], 16 bytes each; the lanes 32.. start one
+// slot later, so that the k-groups of a column land on different banks when they are written.
 // Tile nt holds the columns NT * j + nt: a lane's NT results of a row are then neighbours in memory.
 constexpr int FRAG = 66 * 16;
 
 template <class T, bool TRANS, int NT, int THREADS> struct Wstage {
-    static constexpr int P = Ty<T>::P;
-    static constexpr int ITEMS_ALL = TRANS ? 8 * NT * 16 : 8 * NT * 32;
+    static constexpr int P = Ty<T>::P, S = SS<T>, G = 2 * S;          // G groups of 8 consecutive channels in a step
+    static constexpr int ITEMS_ALL = TRANS ? G * NT * 16 : G * NT * 32;
     static constexpr int ITEMS = (ITEMS_ALL + THREADS - 1) / THREADS;
-    static constexpr int BYTES = NT * 4 * P * FRAG;
+    static constexpr int BYTES = NT * S * P * FRAG;
     // not TRANS: 8 consecutive k of a column; TRANS: 8 consecutive k (rows of w) of two neighbouring columns
     static constexpr int WORDS = TRANS ? (sizeof(T) == 4 ? 16 : 8) : (sizeof(T) == 4 ? 8 : 4);
     unsigned r[ITEMS][WORDS];
+    static_assert(ITEMS_ALL % THREADS == 0, "every thread has the same number of items");
 
-    __device__ __forceinline__ void load(const Mm &p, int n0, int k0)
+    // A step whose channels all exist.  Columns behind the last are other columns: nobody stores their results.  (TRANS: N >= 2)
+    __device__ __forceinline__ void load_full(const Mm &p, int n0, int k0)
     {
         const T *w = (const T *)p.w;
 #pragma unroll
         for (int i = 0; i < ITEMS; i++) {
             const int e = (int)threadIdx.x + i * THREADS;
-#pragma unroll
-            for (int j = 0; j < WORDS; j++) r[i][j] = 0u;
-            if (e >= ITEMS_ALL) continue;
             if constexpr (!TRANS) {
-                const int k = k0 + 8 * (e & 7), n = n0 + (e >> 3);
-                if (n >= p.N) continue;
-                const T *q = w + (size_t)n * p.K + k;
-                if (k + 8 <= p.K) {
+                const int n = n0 + e / G;
+                const T *q = w + (size_t)(n < p.N ? n : p.N - 1) * p.K + k0 + 8 * (e % G);
 #pragma unroll
-                    for (int j = 0; j < WORDS / 4; j++) {
-                        gg_u32x4 u;
-                        if constexpr (sizeof(T) == 4) u = *(const gg_u32x4_a4 *)(q + 4 * j);
-                        else u = *(const gg_u32x4_a2 *)q;
+                for (int j = 0; j < WORDS / 4; j++) {
+                    gg_u32x4 u;
+                    if constexpr (sizeof(T) == 4) u = *(const gg_u32x4_a4 *)(q + 4 * j);
+                    else u = *(const gg_u32x4_a2 *)q;
 #pragma unroll
-                        for (int t = 0; t < 4; t++) r[i][4 * j + t] = u[t];
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        if (k + j >= p.K) continue;
-                        if constexpr (sizeof(T) == 4) r[i][j] = ((const unsigned *)q)[j];
-                        else r[i][j / 2] |= (unsigned)((const unsigned short *)q)[j] << (16 * (j & 1));
-                    }
+                    for (int t = 0; t < 4; t++) r[i][4 * j + t] = u[t];
                 }
             } else {
-                const int n = n0 + 2 * (e % (NT * 16)), k = k0 + 8 * (e / (NT * 16));
-                if (n >= p.N) continue;
+                const int n = n0 + 2 * (e % (NT * 16));
+                const bool last = n + 1 >= p.N;                      // (the pair in front; its second is column N - 1)
+                const T *q = w + (size_t)(k0 + 8 * (e / (NT * 16))) * p.N + (last ? p.N - 2 : n);
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    if (k + j >= p.K) continue;
-                    const T *q = w + (size_t)(k + j) * p.N + n;
                     if constexpr (sizeof(T) == 4) {
-                        r[i][2 * j] = ((const unsigned *)q)[0];
-                        if (n + 1 < p.N) r[i][2 * j + 1] = ((const unsigned *)q)[1];
+                        const gg_u32x2 u = *(const gg_u32x2_a4 *)(q + (size_t)j * p.N);
+                        r[i][2 * j] = last ? u[1] : u[0];
+                        r[i][2 * j + 1] = u[1];
                     } else {
-                        r[i][j] = ((const unsigned short *)q)[0];
-                        if (n + 1 < p.N) r[i][j] |= (unsigned)((const unsigned short *)q)[1] << 16;
+                        const unsigned u = *(const gg_u32_a2 *)(q + (size_t)j * p.N);
+                        r[i][j] = last ? u >> 16 : u;
                     }
                 }
             }
         }
     }
+    // the last step, from channel k0 on: zeros behind K
+    __device__ __forceinline__ void load_tail(const Mm &p, int n0, int k0)
+    {
+        const T *w = (const T *)p.w;
+#pragma unroll
+        for (int i = 0; i < ITEMS; i++) {
+            const int e = (int)threadIdx.x + i * THREADS;
+            const int n = n0 + (TRANS ? 2 * (e % (NT * 16)) : e / G), k = k0 + 8 * (TRANS ? e / (NT * 16) : e % G);
+#pragma unroll
+            for (int j = 0; j < WORDS; j++) r[i][j] = 0u;
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+#pragma unroll
+                for (int c = 0; c < (TRANS ? 2 : 1); c++) {
+                    if (k + j >= p.K || n + c >= p.N) continue;
+                    const T *q = w + (TRANS ? (size_t)(k + j) * p.N + n + c : (size_t)n * p.K + k + j);
+                    const int at = TRANS ? 2 * j + c : j;            // element of the item
+                    if constexpr (sizeof(T) == 4) r[i][at] = *(const unsigned *)q;
+                    else r[i][at / 2] |= (unsigned)*(const unsigned short *)q << (16 * (at & 1));
+                }
+        }
+    }
 
     static __device__ __forceinline__ void put(char *lds, int nl, int k8, const gg_u32x4 (&f)[P])
     {
-        const int nt = nl % NT, j = nl / NT, h = k8 >> 2, s = k8 & 3;
+        const int nt = nl % NT, j = nl / NT, h = k8 / S, s = k8 % S;
 #pragma unroll
-        for (int q = 0; q < P; q++) *(gg_u32x4 *)(lds + ((nt * 4 + s) * P + q) * FRAG + (h * 33 + j) * 16) = f[q];
+        for (int q = 0; q < P; q++) *(gg_u32x4 *)(lds + ((nt * S + s) * P + q) * FRAG + (h * 33 + j) * 16) = f[q];
     }
 
     __device__ __forceinline__ void store(char *lds) const
@@ -245,7 +271,6 @@ template <class T, bool TRANS, int NT, int THREADS> struct Wstage {
 #pragma unroll
         for (int i = 0; i < ITEMS; i++) {
             const int e = (int)threadIdx.x + i * THREADS;
-            if (e >= ITEMS_ALL) continue;
             if constexpr (!TRANS) {
                 gg_u32x4 f[P];
                 if constexpr (sizeof(T) == 4) {
@@ -258,7 +283,7 @@ template <class T, bool TRANS, int NT, int THREADS> struct Wstage {
                 } else {
                     f[0] = gg_u32x4{r[i][0], r[i][1], r[i][2], r[i][3]};
                 }
-                put(lds, e >> 3, e & 7, f);
+                put(lds, e / G, e % G, f);
             } else {
                 const int nl = 2 * (e % (NT * 16)), k8 = e / (NT * 16);
 #pragma unroll
@@ -271,7 +296,7 @@ template <class T, bool TRANS, int NT, int THREADS> struct Wstage {
                             split2(__uint_as_float(r[i][4 * j + c]), __uint_as_float(r[i][4 * j + 2 + c]), h, m, l);
                             f[0][j] = h; f[1][j] = m; f[2][j] = l;
                         } else {
-                            f[0][j] = c == 0 ? (r[i][2 * j] & 0xffffu) | (r[i][2 * j + 1] << 16) : (r[i][2 * j] >> 16) | (r[i][2 * j + 1] & 0xffff0000u);
+                            f[0][j] = gg_pair16(r[i][2 * j], r[i][2 * j + 1], c);
                         }
                     }
                     put(lds, nl + c, k8, f);
@@ -300,95 +325,97 @@ template <class T, int NT> __device__ __forceinline__ void put_row(T *y, long lo
     }
 }
 
-// ---- many rows: a wave owns MR x 32 rows and 32 NT columns, its rows straight from memory into registers (each row is read by
-// one wave only), W through LDS, the next step of both in flight while this one is multiplied -------------------------------
-template <class T, bool TRANS, bool SAVE, int NT, int WAVES, int MR>
-__global__ __launch_bounds__(WAVES * 64) void gg_k_lin8(Mm p)
+// ---- many rows: a wave owns 32 rows and 32 NT columns, its rows straight from memory into registers (each row is read by one wave
+// only), W through LDS, the next step of both in flight while this one is multiplied; three or four workgroups per CU, so that
+// one's barriers and stores are another's matrix instructions ----------------------------------------------------------------
+constexpr int MW = 4;             // waves
+template <class T, bool TRANS, bool SAVE, int NT>
+__global__ __launch_bounds__(MW * 64, 3) void gg_k_lin8(Mm p)
 {
-    constexpr int P = Ty<T>::P, THREADS = WAVES * 64;
-    typedef Wstage<T, TRANS, NT, THREADS> W;
+    constexpr int P = Ty<T>::P, S = SS<T>;
+    typedef Wstage<T, TRANS, NT, MW * 64> W;
     extern __shared__ __attribute__((aligned(16))) char lds8[];
     unsigned brow, bcol;
     if (!place(p, brow, bcol)) return;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, j = lane & 31;
     const int n0 = (int)bcol * 32 * NT;
-    const long long m0 = (long long)brow * (WAVES * MR * 32) + wave * (MR * 32);
-    const int Cp = gg_a8_cp(p.K);
-    const int steps = (p.K + 63) / 64;
-    const T *rows[MR];
-    bool live[MR];
+    const long long m0 = (long long)brow * (MW * 32) + wave * 32, r = m0 + j;
+    const bool live = r < p.R;
+    const int Cp = gg_a8_cp(p.K), steps = (p.K + KS<T> - 1) / KS<T>, kh = KS<T> / 2 * h;
+    const T *row = (const T *)p.a + (size_t)(live ? r : p.R - 1) * p.lda;
+    F16 acc[NT];
 #pragma unroll
-    for (int m = 0; m < MR; m++) {
-        const long long r = m0 + m * 32 + j;
-        live[m] = r < p.R;
-        rows[m] = (const T *)p.a + (size_t)(live[m] ? r : p.R - 1) * p.lda;
-    }
-    F16 acc[MR][NT];
-#pragma unroll
-    for (int m = 0; m < MR; m++)
-#pragma unroll
-        for (int t = 0; t < NT; t++) acc[m][t] = zero16();
+    for (int t = 0; t < NT; t++) acc[t] = zero16();
 
-    W ws;
-    Block<T> a[MR];
-    ws.load(p, n0, 0);
-#pragma unroll
-    for (int m = 0; m < MR; m++) a[m].load(rows[m], 32 * h, p.K);
-    ws.store(lds8);
-    __syncthreads();
-    for (int st = 0; st < steps; st++) {
-        const char *cur = lds8 + (st & 1) * W::BYTES;
-        Block<T> nx[MR];
-        const bool more = st + 1 < steps;
-        if (more) {
-            ws.load(p, n0, 64 * (st + 1));
-#pragma unroll
-            for (int m = 0; m < MR; m++) nx[m].load(rows[m], 64 * (st + 1) + 32 * h, p.K);
-        }
+    auto keep = [&](const Block<T> &b, int st) {
         if (SAVE && bcol == 0) {
-            const int blk = 2 * st + h;
+            const int k = st * KS<T> + kh;
+            b.save(p.codes + (size_t)r * Cp, p.scales + (size_t)r * (Cp / 32), k, live && k < Cp);
+        }
+    };
+    auto multiply = [&](const Block<T> &b, const char *cur) {
 #pragma unroll
-            for (int m = 0; m < MR; m++) {
-                const long long r = m0 + m * 32 + j;
-                if (live[m] && blk * 32 < p.K) a[m].save(p.codes + (size_t)r * Cp + blk * 32, p.scales + (size_t)r * (Cp / 32) + blk);
+        for (int s = 0; s < S; s++) {
+            gg_u32x4 fa[P];
+            b.frag(s, fa);
+#pragma unroll
+            for (int t = 0; t < NT; t += 2) {                     // (two tiles at a time: independent neighbours, few registers)
+                gg_u32x4 fb[2][P];
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int q = 0; q < P; q++) fb[u][q] = *(const gg_u32x4 *)(cur + (((t + u) * S + s) * P + q) * FRAG + (h * 33 + j) * 16);
+                F16(&two)[2] = *(F16(*)[2])&acc[t];
+                mul<T>(fa, fb, two);
             }
         }
-#pragma unroll
-        for (int s = 0; s < 4; s++) {
-            gg_u32x4 fa[MR][P];
-#pragma unroll
-            for (int m = 0; m < MR; m++) a[m].frag(s, fa[m]);
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                gg_u32x4 fb[P];
-#pragma unroll
-                for (int q = 0; q < P; q++) fb[q] = *(const gg_u32x4 *)(cur + ((t * 4 + s) * P + q) * FRAG + (h * 33 + j) * 16);
-#pragma unroll
-                for (int m = 0; m < MR; m++) acc[m][t] = mul<T>(fa[m], fb, acc[m][t]);
-            }
-        }
-        if (more) {
-            ws.store(lds8 + ((st + 1) & 1) * W::BYTES);
-#pragma unroll
-            for (int m = 0; m < MR; m++) a[m] = nx[m];
-        }
+    };
+    const int full = p.K / KS<T>;
+    if (full) {
+        W ws;
+        Block<T> a, nx;
+        ws.load_full(p, n0, 0);
+        a.load_full(row + kh);
+        ws.store(lds8);
         __syncthreads();
+        for (int st = 0; st < full; st++) {
+            const bool more = st + 1 < full;
+            if (more) {
+                ws.load_full(p, n0, (st + 1) * KS<T>);
+                nx.load_full(row + (st + 1) * KS<T> + kh);
+            }
+            keep(a, st);
+            multiply(a, lds8 + (st & 1) * W::BYTES);
+            if (more) {
+                ws.store(lds8 + ((st + 1) & 1) * W::BYTES);
+                a = nx;
+            }
+            __syncthreads();
+        }
+    }
+    if (full < steps) {
+        W ws;
+        Block<T> a;
+        ws.load_tail(p, n0, full * KS<T>);
+        a.load(row, full * KS<T> + kh, p.K);
+        ws.store(lds8 + (full & 1) * W::BYTES);
+        __syncthreads();
+        keep(a, full);
+        multiply(a, lds8 + (full & 1) * W::BYTES);
     }
     const int n = n0 + NT * j;
     float b[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) b[t] = n + t < p.N ? gg_ld_param(p.bias, GGRowT<T>::id, n + t, 0.f) : 0.f;
 #pragma unroll
-    for (int m = 0; m < MR; m++)
+    for (int i = 0; i < 16; i++) {
+        const long long o = m0 + ggm_row(i, lane);
+        if (o >= p.R) continue;
+        float v[NT];
 #pragma unroll
-        for (int r = 0; r < 16; r++) {
-            const long long row = m0 + m * 32 + ggm_row(r, lane);
-            if (row >= p.R) continue;
-            float v[NT];
-#pragma unroll
-            for (int t = 0; t < NT; t++) v[t] = acc[m][t][r] + b[t];
-            put_row<T, NT>((T *)p.y, row, n, p.N, v);
-        }
+        for (int t = 0; t < NT; t++) v[t] = acc[t][i] + b[t];
+        put_row<T, NT>((T *)p.y, o, n, p.N, v);
+    }
 }
 
 // ---- few rows: a workgroup owns 32 x 32 results, its waves share the contraction (a step of 64 each in turn) and add up in LDS;
@@ -404,42 +431,39 @@ __global__ __launch_bounds__(SW * 64) void gg_k_lin8_few(Mm p)
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, j = lane & 31;
     const int n = (int)bcol * 32 + j;
     const long long r = (long long)brow * 32 + j;
-    const int Cp = gg_a8_cp(p.K), steps = (p.K + 63) / 64;
+    const int Cp = gg_a8_cp(p.K), steps = (p.K + KS<T> - 1) / KS<T>;
     const T *row = (const T *)p.a + (size_t)(r < p.R ? r : p.R - 1) * p.lda;
     const T *w = (const T *)p.w;
-    F16 acc = zero16();
+    const int nn = n < p.N ? n : p.N - 1;
+    F16 acc[1] = {zero16()};
     for (int st = wave; st < steps; st += SW) {
-        const int k0 = 64 * st + 32 * h;
+        const int k0 = KS<T> * st + KS<T> / 2 * h;
         Block<T> a, b;
         a.load(row, k0, p.K);
         if constexpr (!TRANS) {
-            b.load(w + (size_t)(n < p.N ? n : p.N - 1) * p.K, k0, p.K);
+            b.load(w + (size_t)nn * p.K, k0, p.K);
         } else {
-            const int nn = n < p.N ? n : p.N - 1;
 #pragma unroll
-            for (int i = 0; i < Block<T>::NW; i++) b.w[i] = gg_u32x4{0u, 0u, 0u, 0u};
+            for (int i = 0; i < 4; i++) b.w[i] = gg_u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
-            for (int i = 0; i < 32; i++) {
+            for (int i = 0; i < Block<T>::CH; i++) {
                 if (k0 + i >= p.K) continue;
                 const T *q = w + (size_t)(k0 + i) * p.N + nn;
                 if constexpr (sizeof(T) == 4) b.w[i / 4][i % 4] = *(const unsigned *)q;
                 else b.w[i / 8][(i % 8) / 2] |= (unsigned)*(const unsigned short *)q << (16 * (i & 1));
             }
         }
-        if (SAVE && bcol == 0) {
-            const int blk = 2 * st + h;
-            if (r < p.R && blk * 32 < p.K) a.save(p.codes + (size_t)r * Cp + blk * 32, p.scales + (size_t)r * (Cp / 32) + blk);
-        }
+        if (SAVE && bcol == 0) a.save(p.codes + (size_t)r * Cp, p.scales + (size_t)r * (Cp / 32), k0, r < p.R && k0 < Cp);
 #pragma unroll
-        for (int s = 0; s < 4; s++) {
-            gg_u32x4 fa[P], fb[P];
+        for (int s = 0; s < SS<T>; s++) {
+            gg_u32x4 fa[P], fb[1][P];
             a.frag(s, fa);
-            b.frag(s, fb);
-            acc = mul<T>(fa, fb, acc);
+            b.frag(s, fb[0]);
+            mul<T>(fa, fb, acc);
         }
     }
 #pragma unroll
-    for (int i = 0; i < 16; i++) part[wave][i][lane] = acc[i];
+    for (int i = 0; i < 16; i++) part[wave][i][lane] = acc[0][i];
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 16 / SW; i++) {
@@ -463,7 +487,7 @@ constexpr int GT = 128;           // results of a tile per side
 constexpr int GW = 4;             // waves
 struct Wg {
     const void *dy;               // [R][N], stride ldy
-    const uint8_t *codes, *scales; // NULL: no dw, only db (tk = 1)
+    const uint8_t *codes, *scales; // without dw (tk = 1): any readable bytes, Cp = 0
     void *dw, *db;                // [N][K], [N]
     float *part, *dbpart;         // splits > 1: [split][tile][128][128], [split][tiles_n * 128]
     long long R, ldy;
@@ -475,36 +499,46 @@ template <class T> struct Strip {
     static constexpr int DW = sizeof(T) == 4 ? 4 : 2;
     unsigned d[8][DW];
     unsigned c[8], s[8];
-    __device__ __forceinline__ void load(const Wg &p, long long r0, int n, int k, bool rows)
+    // rows 8 h + 0..7 of a strip that lies inside: `dy`, `codes`, `scales` are the strip's first row (uniform), od / oc / os the lane's
+    // byte offsets: no arithmetic per load
+    __device__ __forceinline__ void load_full(const Wg &p, const char *dy, const char *codes, const char *scales, unsigned od, unsigned oc,
+                                              unsigned os)
+    {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const char *q = dy + (size_t)i * p.ldy * sizeof(T);
+            if constexpr (sizeof(T) == 4) {
+                const gg_u32x4 u = *(const gg_u32x4_a4 *)(q + od);
+#pragma unroll
+                for (int t = 0; t < 4; t++) d[i][t] = u[t];
+            } else {
+                const gg_u32x2 u = *(const gg_u32x2_a2 *)(q + od);
+                d[i][0] = u[0]; d[i][1] = u[1];
+            }
+            c[i] = *(const unsigned *)(codes + (size_t)i * p.Cp + oc);
+            s[i] = *(const uint8_t *)(scales + (size_t)i * (p.Cp / 32) + os);
+        }
+    }
+    // ... of a strip that may end behind the last row or column
+    __device__ __forceinline__ void load_tail(const Wg &p, long long r0, int n, int k)
     {
         const int nb = p.Cp / 32;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const long long r = r0 + i;
-            const bool in = rows && r < p.R;
+            const bool in = r < p.R;
             const T *q = (const T *)p.dy + (size_t)(in ? r : 0) * p.ldy + n;
 #pragma unroll
             for (int t = 0; t < DW; t++) d[i][t] = 0u;
             c[i] = 0u;
             s[i] = GG_A8_MIN_BYTE;
-            if (in && n + 4 <= p.N) {
-                if constexpr (sizeof(T) == 4) {
-                    const gg_u32x4 u = *(const gg_u32x4_a4 *)q;
 #pragma unroll
-                    for (int t = 0; t < 4; t++) d[i][t] = u[t];
-                } else {
-                    const gg_u32x2 u = *(const gg_u32x2_a2 *)q;
-                    d[i][0] = u[0]; d[i][1] = u[1];
-                }
-            } else if (in && n < p.N) {
-#pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    if (n + t >= p.N) continue;
-                    if constexpr (sizeof(T) == 4) d[i][t] = ((const unsigned *)q)[t];
-                    else d[i][t / 2] |= (unsigned)((const unsigned short *)q)[t] << (16 * (t & 1));
-                }
+            for (int t = 0; t < 4; t++) {
+                if (!in || n + t >= p.N) continue;
+                if constexpr (sizeof(T) == 4) d[i][t] = ((const unsigned *)q)[t];
+                else d[i][t / 2] |= (unsigned)((const unsigned short *)q)[t] << (16 * (t & 1));
             }
-            if (in && p.codes && k < p.Cp) {
+            if (in && k < p.Cp) {
                 c[i] = *(const unsigned *)(p.codes + (size_t)r * p.Cp + k);
                 s[i] = p.scales[(size_t)r * nb + k / 32];
             }
@@ -526,8 +560,7 @@ template <class T> struct Strip {
                 split2(__uint_as_float(d[2 * q][t]), __uint_as_float(d[2 * q + 1][t]), h, m, l);
                 f[0][q] = h; f[1][q] = m; f[2][q] = l;
             } else {
-                const unsigned u = d[2 * q][t / 2], v = d[2 * q + 1][t / 2];
-                f[0][q] = (t & 1) ? (u >> 16) | (v & 0xffff0000u) : (u & 0xffffu) | (v << 16);
+                f[0][q] = gg_pair16(d[2 * q][t / 2], d[2 * q + 1][t / 2], t & 1);
             }
         }
     }
@@ -543,7 +576,7 @@ template <class T> struct Strip {
 #pragma unroll
             for (int t = 0; t < 4; t++) {
                 if constexpr (std::is_same<T, gg_f16>::value) f[t][0][q] = gg_cvt_f16(u[t] * su, v[t] * sv);
-                else f[t][0][q] = (__float_as_uint(u[t] * su) >> 16) | (__float_as_uint(v[t] * sv) & 0xffff0000u);
+                else f[t][0][q] = gg_pair16(__float_as_uint(u[t] * su), __float_as_uint(v[t] * sv), 1);
             }
         }
     }
@@ -553,46 +586,70 @@ template <class T>
 __global__ __launch_bounds__(GW * 64, 1) void gg_k_lin8_wgrad(Wg p)
 {
     constexpr int P = Ty<T>::P;
+    constexpr int D = 3;              // strips in flight (a wave's own: there is one per SIMD)
     extern __shared__ __attribute__((aligned(16))) float ldsf[];    // [GW][4][16][64]
     // (the tiles of one split read the same rows: same XCD, as in place())
     const unsigned tiles = p.tn * p.tk, id = blockIdx.x, xcd = id & 7, slot = id >> 3;
     const unsigned tile = slot % tiles, split = (slot / tiles) * 8 + xcd;
     if (split >= p.splits) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, j = lane & 31;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5, j = lane & 31;
     const int n0 = (int)(tile / p.tk) * GT, k0 = (int)(tile % p.tk) * GT, n = n0 + 4 * j, k = k0 + 4 * j;
     const bool first = tile % p.tk == 0;
     const long long strips = (p.R + 15) / 16, stride = (long long)p.splits * GW;
+    // Strips that are loaded unchecked.  What a lane reads behind the last column belongs to results that nobody stores (such lanes
+    // read the columns from 0 on, and at most 3 values behind a row's end: the rows of these strips have 4 more behind them).
+    const long long whole = p.R > 4 ? (p.R - 4) / 16 : 0;
+    const unsigned od = (unsigned)((8 * h * p.ldy + (n < p.N ? n : 0)) * (long long)sizeof(T));
+    const int kc = k < p.Cp ? k : 0;
+    const unsigned oc = (unsigned)(8 * h * p.Cp + kc), os = (unsigned)(8 * h * (p.Cp / 32) + kc / 32);
     F16 acc[4][4];
 #pragma unroll
     for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int t = 0; t < 4; t++) acc[i][t] = zero16();
     float dbs[4] = {0.f, 0.f, 0.f, 0.f};
-    long long g = (long long)split * GW + wave;
-    Strip<T> cur, nxt;
-    cur.load(p, g * 16 + 8 * h, n, k, g < strips);
-    for (; g < strips; g += stride) {
-        const long long gn = g + stride;
-        nxt.load(p, gn * 16 + 8 * h, n, k, gn < strips);
+    Strip<T> q[D];
+    auto fetch = [&](long long g, Strip<T> &s) {
+        if (g < whole)
+            s.load_full(p, (const char *)p.dy + (size_t)g * 16 * p.ldy * sizeof(T), (const char *)p.codes + (size_t)g * 16 * p.Cp,
+                        (const char *)p.scales + (size_t)g * 16 * (p.Cp / 32), od, oc, os);
+    };
+    auto use = [&](const Strip<T> &s) {
         gg_u32x4 fx[4][1];
-        cur.frag_x(fx);
+        s.frag_x(fx);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             gg_u32x4 fd[P];
-            cur.frag_dy(i, fd);
-#pragma unroll
-            for (int t = 0; t < 4; t++) acc[i][t] = mul<T>(fd, fx[t], acc[i][t]);
+            s.frag_dy(i, fd);
+            mul<T>(fd, fx, acc[i]);
         }
         if (first) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                float s = cur.dyv(0, i);
+                float v = s.dyv(0, i);
 #pragma unroll
-                for (int q = 1; q < 8; q++) s += cur.dyv(q, i);
-                dbs[i] += s;
+                for (int e = 1; e < 8; e++) v += s.dyv(e, i);
+                dbs[i] += v;
             }
         }
-        cur = nxt;
+    };
+    long long g = (long long)split * GW + wave;
+#pragma unroll
+    for (int d = 0; d < D - 1; d++) fetch(g + d * stride, q[d]);
+    while (g < whole) {
+#pragma unroll
+        for (int d = 0; d < D; d++) {
+            if (g < whole) {
+                fetch(g + (D - 1) * stride, q[(d + D - 1) % D]);
+                use(q[d]);
+                g += stride;
+            }
+        }
+    }
+    for (; g < strips; g += stride) {                             // (the last one or two strips of all)
+        Strip<T> s;
+        s.load_tail(p, g * 16 + 8 * h, n, k);
+        use(s);
     }
     // the waves' sums: a quarter of the tile's rows at a time
     float *pt = p.part ? p.part + ((size_t)split * tiles + tile) * GT * GT : nullptr;
@@ -673,34 +730,29 @@ __global__ __launch_bounds__(256) void gg_k_lin8_wsum(Wg p, unsigned nw)
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
-template <class T, bool TRANS, bool SAVE, int NT, int WAVES, int MR> int launch_many(Mm &p, hipStream_t st)
-{
-    constexpr int LDS = 2 * Wstage<T, TRANS, NT, WAVES * 64>::BYTES;
-    static GGDevOnce done;
-    if (!done) {
-        if (hipFuncSetAttribute((const void *)gg_k_lin8<T, TRANS, SAVE, NT, WAVES, MR>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess)
-            return GRIDGCN_ELAUNCH;
-        done = true;
-    }
-    const long long rows = (long long)WAVES * MR * 32;
-    p.nrow = (unsigned)((p.R + rows - 1) / rows);
-    p.ncol = (unsigned)((p.N + 32 * NT - 1) / (32 * NT));
-    gg_k_lin8<T, TRANS, SAVE, NT, WAVES, MR><<<place_grid(p.nrow, p.ncol), WAVES * 64, LDS, st>>>(p);
-    return 0;
-}
-
 template <class T, bool TRANS, bool SAVE> int launch_mm(Mm &p, hipStream_t st)
 {
-    constexpr int WAVES = sizeof(T) == 4 ? 8 : 4, MR = sizeof(T) == 4 ? 1 : 2;
-    const long long blocks = (p.R + WAVES * MR * 32 - 1) / (WAVES * MR * 32) * ((p.N + 127) / 128);
-    // fewer workgroups than half the CUs: smaller ones, their waves on the contraction
-    if (blocks < 128) {
+    constexpr int NT = 4;
+    const long long blocks = (p.R + MW * 32 - 1) / (MW * 32) * ((p.N + 32 * NT - 1) / (32 * NT));
+    // fewer workgroups than half the CUs: smaller ones, their waves on the contraction.  (One column: the pairs of W's columns that
+    // the other kernel loads do not exist.)
+    if (blocks < 128 || (TRANS && p.N < 2)) {
         p.nrow = (unsigned)((p.R + 31) / 32);
         p.ncol = (unsigned)((p.N + 31) / 32);
         gg_k_lin8_few<T, TRANS, SAVE><<<place_grid(p.nrow, p.ncol), SW * 64, 0, st>>>(p);
         return 0;
     }
-    return launch_many<T, TRANS, SAVE, 4, WAVES, MR>(p, st);
+    constexpr int LDS = 2 * Wstage<T, TRANS, NT, MW * 64>::BYTES;
+    static GGDevOnce done;
+    if (!done) {
+        if (hipFuncSetAttribute((const void *)gg_k_lin8<T, TRANS, SAVE, NT>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess)
+            return GRIDGCN_ELAUNCH;
+        done = true;
+    }
+    p.nrow = (unsigned)((p.R + MW * 32 - 1) / (MW * 32));
+    p.ncol = (unsigned)((p.N + 32 * NT - 1) / (32 * NT));
+    gg_k_lin8<T, TRANS, SAVE, NT><<<place_grid(p.nrow, p.ncol), MW * 64, LDS, st>>>(p);
+    return 0;
 }
 
 unsigned splits_of(long long R, unsigned tiles)
@@ -756,7 +808,7 @@ extern "C" {
 int gridgcn_linear_act8_fwd(const void *x, int dtype, long long R, int K, long long ldx, const void *W, const void *bias,
                             int N, void *y, uint8_t *codes, uint8_t *scales, void *stream)
 {
-    if (!x || !W || !y || !type_ok(dtype) || !sizes_ok(R, K, N) || ldx < K || !codes != !scales || ((uintptr_t)codes & 15))
+    if (!x || !W || !y || !type_ok(dtype) || !sizes_ok(R, K, N) || ldx < K || ldx > GRIDGCN_MAX_LD || !codes != !scales || ((uintptr_t)codes & 15))
         return GRIDGCN_EINVAL;
     Mm p = {};
     p.a = x; p.w = W; p.bias = bias; p.y = y; p.codes = codes; p.scales = scales; p.R = R; p.lda = ldx; p.K = K; p.N = N;
@@ -781,12 +833,14 @@ int gridgcn_linear_act8_bwd(const void *dy, int dtype, long long R, int N, long 
                             const uint8_t *codes, const uint8_t *scales, void *dx, void *dW, void *dbias, void *ws,
                             size_t ws_bytes, void *stream)
 {
-    if (!dy || !type_ok(dtype) || !sizes_ok(R, K, N) || ldy < N || (dx && !W) || (dW && (!codes || !scales)) ||
+    if (!dy || !type_ok(dtype) || !sizes_ok(R, K, N) || ldy < N || ldy > GRIDGCN_MAX_LD || (dx && !W) || (dW && (!codes || !scales)) ||
         ((uintptr_t)codes & 15))
         return GRIDGCN_EINVAL;
     Wg g = {};
     g.dy = dy; g.dw = dW; g.db = dbias; g.R = R; g.ldy = ldy; g.N = N; g.K = K; g.Cp = gg_a8_cp(K);
-    if (dW) { g.codes = codes; g.scales = scales; }
+    g.codes = dW ? codes : (const uint8_t *)dy;
+    g.scales = dW ? scales : (const uint8_t *)dy;
+    if (!dW) g.Cp = 0;
     g.tn = (N + GT - 1) / GT;
     g.tk = dW ? (K + GT - 1) / GT : 1;
     g.splits = splits_of(R, g.tn * g.tk);

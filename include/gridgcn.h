@@ -857,6 +857,8 @@ int gridgcn_gridconv_forward(const float *src, const int32_t *nebidx, const floa
  *   gives NaN), and codes / scales (both or neither) the 8-bit form of x.
  * gridgcn_linear_act8_bwd: dx[R][K] = dy W;  dW[N][K] = dy^T x^ with x^ the values of codes / scales;  dbias[N] = sum of
  *   dy; any of them may be NULL (codes, scales only for dW; W only for dx).
+ * *_workspace_bytes may answer 0: ws may then be NULL (group norm: stats = whether the call passes stats, save8 =
+ *   whether it passes codes to write; both ignored with backward).  Row strides of at most GRIDGCN_MAX_LD elements.
  * Sums have one order: the same call gives the same bits. */
 #define GRIDGCN_F32 0
 #define GRIDGCN_BF16 1
@@ -867,11 +869,13 @@ int gridgcn_gridconv_forward(const float *src, const int32_t *nebidx, const floa
 #define GRIDGCN_ACT_GELU 3       /* t/2 (1 + erf(t / sqrt 2)) */
 #define GRIDGCN_ACT8_MAX_C 65536 /* channels of a row in the 8-bit form */
 #define GRIDGCN_GN_MAX_C 8192    /* channels of gridgcn_group_norm_act_* */
+#define GRIDGCN_MAX_LD (1 << 24) /* row strides of these entries, in elements */
 int gridgcn_act8_pack(const void *x, int dtype, long long R, int C, long long ldx, uint8_t *codes,
                       uint8_t *scales, void *stream);
 int gridgcn_act8_unpack(const uint8_t *codes, const uint8_t *scales, long long R, int C, int dtype, void *x,
                         long long ldx, void *stream);
-int gridgcn_group_norm_act_workspace_bytes(int B, long long N, int C, int G, int dtype, int save8, size_t *bytes);
+int gridgcn_group_norm_act_workspace_bytes(int B, long long N, int C, int G, int dtype, int save8, int stats,
+                                           int backward, size_t *bytes);
 int gridgcn_group_norm_act_fwd(const void *x, int dtype, int B, long long N, int C, long long ldb, long long ldn,
                                int G, const void *gamma, const void *beta, int ptype, const int32_t *counts,
                                float eps, int act, void *y, double *stats, uint8_t *codes, uint8_t *scales,

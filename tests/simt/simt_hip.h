@@ -610,6 +610,16 @@ static inline simt_f32x2 simt_cvt_pk_f32_fp8(int w, bool high)
 }
 #define __builtin_amdgcn_cvt_pk_fp8_f32 simt_cvt_pk_fp8_f32
 #define __builtin_amdgcn_cvt_pk_f32_fp8 simt_cvt_pk_f32_fp8
+static inline float simt_rcp(float x) { return 1.0f / x; }
+#define __builtin_amdgcn_rcpf simt_rcp
+static inline int simt_perm(unsigned a, unsigned b, unsigned sel)     // v_perm_b32: bytes 0-3 from b, 4-7 from a
+{
+    const uint64_t v = ((uint64_t)a << 32) | b;
+    unsigned r = 0;
+    for (int i = 0; i < 4; i++) r |= (unsigned)((v >> (8 * ((sel >> (8 * i)) & 7))) & 0xff) << (8 * i);
+    return (int)r;
+}
+#define __builtin_amdgcn_perm simt_perm
 #define __expf expf                                                    // (the GPU's: exp2 of a rounded product)
 
 static inline float rsqrtf(float x) { return 1.0f / sqrtf(x); }   // (the GPU's is an approximation within 1 ulp)

@@ -390,10 +390,11 @@ def test_c_entries_refuse_without_a_launch():
     assert lib.gridgcn_act8_pack(a, 0, 1, 8, 7, a, a, None) == EINVAL
     assert lib.gridgcn_act8_pack(a, 0, 1, 8, 8, a + 4, a, None) == EINVAL
     assert lib.gridgcn_act8_unpack(a, a, 0, 8, 0, a, 8, None) == EINVAL
-    assert lib.gridgcn_group_norm_act_workspace_bytes(2, 10, 9, 2, 0, 0, ctypes.byref(n)) == EINVAL
-    assert lib.gridgcn_group_norm_act_workspace_bytes(2, 10, 8, 2, 0, 1, ctypes.byref(n)) == 0 and n.value > 0
+    assert lib.gridgcn_group_norm_act_workspace_bytes(2, 10, 9, 2, 0, 0, 0, 0, ctypes.byref(n)) == EINVAL
+    size = lambda N, back: (lib.gridgcn_group_norm_act_workspace_bytes(2, N, 8, 2, 0, 1, 0, back, ctypes.byref(n)), n.value)[1]   # noqa: E731
+    assert size(10, 0) == 0 and size(100000, 0) > 0 and size(10, 1) > 0 and size(100000, 1) > 0
     fwd = lambda **k: lib.gridgcn_group_norm_act_fwd(                                        # noqa: E731
-        k.get("x", a), k.get("dt", 0), 2, 10, 8, 80, k.get("ldn", 8), k.get("G", 2), a, a, 0, None, k.get("eps", 1e-5),
+        k.get("x", a), k.get("dt", 0), 2, 100000, 8, 800000, k.get("ldn", 8), k.get("G", 2), a, a, 0, None, k.get("eps", 1e-5),
         k.get("act", 1), a, None, k.get("codes"), k.get("scales"), k.get("ws", a), k.get("nb", 0), None)
     assert fwd() == EWS and fwd(ws=None, nb=1 << 20) == EWS
     for kw in (dict(x=None), dict(dt=7), dict(ldn=7), dict(G=3), dict(eps=-1.0), dict(act=4), dict(codes=a)):
@@ -411,6 +412,7 @@ def test_c_entries_refuse_without_a_launch():
     assert lib.gridgcn_linear_act8_bwd(a, 0, 4, 4, 4, None, 8, a, a, a, a, a, a, 256, None) == EINVAL
     assert lib.gridgcn_linear_act8_bwd(a, 0, 4, 4, 4, a, 8, None, None, a, a, a, a, 256, None) == EINVAL
     assert lib.gridgcn_linear_act8_bwd(a, 0, 1 << 20, 4, 4, a, 8, a, a, None, a, None, a, 256, None) == EWS
+    assert lib.gridgcn_linear_act8_fwd(a, 0, 4, 8, (1 << 24) + 1, a, None, 4, a, None, None, None) == EINVAL
 
 
 def test_torch_ops_trace_on_fake_tensors():
