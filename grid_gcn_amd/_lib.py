@@ -60,7 +60,7 @@ EXPORTS = [
     "gridgcn_linear_fwd_direct_drop", "gridgcn_linear_dw_drop",
     "gridgcn_act8_pack", "gridgcn_act8_unpack",
     "gridgcn_group_norm_act_workspace_bytes", "gridgcn_group_norm_act_fwd", "gridgcn_group_norm_act_bwd",
-    "gridgcn_linear_act8_fwd", "gridgcn_linear_act8_bwd_workspace_bytes", "gridgcn_linear_act8_bwd",
+    "gridgcn_linear_act8_fwd", "gridgcn_linear_act8_workspace_bytes", "gridgcn_linear_act8_bwd",
 ]
 
 
@@ -340,9 +340,9 @@ def declare(lib, path="<library>"):
     lib.gridgcn_group_norm_act_bwd.argtypes = [vp, ll, ll, vp, ll, ll, vp, vp, ci, ci, ll, ci, ci, vp, vp, vp, ci, vp,
                                                ci, vp, vp, vp, vp, cs, vp]
     lib.gridgcn_linear_act8_fwd.restype = ci
-    lib.gridgcn_linear_act8_fwd.argtypes = [vp, ci, ll, ci, ll, vp, vp, ci, vp, vp, vp, vp]
-    lib.gridgcn_linear_act8_bwd_workspace_bytes.restype = ci
-    lib.gridgcn_linear_act8_bwd_workspace_bytes.argtypes = [ll, ci, ci, ctypes.POINTER(cs)]
+    lib.gridgcn_linear_act8_fwd.argtypes = [vp, ci, ll, ci, ll, vp, vp, ci, vp, vp, vp, vp, cs, vp]
+    lib.gridgcn_linear_act8_workspace_bytes.restype = ci
+    lib.gridgcn_linear_act8_workspace_bytes.argtypes = [ll, ci, ci, ci, ci, ctypes.POINTER(cs)]
     lib.gridgcn_linear_act8_bwd.restype = ci
     lib.gridgcn_linear_act8_bwd.argtypes = [vp, ci, ll, ci, ll, vp, ci, vp, vp, vp, vp, vp, vp, cs, vp]
     return lib

@@ -278,26 +278,29 @@ def _check_linear(x, weight, bias):
     return K, N
 
 
+@functools.lru_cache(maxsize=1024)
+def _linear_workspace_bytes(R, K, N, dt, backward):
+    nb = ctypes.c_size_t(0)
+    _lib.check(_lib.load().gridgcn_linear_act8_workspace_bytes(R, K, N, dt, backward, ctypes.byref(nb)),
+               "gridgcn_linear_act8_workspace_bytes")
+    return nb.value
+
+
 def _linear_forward(x, weight, bias, save8):
     lib, dev = _lib.load(), x.device
     N, K = weight.shape
     x2, ld = _rows2(x)
-    R = x2.shape[0]
+    R, dt = x2.shape[0], _DTYPES[x.dtype]
+    nb = _linear_workspace_bytes(R, K, N, dt, 0)
     with _on(dev):
         y = torch.empty(x.shape[:-1] + (N,), dtype=x.dtype, device=dev)
         codes, scales = _new_act8(R, K, dev) if save8 else (None, None)
+        ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
         w, b = _packed(weight), _packed(bias)
-        rc = lib.gridgcn_linear_act8_fwd(x2.data_ptr(), _DTYPES[x.dtype], R, K, ld, w.data_ptr(), _p(b), N, y.data_ptr(), _p(codes),
-                                         _p(scales), _st(x))
+        rc = lib.gridgcn_linear_act8_fwd(x2.data_ptr(), dt, R, K, ld, w.data_ptr(), _p(b), N, y.data_ptr(), _p(codes),
+                                         _p(scales), _p(ws), nb, _st(x))
     _lib.check(rc, "gridgcn_linear_act8_fwd")
     return y, codes, scales
-
-
-@functools.lru_cache(maxsize=1024)
-def _linear_workspace_bytes(R, K, N):
-    nb = ctypes.c_size_t(0)
-    _lib.check(_lib.load().gridgcn_linear_act8_bwd_workspace_bytes(R, K, N, ctypes.byref(nb)), "gridgcn_linear_act8_bwd_workspace_bytes")
-    return nb.value
 
 
 def _linear_backward(dy, weight, codes, scales, x_shape, need):
@@ -305,15 +308,15 @@ def _linear_backward(dy, weight, codes, scales, x_shape, need):
     lib, dev = _lib.load(), dy.device
     N, K = weight.shape
     g2, ld = _rows2(dy)
-    R = g2.shape[0]
-    nb = _linear_workspace_bytes(R, K, N) if need[1] or need[2] else 0
+    R, dt = g2.shape[0], _DTYPES[dy.dtype]
+    nb = _linear_workspace_bytes(R, K, N, dt, 1)
     with _on(dev):
         dx = torch.empty(x_shape, dtype=dy.dtype, device=dev) if need[0] else None
         dw = torch.empty((N, K), dtype=dy.dtype, device=dev) if need[1] else None
         db = torch.empty(N, dtype=dy.dtype, device=dev) if need[2] else None
         ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
         w = _packed(weight) if need[0] else None
-        rc = lib.gridgcn_linear_act8_bwd(g2.data_ptr(), _DTYPES[dy.dtype], R, N, ld, _p(w), K, _p(codes), _p(scales), _p(dx),
+        rc = lib.gridgcn_linear_act8_bwd(g2.data_ptr(), dt, R, N, ld, _p(w), K, _p(codes), _p(scales), _p(dx),
                                          _p(dw), _p(db), _p(ws), nb, _st(dy))
     _lib.check(rc, "gridgcn_linear_act8_bwd")
     return dx, dw, db
@@ -339,8 +342,8 @@ def linear_act8(x, weight, bias=None):
     """y = x W^T + bias on x [..., K], weight [N, K], bias [N] (all of one type: float32, bfloat16 or float16), keeping for the
     backward the 8-bit form of x (act8_pack) instead of x: 1.03 bytes a value, written in the forward's pass over x.
 
-    Sums are in float32.  A float32 product is six bf16 products of operands cut into three exact bf16 parts: its error is that of
-    a float32 product; an operand that is infinite or beyond bf16's largest number (3.39e38) gives NaN.
+    Sums are in float32.  A float32 operand enters the matrix instructions as a sum of 16-bit numbers; the error of a product is that
+    of a float32 product, but an operand that is infinite or beyond 3.39e38 gives NaN.
     Backward: dx = dy W and dbias as ever; dW = dy^T x^ with x^ the 8-bit values of x.  Not differentiable twice."""
     K, N = _check_linear(x, weight, bias)
     if x.numel() == 0:

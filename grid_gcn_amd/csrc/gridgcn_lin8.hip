@@ -4,14 +4,18 @@
 //   backward  dx [R, K] = dy W;   dW [N, K] = dy^T x^, x^ the values of the 8-bit form;   db = sum of dy's rows
 //
 // Rows are many (one per point or edge), K and N a few hundred: with 16-bit rows all three products wait for memory, with
-// 32-bit rows they would wait for the fp32 matrix instruction (1/16 of the bf16 rate).  So a 32-bit operand enters as three bf16
-// numbers, x = hi + mid + lo (to nearest each: the remainder has 16, then 8 bits: nothing is lost), and a product keeps the
-// six partial products down to 2^-18 of the largest; what is dropped is below 2^-26, under the rounding of the fp32 sums.
-// A value of the 8-bit form is exact in bf16 as it is: dW needs three.
+// 32-bit rows they would wait for the fp32 matrix instruction (1/16 of the bf16 rate).  So a 32-bit operand enters as a sum of
+// 16-bit numbers, to nearest each, and a product as the partial products that are above float32's own rounding:
+//   * y and dx, many rows: x * 2^-e = hi + lo in fp16 (11 + 11 bits and the sign of lo: all of float32's 24 but the last half
+//     step), e of a row of x and of a column of W, taken out of the sums as a power of two at the end; three partial products,
+//     what is dropped (lo lo) is below 2^-24 of the product;
+//   * few rows, and dW, where no common scale can leave the sum: x = hi + mid + lo in bf16, exactly; six partial products (dropped:
+//     below 2^-26) -- three in dW, as a value of the 8-bit form is exact in bf16 as it is.
 #include "../../include/gridgcn.h"
 #include "gridgcn_act8.h"
 #include "gridgcn_mma.h"
 #include "gridgcn_once.h"
+#include <initializer_list>
 #include <type_traits>
 
 namespace {
@@ -32,6 +36,12 @@ template <class T> struct Ty {                       // 16-bit rows: the operand
 template <> struct Ty<float> {
     static constexpr int P = 3;
     static __device__ __forceinline__ F16 mfma(gg_u32x4 a, gg_u32x4 b, F16 c) { return Ty<gg_bf16>::mfma(a, b, c); }
+};
+
+// the operands of y and dx at many rows: 32-bit rows as two fp16 numbers
+template <class T> struct Mt {
+    static constexpr int P = sizeof(T) == 4 ? 2 : 1;
+    typedef typename std::conditional<std::is_same<T, gg_bf16>::value, Ty<gg_bf16>, Ty<gg_f16>>::type M;
 };
 
 __device__ __forceinline__ F16 zero16()
@@ -58,15 +68,23 @@ __device__ __forceinline__ void split2(float a, float b, unsigned &h, unsigned &
     l = gg_cvt_bf16(a, b);
 }
 
+// two floats as two fp16 pairs (of magnitudes that fp16 holds)
+__device__ __forceinline__ void halve2(float a, float b, unsigned &h, unsigned &l)
+{
+    h = gg_cvt_f16(a, b);
+    l = gg_cvt_f16(a - gg_f16of(h, 0), b - gg_f16of(h, 1));
+}
+
 // acc[t] += A B[t] from the pieces of both, the smallest partial products first; neighbouring instructions on different tiles
-template <class T, int NT, int PA, int PB>
-__device__ __forceinline__ void mul(const gg_u32x4 (&a)[PA], const gg_u32x4 (&b)[NT][PB], F16 (&c)[NT])
+template <class M, int TN, int PA, int PB>
+__device__ __forceinline__ void mul(const gg_u32x4 (&a)[PA], const gg_u32x4 (&b)[TN][PB], F16 (&c)[TN])
 {
     auto one = [&](int i, int j) {
 #pragma unroll
-        for (int t = 0; t < NT; t++) c[t] = Ty<T>::mfma(a[i], b[t][j], c[t]);
+        for (int t = 0; t < TN; t++) c[t] = M::mfma(a[i], b[t][j], c[t]);
     };
     if constexpr (PA == 3 && PB == 3) { one(2, 0); one(1, 1); one(0, 2); one(1, 0); one(0, 1); }
+    else if constexpr (PA == 2) { one(1, 0); one(0, 1); }
     else if constexpr (PA == 3) { one(2, 0); one(1, 0); }
     one(0, 0);
 }
@@ -118,9 +136,19 @@ template <class T> struct Block {
         else if constexpr (std::is_same<T, gg_bf16>::value) return (i & 1) ? gg_hi16f(w[i / 8][(i % 8) / 2]) : gg_lo16f(w[i / 8][(i % 8) / 2]);
         else return gg_f16of(w[i / 8][(i % 8) / 2], i & 1);
     }
-    // the 8-bit form: 16-bit rows, the lane holds a block of 32; 32-bit rows, the two halves hold one together (every lane of
-    // the wave calls; `on`: this lane stores).  k: first channel of the lane's share, in a row of Cp padded channels
-    __device__ __forceinline__ void save(uint8_t *codes, uint8_t *scales, int k, bool on) const
+    // channels 8 s .. of 32-bit rows, times `by`, as two fp16 numbers
+    __device__ __forceinline__ void frag2(int s, float by, gg_u32x4 (&f)[2]) const
+    {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            unsigned h, l;
+            halve2(get(8 * s + 2 * j) * by, get(8 * s + 2 * j + 1) * by, h, l);
+            f[0][j] = h; f[1][j] = l;
+        }
+    }
+    // Scale byte of the 8-bit form: 16-bit rows, the lane holds a block of 32; 32-bit rows, the two halves hold one together (every
+    // lane of the wave calls).  clean: as gg_a8_block_byte
+    __device__ __forceinline__ unsigned byte(bool &clean) const
     {
         auto top = [&](bool finite) {
             unsigned m = 0;
@@ -136,35 +164,35 @@ template <class T> struct Block {
             return m;
         };
         unsigned m = top(false);
-        const bool clean = !__any(m >= 0x7f800000u);                  // (as gg_a8_block_byte)
+        clean = !__any(m >= 0x7f800000u);
         if (!clean) m = top(true);
-        const unsigned byte = gg_a8_byte(m);
-        const float s = gg_a8_unscale(byte);
+        return gg_a8_byte(m);
+    }
+    // codes of channels 16 i .. 16 i + 15 of the lane's share
+    __device__ __forceinline__ gg_u32x4 codes(int i, unsigned byte, bool clean) const
+    {
         Block b = *this;
 #pragma unroll
-        for (int i = 0; i < 4; i++) asm volatile("" : "+v"(b.w[i]));  // (16-bit rows: unpacked again, not held unpacked)
-        if (!on) return;
+        for (int j = 0; j < 4; j++) asm volatile("" : "+v"(b.w[j]));     // (16-bit rows: unpacked again, not held unpacked since byte())
+        gg_u32x4 o;
 #pragma unroll
-        for (int i = 0; i < CH / 16; i++) {
-            gg_u32x4 o;
+        for (int j = 0; j < 4; j++) {
+            float v[4];
+            unsigned w[1];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                float v[4];
-                unsigned w[1];
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = b.get(16 * i + 4 * j + e);
-                gg_a8_encode<4>(v, byte, clean, w);
-                o[j] = w[0];
-            }
-            *(gg_u32x4 *)(codes + k + 16 * i) = o;
+            for (int e = 0; e < 4; e++) v[e] = b.get(16 * i + 4 * j + e);
+            gg_a8_encode<4>(v, byte, clean, w);
+            o[j] = w[0];
         }
-        if (k % 32 == 0) scales[k / 32] = (uint8_t)byte;
+        return o;
     }
 };
 
 struct Mm {
     const void *a;             // [R][K] rows, stride lda
-    const void *w;             // TRANS ? [K][N] : [N][K], contiguous
+    const void *w;             // few rows: TRANS ? [K][N] : [N][K], contiguous
+    const char *wp;            // many rows: W in operand order (gg_k_lin8_pack), and its columns' scale bytes
+    const int *wbyte;
     const void *bias;
     void *y;                   // [R][N] contiguous
     uint8_t *codes, *scales;
@@ -185,132 +213,83 @@ __device__ __forceinline__ bool place(const Mm &p, unsigned &row, unsigned &col)
 }
 unsigned place_grid(unsigned nrow, unsigned ncol) { return (nrow + 7) / 8 * 8 * ncol; }
 
-// W of a contraction step in LDS, in operand order: [tile of 32 columns][s][piece][lane], 16 bytes each; the lanes 32.. start one
-// slot later, so that the k-groups of a column land on different banks when they are written.
-// Tile nt holds the columns NT * j + nt: a lane's NT results of a row are then neighbours in memory.
-constexpr int FRAG = 66 * 16;
-
-template <class T, bool TRANS, int NT, int THREADS> struct Wstage {
-    static constexpr int P = Ty<T>::P, S = SS<T>, G = 2 * S;          // G groups of 8 consecutive channels in a step
-    static constexpr int ITEMS_ALL = TRANS ? G * NT * 16 : G * NT * 32;
-    static constexpr int ITEMS = (ITEMS_ALL + THREADS - 1) / THREADS;
-    static constexpr int BYTES = NT * S * P * FRAG;
-    // not TRANS: 8 consecutive k of a column; TRANS: 8 consecutive k (rows of w) of two neighbouring columns
-    static constexpr int WORDS = TRANS ? (sizeof(T) == 4 ? 16 : 8) : (sizeof(T) == 4 ? 8 : 4);
-    unsigned r[ITEMS][WORDS];
-    static_assert(ITEMS_ALL % THREADS == 0, "every thread has the same number of items");
-
-    // A step whose channels all exist.  Columns behind the last are other columns: nobody stores their results.  (TRANS: N >= 2)
-    __device__ __forceinline__ void load_full(const Mm &p, int n0, int k0)
-    {
-        const T *w = (const T *)p.w;
-#pragma unroll
-        for (int i = 0; i < ITEMS; i++) {
-            const int e = (int)threadIdx.x + i * THREADS;
-            if constexpr (!TRANS) {
-                const int n = n0 + e / G;
-                const T *q = w + (size_t)(n < p.N ? n : p.N - 1) * p.K + k0 + 8 * (e % G);
-#pragma unroll
-                for (int j = 0; j < WORDS / 4; j++) {
-                    gg_u32x4 u;
-                    if constexpr (sizeof(T) == 4) u = *(const gg_u32x4_a4 *)(q + 4 * j);
-                    else u = *(const gg_u32x4_a2 *)q;
-#pragma unroll
-                    for (int t = 0; t < 4; t++) r[i][4 * j + t] = u[t];
-                }
-            } else {
-                const int n = n0 + 2 * (e % (NT * 16));
-                const bool last = n + 1 >= p.N;                      // (the pair in front; its second is column N - 1)
-                const T *q = w + (size_t)(k0 + 8 * (e / (NT * 16))) * p.N + (last ? p.N - 2 : n);
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    if constexpr (sizeof(T) == 4) {
-                        const gg_u32x2 u = *(const gg_u32x2_a4 *)(q + (size_t)j * p.N);
-                        r[i][2 * j] = last ? u[1] : u[0];
-                        r[i][2 * j + 1] = u[1];
-                    } else {
-                        const unsigned u = *(const gg_u32_a2 *)(q + (size_t)j * p.N);
-                        r[i][j] = last ? u >> 16 : u;
-                    }
-                }
-            }
-        }
-    }
-    // the last step, from channel k0 on: zeros behind K
-    __device__ __forceinline__ void load_tail(const Mm &p, int n0, int k0)
-    {
-        const T *w = (const T *)p.w;
-#pragma unroll
-        for (int i = 0; i < ITEMS; i++) {
-            const int e = (int)threadIdx.x + i * THREADS;
-            const int n = n0 + (TRANS ? 2 * (e % (NT * 16)) : e / G), k = k0 + 8 * (TRANS ? e / (NT * 16) : e % G);
-#pragma unroll
-            for (int j = 0; j < WORDS; j++) r[i][j] = 0u;
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-#pragma unroll
-                for (int c = 0; c < (TRANS ? 2 : 1); c++) {
-                    if (k + j >= p.K || n + c >= p.N) continue;
-                    const T *q = w + (TRANS ? (size_t)(k + j) * p.N + n + c : (size_t)n * p.K + k + j);
-                    const int at = TRANS ? 2 * j + c : j;            // element of the item
-                    if constexpr (sizeof(T) == 4) r[i][at] = *(const unsigned *)q;
-                    else r[i][at / 2] |= (unsigned)*(const unsigned short *)q << (16 * (at & 1));
-                }
-        }
-    }
-
-    static __device__ __forceinline__ void put(char *lds, int nl, int k8, const gg_u32x4 (&f)[P])
-    {
-        const int nt = nl % NT, j = nl / NT, h = k8 / S, s = k8 % S;
-#pragma unroll
-        for (int q = 0; q < P; q++) *(gg_u32x4 *)(lds + ((nt * S + s) * P + q) * FRAG + (h * 33 + j) * 16) = f[q];
-    }
-
-    __device__ __forceinline__ void store(char *lds) const
-    {
-#pragma unroll
-        for (int i = 0; i < ITEMS; i++) {
-            const int e = (int)threadIdx.x + i * THREADS;
-            if constexpr (!TRANS) {
-                gg_u32x4 f[P];
-                if constexpr (sizeof(T) == 4) {
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        unsigned h, m, l;
-                        split2(__uint_as_float(r[i][2 * j]), __uint_as_float(r[i][2 * j + 1]), h, m, l);
-                        f[0][j] = h; f[1][j] = m; f[2][j] = l;
-                    }
-                } else {
-                    f[0] = gg_u32x4{r[i][0], r[i][1], r[i][2], r[i][3]};
-                }
-                put(lds, e / G, e % G, f);
-            } else {
-                const int nl = 2 * (e % (NT * 16)), k8 = e / (NT * 16);
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    gg_u32x4 f[P];
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        if constexpr (sizeof(T) == 4) {
-                            unsigned h, m, l;
-                            split2(__uint_as_float(r[i][4 * j + c]), __uint_as_float(r[i][4 * j + 2 + c]), h, m, l);
-                            f[0][j] = h; f[1][j] = m; f[2][j] = l;
-                        } else {
-                            f[0][j] = gg_pair16(r[i][2 * j], r[i][2 * j + 1], c);
-                        }
-                    }
-                    put(lds, nl + c, k8, f);
-                }
-            }
-        }
-    }
+// ---- W in operand order, for many rows: [column block][step][tile of 32 columns][s][piece][lane], 16 bytes each; zeros behind K and N.
+// Tile nt of a column block holds its columns NT * j + nt: a lane's NT results of a row are then neighbours in memory.
+// 32-bit: two fp16 numbers of W * 2^(127 - byte), byte of a column as in the 8-bit form.  A workgroup = 32 columns. -------------
+constexpr int NT = 4, PT = 512;
+template <class T> constexpr int STEP = NT * SS<T> * Mt<T>::P * 1024;          // bytes of a step: 16 KB either way
+struct Pk {
+    const void *w;
+    char *wp;
+    int *wbyte;
+    int K, N, steps;
 };
+template <class T, bool TRANS> __device__ __forceinline__ void ld8(const T *w, int n, int k, int K, int N, gg_u32x4 (&u)[sizeof(T) / 2])
+{
+    // 8 consecutive k of column n
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) u[i] = gg_u32x4{0u, 0u, 0u, 0u};
+    if (n >= N) return;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        if (k + e >= K) continue;
+        const T *q = w + (TRANS ? (size_t)(k + e) * N + n : (size_t)n * K + k + e);
+        if constexpr (sizeof(T) == 4) u[e / 4][e % 4] = *(const unsigned *)q;
+        else u[0][e / 2] |= (unsigned)*(const unsigned short *)q << (16 * (e & 1));
+    }
+}
+template <class T, bool TRANS> __global__ __launch_bounds__(PT) void gg_k_lin8_pack(Pk p)
+{
+    constexpr int S = SS<T>, P = Mt<T>::P, L = PT / 32;            // L lanes share a column
+    __shared__ unsigned red[32][L + 1];
+    const int c = TRANS ? (int)threadIdx.x & 31 : (int)threadIdx.x / L, kl = TRANS ? (int)threadIdx.x >> 5 : (int)threadIdx.x % L;
+    const int n = blockIdx.x * 32 + c, groups = p.steps * (KS<T> / 8);
+    unsigned byte = 0;
+    if constexpr (P == 2) {
+        unsigned m = 0;
+        for (int g = kl; g < groups; g += L) {
+            gg_u32x4 u[2];
+            ld8<T, TRANS>((const T *)p.w, n, 8 * g, p.K, p.N, u);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const unsigned a = u[e / 4][e % 4] & 0x7fffffffu;
+                m = m > a ? m : a;
+            }
+        }
+        red[c][kl] = m;
+        __syncthreads();
+        for (int i = 0; i < L; i++) m = m > red[c][i] ? m : red[c][i];
+        byte = gg_a8_byte(m);
+        if (kl == 0) p.wbyte[n] = (int)byte;
+    }
+    const int nl = n % (32 * NT), nt = nl % NT, j = nl / NT;
+    char *base = p.wp + (size_t)(n / (32 * NT)) * p.steps * STEP<T>;
+    for (int g = kl; g < groups; g += L) {
+        const int st = g / (KS<T> / 8), gi = g % (KS<T> / 8), h = gi / S, s = gi % S;
+        gg_u32x4 u[sizeof(T) / 2], f[P];
+        ld8<T, TRANS>((const T *)p.w, n, 8 * g, p.K, p.N, u);
+        if constexpr (P == 2) {
+            const float by = gg_a8_unscale(byte);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                unsigned hi, lo;
+                halve2(__uint_as_float(u[e / 2][2 * (e & 1)]) * by, __uint_as_float(u[e / 2][2 * (e & 1) + 1]) * by, hi, lo);
+                f[0][e] = hi; f[1][e] = lo;
+            }
+        } else {
+            f[0] = u[0];
+        }
+#pragma unroll
+        for (int q = 0; q < P; q++)
+            *(gg_u32x4 *)(base + (size_t)st * STEP<T> + ((nt * S + s) * P + q) * 1024 + (h * 32 + j) * 16) = f[q];
+    }
+}
 
-// y of one row for NT neighbouring columns
-template <class T, int NT> __device__ __forceinline__ void put_row(T *y, long long row, int n, int N, const float (&v)[NT])
+// y of one row for M neighbouring columns
+template <class T, int M> __device__ __forceinline__ void put_row(T *y, long long row, int n, int N, const float (&v)[M])
 {
     T *q = y + (size_t)row * N + n;
-    if (NT == 4 && n + 4 <= N) {
+    if (M == 4 && n + 4 <= N) {
         if constexpr (sizeof(T) == 4) {
             *(gg_u32x4_a4 *)q = gg_u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
         } else if constexpr (std::is_same<T, gg_bf16>::value) {
@@ -320,100 +299,150 @@ template <class T, int NT> __device__ __forceinline__ void put_row(T *y, long lo
         }
     } else {
 #pragma unroll
-        for (int t = 0; t < NT; t++)
+        for (int t = 0; t < M; t++)
             if (n + t < N) GGRowT<T>::put(q + t, v[t]);
     }
 }
 
 // ---- many rows: a wave owns 32 rows and 32 NT columns, its rows straight from memory into registers (each row is read by one wave
-// only), W through LDS, the next step of both in flight while this one is multiplied; three or four workgroups per CU, so that
-// one's barriers and stores are another's matrix instructions ----------------------------------------------------------------
+// only), W through LDS (copied there without passing registers), the next step of both in flight while this one is multiplied;
+// three workgroups per CU, so that one's barriers and stores are another's matrix instructions.
+// 32-bit rows: a row's scale is that of its first 32 channels, and grows (the sums are scaled down) where a later block is
+// more than 2^3 larger, which fp16's range allows for; smaller blocks keep 33 bits below the largest value of the row.
+// The 8-bit form is held back until 128 bytes of a row are complete: stored as they come, 16 bytes of a line per step, lines left the
+// L2 half written and the kernel moved a third more bytes.  The column blocks of one row block take turns at it. ----------------
 constexpr int MW = 4;             // waves
-template <class T, bool TRANS, bool SAVE, int NT>
+constexpr int HEADROOM = 3;
+template <class T, bool SAVE>
 __global__ __launch_bounds__(MW * 64, 3) void gg_k_lin8(Mm p)
 {
-    constexpr int P = Ty<T>::P, S = SS<T>;
-    typedef Wstage<T, TRANS, NT, MW * 64> W;
-    extern __shared__ __attribute__((aligned(16))) char lds8[];
+    constexpr int P = Mt<T>::P, S = SS<T>, PC = Block<T>::CH / 16, GROUP = 128 / KS<T>;      // GROUP steps make 128 codes of a row
+    __shared__ __attribute__((aligned(16))) char lds[2][STEP<T>];
     unsigned brow, bcol;
     if (!place(p, brow, bcol)) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, h = lane >> 5, j = lane & 31;
-    const int n0 = (int)bcol * 32 * NT;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5, j = lane & 31;
     const long long m0 = (long long)brow * (MW * 32) + wave * 32, r = m0 + j;
     const bool live = r < p.R;
-    const int Cp = gg_a8_cp(p.K), steps = (p.K + KS<T> - 1) / KS<T>, kh = KS<T> / 2 * h;
+    const int Cp = gg_a8_cp(p.K), steps = (p.K + KS<T> - 1) / KS<T>, full = p.K / KS<T>, kh = KS<T> / 2 * h;
     const T *row = (const T *)p.a + (size_t)(live ? r : p.R - 1) * p.lda;
+    const char *wp = p.wp + (size_t)bcol * steps * STEP<T> + threadIdx.x * 16;
     F16 acc[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) acc[t] = zero16();
+    int rbyte = 0;                // scale byte of the row (32-bit rows)
+    gg_u32x4 held[4];             // codes of the group so far, the last ones behind
+    unsigned heldb = 0;           // ... scale bytes likewise
 
-    auto keep = [&](const Block<T> &b, int st) {
-        if (SAVE && bcol == 0) {
-            const int k = st * KS<T> + kh;
-            b.save(p.codes + (size_t)r * Cp, p.scales + (size_t)r * (Cp / 32), k, live && k < Cp);
-        }
+    auto fetch_w = [&](int st) {
+#pragma unroll
+        for (int i = 0; i < STEP<T> / (MW * 64 * 16); i++)
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)(wp + (size_t)st * STEP<T> + i * (MW * 64 * 16)),
+                                             (__attribute__((address_space(3))) void *)(&lds[st & 1][i * (MW * 64 * 16) + wave * 1024]), 16, 0, 0);
     };
-    auto multiply = [&](const Block<T> &b, const char *cur) {
+    auto arrived = [&]() {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    };
+    auto step = [&](Block<T> &b, int st) {
+        bool clean = true;
+        unsigned byte = 0;
+        const bool mine = SAVE && (unsigned)(st / GROUP) % p.ncol == bcol;
+        if (P == 2 || mine) byte = b.byte(clean);
+        float by = 1.f;
+        if constexpr (P == 2) {
+            if (st == 0) rbyte = (int)byte;
+            if (__any((int)byte > rbyte + HEADROOM)) {
+                const int up = (int)byte > rbyte + HEADROOM ? (int)byte : rbyte, d = rbyte - up;
+                rbyte = up;
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int di = __shfl(d, ggm_row(i, lane));
+#pragma unroll
+                    for (int t = 0; t < NT; t++) acc[t][i] = ldexpf(acc[t][i], di);
+                }
+            }
+            by = gg_a8_unscale((unsigned)rbyte);
+        }
+        if (mine) {
+#pragma unroll
+            for (int i = 0; i < 4 - PC; i++) held[i] = held[i + PC];
+#pragma unroll
+            for (int i = 0; i < PC; i++) held[4 - PC + i] = b.codes(i, byte, clean);
+            if constexpr (PC == 1) {
+                heldb = (heldb >> 8) | (byte << 24);
+            } else {
+                const unsigned o = (unsigned)__shfl_xor((int)byte, 32);
+                heldb = (heldb >> 16) | ((h ? o | (byte << 8) : byte | (o << 8)) << 16);
+            }
+            const int in = st % GROUP;                            // place of the step in its group
+            if ((in == GROUP - 1 || st == steps - 1) && live) {
+                const int k0 = (st - in) * KS<T>;
+                uint8_t *q = p.codes + (size_t)r * Cp;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int e = i - (4 - (in + 1) * PC);            // piece of the group
+                    const int k = k0 + (PC == 1 ? 32 * e + 16 * h : 64 * (e / 2) + 32 * h + 16 * (e & 1));
+                    if (e >= 0 && k < Cp) *(gg_u32x4 *)(q + k) = held[i];
+                }
+                if (h == 0) {
+                    const int have = (in + 1) * PC, left = (Cp - k0) / 32, n = have < left ? have : left;
+                    const unsigned w = heldb >> (8 * (4 - have));
+                    uint8_t *sq = p.scales + (size_t)r * (Cp / 32) + k0 / 32;
+                    if (n == 4) *(gg_u32_a1 *)sq = w;
+                    else
+                        for (int i = 0; i < n; i++) sq[i] = (uint8_t)(w >> (8 * i));
+                }
+            }
+        }
+        const char *cur = lds[st & 1];
 #pragma unroll
         for (int s = 0; s < S; s++) {
             gg_u32x4 fa[P];
-            b.frag(s, fa);
+            if constexpr (P == 2) b.frag2(s, by, fa);
+            else b.frag(s, fa);
 #pragma unroll
             for (int t = 0; t < NT; t += 2) {                     // (two tiles at a time: independent neighbours, few registers)
                 gg_u32x4 fb[2][P];
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
-                    for (int q = 0; q < P; q++) fb[u][q] = *(const gg_u32x4 *)(cur + (((t + u) * S + s) * P + q) * FRAG + (h * 33 + j) * 16);
+                    for (int q = 0; q < P; q++) fb[u][q] = *(const gg_u32x4 *)(cur + (((t + u) * S + s) * P + q) * 1024 + lane * 16);
                 F16(&two)[2] = *(F16(*)[2])&acc[t];
-                mul<T>(fa, fb, two);
+                mul<typename Mt<T>::M>(fa, fb, two);
             }
         }
     };
-    const int full = p.K / KS<T>;
-    if (full) {
-        W ws;
-        Block<T> a, nx;
-        ws.load_full(p, n0, 0);
-        a.load_full(row + kh);
-        ws.store(lds8);
-        __syncthreads();
-        for (int st = 0; st < full; st++) {
-            const bool more = st + 1 < full;
-            if (more) {
-                ws.load_full(p, n0, (st + 1) * KS<T>);
-                nx.load_full(row + (st + 1) * KS<T> + kh);
-            }
-            keep(a, st);
-            multiply(a, lds8 + (st & 1) * W::BYTES);
-            if (more) {
-                ws.store(lds8 + ((st + 1) & 1) * W::BYTES);
-                a = nx;
-            }
-            __syncthreads();
-        }
+    Block<T> a, nx;
+    fetch_w(0);
+    if (full) a.load_full(row + kh);
+    arrived();
+    for (int st = 0; st < full; st++) {
+        if (st + 1 < steps) fetch_w(st + 1);
+        if (st + 1 < full) nx.load_full(row + (st + 1) * KS<T> + kh);
+        step(a, st);
+        a = nx;
+        arrived();
     }
     if (full < steps) {
-        W ws;
-        Block<T> a;
-        ws.load_tail(p, n0, full * KS<T>);
         a.load(row, full * KS<T> + kh, p.K);
-        ws.store(lds8 + (full & 1) * W::BYTES);
-        __syncthreads();
-        keep(a, full);
-        multiply(a, lds8 + (full & 1) * W::BYTES);
+        step(a, full);
     }
-    const int n = n0 + NT * j;
+    const int n = ((int)bcol * 32 + j) * NT;
     float b[NT];
+    int cb[NT];
 #pragma unroll
-    for (int t = 0; t < NT; t++) b[t] = n + t < p.N ? gg_ld_param(p.bias, GGRowT<T>::id, n + t, 0.f) : 0.f;
+    for (int t = 0; t < NT; t++) {
+        b[t] = n + t < p.N ? gg_ld_param(p.bias, GGRowT<T>::id, n + t, 0.f) : 0.f;
+        cb[t] = P == 2 ? p.wbyte[n + t] - 254 : 0;
+    }
 #pragma unroll
     for (int i = 0; i < 16; i++) {
         const long long o = m0 + ggm_row(i, lane);
+        const int rb = P == 2 ? __shfl(rbyte, ggm_row(i, lane)) : 0;
         if (o >= p.R) continue;
         float v[NT];
 #pragma unroll
-        for (int t = 0; t < NT; t++) v[t] = acc[t][i] + b[t];
+        for (int t = 0; t < NT; t++) v[t] = (P == 2 ? ldexpf(acc[t][i], rb + cb[t]) : acc[t][i]) + b[t];
         put_row<T, NT>((T *)p.y, o, n, p.N, v);
     }
 }
@@ -453,13 +482,21 @@ __global__ __launch_bounds__(SW * 64) void gg_k_lin8_few(Mm p)
                 else b.w[i / 8][(i % 8) / 2] |= (unsigned)*(const unsigned short *)q << (16 * (i & 1));
             }
         }
-        if (SAVE && bcol == 0) a.save(p.codes + (size_t)r * Cp, p.scales + (size_t)r * (Cp / 32), k0, r < p.R && k0 < Cp);
+        if (SAVE && bcol == 0) {
+            bool clean;
+            const unsigned byte = a.byte(clean);
+            if (r < p.R && k0 < Cp) {
+#pragma unroll
+                for (int i = 0; i < Block<T>::CH / 16; i++) *(gg_u32x4 *)(p.codes + (size_t)r * Cp + k0 + 16 * i) = a.codes(i, byte, clean);
+                if (k0 % 32 == 0) p.scales[(size_t)r * (Cp / 32) + k0 / 32] = (uint8_t)byte;
+            }
+        }
 #pragma unroll
         for (int s = 0; s < SS<T>; s++) {
             gg_u32x4 fa[P], fb[1][P];
             a.frag(s, fa);
             b.frag(s, fb[0]);
-            mul<T>(fa, fb, acc);
+            mul<Ty<T>>(fa, fb, acc);
         }
     }
 #pragma unroll
@@ -621,7 +658,7 @@ __global__ __launch_bounds__(GW * 64, 1) void gg_k_lin8_wgrad(Wg p)
         for (int i = 0; i < 4; i++) {
             gg_u32x4 fd[P];
             s.frag_dy(i, fd);
-            mul<T>(fd, fx, acc[i]);
+            mul<Ty<T>>(fd, fx, acc[i]);
         }
         if (first) {
 #pragma unroll
@@ -730,29 +767,34 @@ __global__ __launch_bounds__(256) void gg_k_lin8_wsum(Wg p, unsigned nw)
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
-template <class T, bool TRANS, bool SAVE> int launch_mm(Mm &p, hipStream_t st)
+// Many rows where the larger workgroups fill at least half the CUs; below that, smaller ones, their waves on the contraction.
+bool many(long long R, int N) { return (R + MW * 32 - 1) / (MW * 32) * ((N + 32 * NT - 1) / (32 * NT)) >= 128; }
+size_t pack_bytes(long long R, int K, int N, int dtype)
 {
-    constexpr int NT = 4;
-    const long long blocks = (p.R + MW * 32 - 1) / (MW * 32) * ((p.N + 32 * NT - 1) / (32 * NT));
-    // fewer workgroups than half the CUs: smaller ones, their waves on the contraction.  (One column: the pairs of W's columns that
-    // the other kernel loads do not exist.)
-    if (blocks < 128 || (TRANS && p.N < 2)) {
+    if (!many(R, N)) return 0;
+    const int ks = dtype == GRIDGCN_F32 ? KS<float> : KS<gg_bf16>;
+    const size_t ncol = (N + 32 * NT - 1) / (32 * NT), steps = (K + ks - 1) / ks;
+    return ncol * (steps * STEP<float> + 32 * NT * sizeof(int));
+}
+
+template <class T, bool TRANS, bool SAVE> void launch_mm(Mm &p, void *ws, hipStream_t st)
+{
+    if (!many(p.R, p.N)) {
         p.nrow = (unsigned)((p.R + 31) / 32);
         p.ncol = (unsigned)((p.N + 31) / 32);
         gg_k_lin8_few<T, TRANS, SAVE><<<place_grid(p.nrow, p.ncol), SW * 64, 0, st>>>(p);
-        return 0;
-    }
-    constexpr int LDS = 2 * Wstage<T, TRANS, NT, MW * 64>::BYTES;
-    static GGDevOnce done;
-    if (!done) {
-        if (hipFuncSetAttribute((const void *)gg_k_lin8<T, TRANS, SAVE, NT>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess)
-            return GRIDGCN_ELAUNCH;
-        done = true;
+        return;
     }
     p.nrow = (unsigned)((p.R + MW * 32 - 1) / (MW * 32));
     p.ncol = (unsigned)((p.N + 32 * NT - 1) / (32 * NT));
-    gg_k_lin8<T, TRANS, SAVE, NT><<<place_grid(p.nrow, p.ncol), MW * 64, LDS, st>>>(p);
-    return 0;
+    Pk k = {};
+    k.w = p.w; k.wp = (char *)ws; k.K = p.K; k.N = p.N;
+    k.steps = (p.K + KS<T> - 1) / KS<T>;
+    k.wbyte = (int *)(k.wp + (size_t)p.ncol * k.steps * STEP<T>);
+    gg_k_lin8_pack<T, TRANS><<<p.ncol * NT, PT, 0, st>>>(k);
+    p.wp = k.wp;
+    p.wbyte = k.wbyte;
+    gg_k_lin8<T, SAVE><<<place_grid(p.nrow, p.ncol), MW * 64, 0, st>>>(p);
 }
 
 unsigned splits_of(long long R, unsigned tiles)
@@ -767,7 +809,7 @@ unsigned splits_of(long long R, unsigned tiles)
 size_t wgrad_bytes(long long R, unsigned tn, unsigned tk)
 {
     const unsigned s = splits_of(R, tn * tk);
-    return s > 1 ? (size_t)s * ((size_t)tn * tk * GT * GT + (size_t)tn * GT) * 4 : 256;
+    return s > 1 ? (size_t)s * ((size_t)tn * tk * GT * GT + (size_t)tn * GT) * 4 : 0;
 }
 
 template <class T> int launch_wgrad(Wg &p, hipStream_t st)
@@ -805,47 +847,61 @@ template <class F> int with_type(int dtype, F f)
 
 extern "C" {
 
-int gridgcn_linear_act8_fwd(const void *x, int dtype, long long R, int K, long long ldx, const void *W, const void *bias,
-                            int N, void *y, uint8_t *codes, uint8_t *scales, void *stream)
+int gridgcn_linear_act8_workspace_bytes(long long R, int K, int N, int dtype, int backward, size_t *bytes)
 {
-    if (!x || !W || !y || !type_ok(dtype) || !sizes_ok(R, K, N) || ldx < K || ldx > GRIDGCN_MAX_LD || !codes != !scales || ((uintptr_t)codes & 15))
+    if (!bytes || !sizes_ok(R, K, N) || !type_ok(dtype)) return GRIDGCN_EINVAL;
+    if (!backward) {
+        *bytes = pack_bytes(R, K, N, dtype);
+        return GRIDGCN_OK;
+    }
+    // (dx, then dW or db alone: one after the other in the same memory)
+    const unsigned tn = (N + GT - 1) / GT;
+    size_t n = pack_bytes(R, N, K, dtype);
+    for (size_t o : {wgrad_bytes(R, tn, (K + GT - 1) / GT), wgrad_bytes(R, tn, 1)}) n = n > o ? n : o;
+    *bytes = n;
+    return GRIDGCN_OK;
+}
+
+int gridgcn_linear_act8_fwd(const void *x, int dtype, long long R, int K, long long ldx, const void *W, const void *bias,
+                            int N, void *y, uint8_t *codes, uint8_t *scales, void *ws, size_t ws_bytes, void *stream)
+{
+    if (!x || !W || !y || !type_ok(dtype) || !sizes_ok(R, K, N) || ldx < K || ldx > GRIDGCN_MAX_LD || !codes != !scales ||
+        ((uintptr_t)codes & 15))
         return GRIDGCN_EINVAL;
+    const size_t need = pack_bytes(R, K, N, dtype);
+    if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15))) return GRIDGCN_EWORKSPACE;
     Mm p = {};
     p.a = x; p.w = W; p.bias = bias; p.y = y; p.codes = codes; p.scales = scales; p.R = R; p.lda = ldx; p.K = K; p.N = N;
     const hipStream_t st = (hipStream_t)stream;
     const int rc = with_type(dtype, [&](auto *t) {
         typedef typename std::remove_pointer<decltype(t)>::type T;
-        return codes ? launch_mm<T, false, true>(p, st) : launch_mm<T, false, false>(p, st);
+        if (codes) launch_mm<T, false, true>(p, ws, st);
+        else launch_mm<T, false, false>(p, ws, st);
+        return 0;
     });
     if (rc) return rc;
     return hipGetLastError() == hipSuccess ? GRIDGCN_OK : GRIDGCN_ELAUNCH;
-}
-
-int gridgcn_linear_act8_bwd_workspace_bytes(long long R, int K, int N, size_t *bytes)
-{
-    if (!bytes || !sizes_ok(R, K, N)) return GRIDGCN_EINVAL;
-    const size_t w = wgrad_bytes(R, (N + GT - 1) / GT, (K + GT - 1) / GT), b = wgrad_bytes(R, (N + GT - 1) / GT, 1);
-    *bytes = w > b ? w : b;
-    return GRIDGCN_OK;
 }
 
 int gridgcn_linear_act8_bwd(const void *dy, int dtype, long long R, int N, long long ldy, const void *W, int K,
                             const uint8_t *codes, const uint8_t *scales, void *dx, void *dW, void *dbias, void *ws,
                             size_t ws_bytes, void *stream)
 {
-    if (!dy || !type_ok(dtype) || !sizes_ok(R, K, N) || ldy < N || ldy > GRIDGCN_MAX_LD || (dx && !W) || (dW && (!codes || !scales)) ||
-        ((uintptr_t)codes & 15))
+    if (!dy || !type_ok(dtype) || !sizes_ok(R, K, N) || ldy < N || ldy > GRIDGCN_MAX_LD || (dx && !W) ||
+        (dW && (!codes || !scales)) || ((uintptr_t)codes & 15))
         return GRIDGCN_EINVAL;
     Wg g = {};
-    g.dy = dy; g.dw = dW; g.db = dbias; g.R = R; g.ldy = ldy; g.N = N; g.K = K; g.Cp = gg_a8_cp(K);
+    g.dy = dy; g.dw = dW; g.db = dbias; g.R = R; g.ldy = ldy; g.N = N; g.K = K;
+    g.Cp = dW ? gg_a8_cp(K) : 0;
     g.codes = dW ? codes : (const uint8_t *)dy;
     g.scales = dW ? scales : (const uint8_t *)dy;
-    if (!dW) g.Cp = 0;
     g.tn = (N + GT - 1) / GT;
     g.tk = dW ? (K + GT - 1) / GT : 1;
     g.splits = splits_of(R, g.tn * g.tk);
-    if ((dW || dbias) && g.splits > 1) {
-        if (!ws || ws_bytes < wgrad_bytes(R, g.tn, g.tk) || ((uintptr_t)ws & 15)) return GRIDGCN_EWORKSPACE;
+    size_t need = dx ? pack_bytes(R, N, K, dtype) : 0;
+    if (dW || dbias) need = need > wgrad_bytes(R, g.tn, g.tk) ? need : wgrad_bytes(R, g.tn, g.tk);
+    if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15))) return GRIDGCN_EWORKSPACE;
+    if (g.splits > 1) {
         g.part = (float *)ws;
         g.dbpart = g.part + (size_t)g.splits * g.tn * g.tk * GT * GT;
     }
@@ -855,8 +911,7 @@ int gridgcn_linear_act8_bwd(const void *dy, int dtype, long long R, int N, long 
         if (dx) {
             Mm p = {};
             p.a = dy; p.w = W; p.y = dx; p.R = R; p.lda = ldy; p.K = N; p.N = K;
-            const int e = launch_mm<T, true, false>(p, st);
-            if (e) return e;
+            launch_mm<T, true, false>(p, ws, st);
         }
         return dW || dbias ? launch_wgrad<T>(g, st) : 0;
     });

@@ -853,8 +853,8 @@ int gridgcn_gridconv_forward(const float *src, const int32_t *nebidx, const floa
  *   the three may be NULL.  Rows n >= counts[b]: dx = 0, dy not read.
  *
  * gridgcn_linear_act8_fwd: y[R][N] = x[R][K] W[N][K]^T + bias[N] (bias may be NULL), all of one type, products summed in
- *   fp32 (float32 operands: each as three bf16 numbers, six products: the error of an fp32 product; an infinite operand
- *   gives NaN), and codes / scales (both or neither) the 8-bit form of x.
+ *   fp32 (float32 operands as sums of 16-bit numbers: the error of an fp32 product; an infinite operand gives NaN),
+ *   and codes / scales (both or neither) the 8-bit form of x.
  * gridgcn_linear_act8_bwd: dx[R][K] = dy W;  dW[N][K] = dy^T x^ with x^ the values of codes / scales;  dbias[N] = sum of
  *   dy; any of them may be NULL (codes, scales only for dW; W only for dx).
  * *_workspace_bytes may answer 0: ws may then be NULL (group norm: stats = whether the call passes stats, save8 =
@@ -886,8 +886,9 @@ int gridgcn_group_norm_act_bwd(const void *dy, long long ldgb, long long ldgn, c
                                const void *beta, int ptype, const int32_t *counts, int act, void *dx,
                                void *dgamma, void *dbeta, void *ws, size_t ws_bytes, void *stream);
 int gridgcn_linear_act8_fwd(const void *x, int dtype, long long R, int K, long long ldx, const void *W,
-                            const void *bias, int N, void *y, uint8_t *codes, uint8_t *scales, void *stream);
-int gridgcn_linear_act8_bwd_workspace_bytes(long long R, int K, int N, size_t *bytes);
+                            const void *bias, int N, void *y, uint8_t *codes, uint8_t *scales, void *ws, size_t ws_bytes,
+                            void *stream);
+int gridgcn_linear_act8_workspace_bytes(long long R, int K, int N, int dtype, int backward, size_t *bytes);
 int gridgcn_linear_act8_bwd(const void *dy, int dtype, long long R, int N, long long ldy, const void *W, int K,
                             const uint8_t *codes, const uint8_t *scales, void *dx, void *dW, void *dbias,
                             void *ws, size_t ws_bytes, void *stream);

@@ -66,4 +66,6 @@ LINEAR = [
     (64, 520, 40, True, 0),
     (300, 40, 129, False, 8),
     (17, 192, 260, True, 0),
+    (260, 35, 5600, True, 0),          # enough workgroups for the kernel of many rows: forward ...
+    (260, 5600, 35, False, 1),         # ... and dx
 ]

@@ -117,7 +117,9 @@ def rewrite(text):
 
 def rewrite_header(text):
     """the raw buffer intrinsics are declared by their LLVM names (`... __asm("llvm.amdgcn.raw.buffer.load.f32")`):
-    the label goes, the emulator defines the functions under their C++ names (tests/simt/simt_buf.cpp)"""
+    the label goes, the emulator defines the functions under their C++ names (tests/simt/simt_buf.cpp); address spaces
+    (global, LDS) are one here"""
+    text = re.sub(r"__attribute__\(\(address_space\(\d\)\)\)", "", text)
     return re.sub(r'\s*__asm\("llvm\.amdgcn\.raw\.buffer\.[^"]+"\)', "", text)
 
 

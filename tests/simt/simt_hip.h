@@ -610,6 +610,12 @@ static inline simt_f32x2 simt_cvt_pk_f32_fp8(int w, bool high)
 }
 #define __builtin_amdgcn_cvt_pk_fp8_f32 simt_cvt_pk_fp8_f32
 #define __builtin_amdgcn_cvt_pk_f32_fp8 simt_cvt_pk_f32_fp8
+// global_load_lds: lane l's bytes go to the (wave-uniform) LDS address + l * size
+static inline void simt_global_load_lds(const void *g, void *l, int size, int off, int)
+{
+    memcpy((char *)l + off + simt_cur->lane * size, (const char *)g + off, size);
+}
+#define __builtin_amdgcn_global_load_lds simt_global_load_lds
 static inline float simt_rcp(float x) { return 1.0f / x; }
 #define __builtin_amdgcn_rcpf simt_rcp
 static inline int simt_perm(unsigned a, unsigned b, unsigned sel)     // v_perm_b32: bytes 0-3 from b, 4-7 from a

@@ -223,6 +223,38 @@ def test_linear_act8(case, dtype):
     check_linear(got, want, case)
 
 
+def growing_rows(R, K, seed):
+    """rows whose magnitude grows along them by 2^40, starts with zeros, falls off, or is far from 1 as a whole"""
+    x = cases.rows((R,), K, torch.float32, seed)
+    k = torch.arange(K) / K
+    x[0::5] *= torch.exp2(40 * k)
+    x[1::5, :K // 2] = 0
+    x[2::5] *= torch.exp2(-40 * k)
+    x[3::5] *= 2.0 ** -90
+    return x
+
+
+def run_scales(dev="cpu"):
+    x, w, dy = growing_rows(260, 72, 3), cases.rows((5600,), 72, torch.float32, 4), growing_rows(260, 5600, 5)
+    w[::3] *= 2.0 ** 20
+    w[1::3] *= 2.0 ** -30
+    xd, wd = x.to(dev).requires_grad_(), w.to(dev)
+    y = ops.linear_act8(xd, wd)
+    dx, = torch.autograd.grad(y, xd, dy.to(dev))
+    want = ref.linear_act8(x, w, None, dy)
+    # on top of the float32 bound: what an fp16 pair drops below 2^-33 of the largest value of its row (of x, dy; 448 2^e) or column
+    # (of W), against the largest of the other operand
+    def dropped(a, b):
+        return 2.0 ** -32 * (a.double().abs().amax(1, keepdim=True) * b.double().abs().sum(0) + a.double().abs().sum(1, keepdim=True) * b.double().abs().amax(0))
+    ref.check(y, want["y"], want["y_tol"] + dropped(x, w.t()), "y")
+    ref.check(dx, want["dx"], want["dx_tol"] + dropped(dy, w), "dx")
+
+
+def test_linear_act8_rows_and_columns_of_every_scale():
+    with emu.emulated_gpu():
+        run_scales()
+
+
 def test_linear_act8_only_some_gradients_and_expanded_dy():
     x, w, b = cases.rows((20,), 40, torch.float32, 3), cases.rows((9,), 40, torch.float32, 4), torch.zeros(9)
     dy = torch.ones(20, 9)
@@ -405,14 +437,16 @@ def test_c_entries_refuse_without_a_launch():
     assert bwd() == EWS
     for kw in (dict(x=None), dict(codes=a), dict(st=None), dict(ldgn=3)):
         assert bwd(**kw) == EINVAL, kw
-    assert lib.gridgcn_linear_act8_fwd(a, 0, 4, 8, 8, None, None, 4, a, None, None, None) == EINVAL
-    assert lib.gridgcn_linear_act8_fwd(a, 0, 4, 8, 8, a, None, 4, a, a, None, None) == EINVAL
-    assert lib.gridgcn_linear_act8_fwd(a, 0, 4, 8, 4, a, None, 4, a, None, None, None) == EINVAL
-    assert lib.gridgcn_linear_act8_bwd_workspace_bytes(0, 8, 4, ctypes.byref(n)) == EINVAL
+    assert lib.gridgcn_linear_act8_fwd(a, 0, 4, 8, 8, None, None, 4, a, None, None, None, 0, None) == EINVAL
+    assert lib.gridgcn_linear_act8_fwd(a, 0, 4, 8, 8, a, None, 4, a, a, None, None, 0, None) == EINVAL
+    assert lib.gridgcn_linear_act8_fwd(a, 0, 4, 8, 4, a, None, 4, a, None, None, None, 0, None) == EINVAL
+    assert lib.gridgcn_linear_act8_fwd(a, 0, 1 << 20, 8, 8, a, None, 4, a, None, None, None, 0, None) == EWS
+    assert lib.gridgcn_linear_act8_workspace_bytes(0, 8, 4, 0, 0, ctypes.byref(n)) == EINVAL
+    assert lib.gridgcn_linear_act8_workspace_bytes(1, 8, 4, 5, 0, ctypes.byref(n)) == EINVAL
     assert lib.gridgcn_linear_act8_bwd(a, 0, 4, 4, 4, None, 8, a, a, a, a, a, a, 256, None) == EINVAL
     assert lib.gridgcn_linear_act8_bwd(a, 0, 4, 4, 4, a, 8, None, None, a, a, a, a, 256, None) == EINVAL
     assert lib.gridgcn_linear_act8_bwd(a, 0, 1 << 20, 4, 4, a, 8, a, a, None, a, None, a, 256, None) == EWS
-    assert lib.gridgcn_linear_act8_fwd(a, 0, 4, 8, (1 << 24) + 1, a, None, 4, a, None, None, None) == EINVAL
+    assert lib.gridgcn_linear_act8_fwd(a, 0, 4, 8, (1 << 24) + 1, a, None, 4, a, None, None, None, 0, None) == EINVAL
 
 
 def test_torch_ops_trace_on_fake_tensors():

@@ -66,6 +66,10 @@ def test_linear_act8(case, dtype):
     cpu.check_linear(got, want, case)
 
 
+def test_linear_act8_rows_and_columns_of_every_scale():
+    cpu.run_scales(DEV)
+
+
 def test_group_norm_relu_gate_at_the_border():
     """as on the CPU, at many rows: the gate is that of 64 bits"""
     x = cases.rows((1, 4000), 4, torch.float32, 11)
