@@ -31,6 +31,7 @@ typedef gg_u32x4 gg_u32x4_a2 __attribute__((aligned(2)));
 typedef gg_u32x2 gg_u32x2_a2 __attribute__((aligned(2)));
 typedef gg_u32x2 gg_u32x2_a4 __attribute__((aligned(4)));
 typedef unsigned gg_u32_a1 __attribute__((aligned(1)));
+typedef unsigned gg_u32_a2 __attribute__((aligned(2)));
 
 __device__ __forceinline__ float gg_lo16f(unsigned u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float gg_hi16f(unsigned u) { return __uint_as_float(u & 0xffff0000u); }

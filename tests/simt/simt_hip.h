@@ -626,6 +626,8 @@ static inline int simt_perm(unsigned a, unsigned b, unsigned sel)     // v_perm_
     return (int)r;
 }
 #define __builtin_amdgcn_perm simt_perm
+static inline unsigned simt_alignbit(unsigned hi, unsigned lo, unsigned n) { return (unsigned)((((uint64_t)hi << 32) | lo) >> (n & 31)); }
+#define __builtin_amdgcn_alignbit simt_alignbit
 #define __expf expf                                                    // (the GPU's: exp2 of a rounded product)
 
 static inline float rsqrtf(float x) { return 1.0f / sqrtf(x); }   // (the GPU's is an approximation within 1 ulp)
