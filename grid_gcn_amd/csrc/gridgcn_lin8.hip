@@ -528,12 +528,12 @@ unsigned v[Block<T>::CH];
 
 // ---- dW, db: the contraction runs over the rows.  A lane loads four neighbouring columns of a row (dy: 16 or 8 bytes, codes: 4)
 // for eight rows: the values of one column are then the 8 consecutive contraction elements an operand wants -- no transposition --
-// and the neighbouring columns are tiles (of dy: two, tile i holds the columns 2 j + i; of x^: four, 4 j + t).  A wave owns 64 x 128
-// results in 128 registers and strips of 16 rows (two waves per SIMD: one unpacks while the other multiplies; 128 x 128 in 256
-// registers, alone on its SIMD, took turns with itself); the waves of a workgroup add up in LDS, the workgroups of a tile
-// through memory in one order. -------------------------------------------------------------------------------------------------
+// and the four columns are four tiles (tile i holds the columns 4 j + i).  A wave owns 128 x 128 results in 256 registers and
+// strips of 16 rows; the waves of a workgroup add up in LDS, the workgroups of a tile through memory in one order.
+// What counts here is the number of vector instructions: on a SIMD they take turns with the matrix instructions (5 cycles each
+// beside 32 per matrix instruction, measured on both layouts; two waves of 64 x 128 unpack the codes twice and were slower).
 constexpr int GT = 128;           // results of a tile per side
-constexpr int GW = 4;             // waves that share the strips, for each half of dy's columns
+constexpr int GW = 4;             // waves
 struct Wg {
     const void *dy;               // [R][N], stride ldy
     const uint8_t *codes, *scales; // without dw (tk = 1): any four readable bytes, Cp = 0
@@ -545,7 +545,8 @@ struct Wg {
 };
 
 template <class T> struct Strip {
-    unsigned d[8][sizeof(T) / 2];     // two columns of dy
+    static constexpr int DW = sizeof(T) == 4 ? 4 : 2;
+    unsigned d[8][DW];                // four columns of dy
     unsigned c[8], s[8];              // four codes; the scale bytes of the tile's four blocks (one word: a loop-carried byte is widened
                                       // at the loop's end, which waits for its load)
     // rows 8 h + 0..7 of a strip that lies inside: `dy`, `codes`, `scales` are the strip's first row (uniform), od / oc / os the lane's
@@ -557,10 +558,12 @@ template <class T> struct Strip {
         for (int i = 0; i < 8; i++) {
             const char *q = dy + (size_t)i * p.ldy * sizeof(T);
             if constexpr (sizeof(T) == 4) {
-                const gg_u32x2 u = *(const gg_u32x2_a4 *)(q + od);
-                d[i][0] = u[0]; d[i][1] = u[1];
+                const gg_u32x4 u = *(const gg_u32x4_a4 *)(q + od);
+#pragma unroll
+                for (int t = 0; t < 4; t++) d[i][t] = u[t];
             } else {
-                d[i][0] = *(const gg_u32_a2 *)(q + od);
+                const gg_u32x2 u = *(const gg_u32x2_a2 *)(q + od);
+                d[i][0] = u[0]; d[i][1] = u[1];
             }
             c[i] = *(const unsigned *)(codes + (size_t)i * p.Cp + oc);
             s[i] = *(const gg_u32_a1 *)(scales + (size_t)i * (p.Cp / 32) + os);
@@ -576,14 +579,14 @@ template <class T> struct Strip {
             const bool in = r < p.R;
             const T *q = (const T *)p.dy + (size_t)(in ? r : 0) * p.ldy;
 #pragma unroll
-            for (int t = 0; t < 2; t++) {
+            for (int t = 0; t < 4; t++) {
                 unsigned v;
                 const T *e = q + (n + t < p.N ? n + t : 0);
                 if constexpr (sizeof(T) == 4) v = *(const unsigned *)e;
                 else v = *(const unsigned short *)e;
                 if (!in || n + t >= p.N) v = 0u;
                 if constexpr (sizeof(T) == 4) d[i][t] = v;
-                else d[i][0] = t ? d[i][0] | (v << 16) : v;
+                else d[i][t / 2] = t & 1 ? d[i][t / 2] | (v << 16) : v;
             }
             c[i] = 0u;
             s[i] = 0u;
@@ -596,8 +599,8 @@ template <class T> struct Strip {
     __device__ __forceinline__ float dyv(int i, int t) const
     {
         if constexpr (sizeof(T) == 4) return __uint_as_float(d[i][t]);
-        else if constexpr (std::is_same<T, gg_bf16>::value) return t ? gg_hi16f(d[i][0]) : gg_lo16f(d[i][0]);
-        else return gg_f16of(d[i][0], t);
+        else if constexpr (std::is_same<T, gg_bf16>::value) return (t & 1) ? gg_hi16f(d[i][t / 2]) : gg_lo16f(d[i][t / 2]);
+        else return gg_f16of(d[i][t / 2], t & 1);
     }
     // column t of dy as an operand
     __device__ __forceinline__ void frag_dy(int t, gg_u32x4 (&f)[Ty<T>::P]) const
@@ -609,59 +612,67 @@ template <class T> struct Strip {
                 split2(__uint_as_float(d[2 * q][t]), __uint_as_float(d[2 * q + 1][t]), h, m, l);
                 f[0][q] = h; f[1][q] = m; f[2][q] = l;
             } else {
-                f[0][q] = gg_pair16(d[2 * q][0], d[2 * q + 1][0], t);
+                f[0][q] = gg_pair16(d[2 * q][t / 2], d[2 * q + 1][t / 2], t & 1);
             }
         }
     }
-    // the four columns of x^ as operands (exact in 16 bits)
+    // two codes of a row with their scale, as two 16-bit numbers (exact)
+    static __device__ __forceinline__ unsigned two(unsigned c, float scale, bool high)
+    {
+        if constexpr (std::is_same<T, gg_f16>::value) {
+            if (high) return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)c, scale, true));
+            return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)c, scale, false));
+        } else {
+            if (high) return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)c, scale, true));
+            return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)c, scale, false));
+        }
+    }
+    // the four columns of x^ as operands
     __device__ __forceinline__ void frag_x(gg_u32x4 (&f)[4][1], unsigned turn) const
     {
         // (2^E: the lane's byte turned to the exponent's place)
         auto scale = [&](unsigned w) { return __uint_as_float((unsigned)__builtin_amdgcn_alignbit(w, w, turn) & 0x7f800000u); };
 #pragma unroll
         for (int q = 0; q < 4; q++) {
-            float u[4], v[4];
-            gg_a8_dec4(c[2 * q], u[0], u[1], u[2], u[3]);
-            gg_a8_dec4(c[2 * q + 1], v[0], v[1], v[2], v[3]);
             const float su = scale(s[2 * q]), sv = scale(s[2 * q + 1]);
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                if constexpr (std::is_same<T, gg_f16>::value) f[t][0][q] = gg_cvt_f16(u[t] * su, v[t] * sv);
-                else f[t][0][q] = gg_pair16(__float_as_uint(u[t] * su), __float_as_uint(v[t] * sv), 1);
+            for (int t = 0; t < 4; t += 2) {
+                const unsigned u = two(c[2 * q], su, t != 0), v = two(c[2 * q + 1], sv, t != 0);
+                f[t][0][q] = gg_pair16(u, v, 0);
+                f[t + 1][0][q] = gg_pair16(u, v, 1);
             }
         }
     }
 };
 
 template <class T>
-__global__ __launch_bounds__(2 * GW * 64, 2) void gg_k_lin8_wgrad(Wg p)
+__global__ __launch_bounds__(GW * 64, 1) void gg_k_lin8_wgrad(Wg p)
 {
     constexpr int P = Ty<T>::P;
-    constexpr int D = sizeof(T) == 4 ? 2 : 3;                       // strips in registers, one of them in use
-    extern __shared__ __attribute__((aligned(16))) float ldsf[];    // [2][GW][4][16][64]
+    constexpr int D = 3;                                            // strips in registers, one of them in use
+    extern __shared__ __attribute__((aligned(16))) float ldsf[];    // [GW][4][16][64]
     // (the tiles of one split read the same rows: same XCD, as in place())
     const unsigned tiles = p.tn * p.tk, id = blockIdx.x, xcd = id & 7, slot = id >> 3;
     const unsigned tile = slot % tiles, split = (slot / tiles) * 8 + xcd;
     if (split >= p.splits) return;
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), wave = w % GW, half = w / GW;
-    const int h = lane >> 5, j = lane & 31;
-    const int n0 = (int)(tile / p.tk) * GT, k0 = (int)(tile % p.tk) * GT, n = n0 + 64 * half + 2 * j, k = k0 + 4 * j;
-    const bool first = tile % p.tk == 0;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5, j = lane & 31;
+    const int n0 = (int)(tile / p.tk) * GT, k0 = (int)(tile % p.tk) * GT, n = n0 + 4 * j, k = k0 + 4 * j;
+    const bool first = tile % p.tk == 0 && p.db;
     const long long strips = (p.R + 15) / 16, stride = (long long)p.splits * GW;
     // Strips that are loaded unchecked.  What a lane reads behind the last column belongs to results that nobody stores (such lanes
-    // read the columns from 0 on, and at most one value of dy and three scale bytes behind a row's end: the rows of these strips have
-    // four more behind them).
+    // read the columns from 0 on, and at most three values of dy and three scale bytes behind a row's end: the rows of these strips
+    // have four more behind them).
     const long long whole = p.R > 4 ? (p.R - 4) / 16 : 0;
     const unsigned od = (unsigned)((8 * h * p.ldy + (n < p.N ? n : 0)) * (long long)sizeof(T));
     const int kc = k < p.Cp ? k : 0;
     const unsigned oc = (unsigned)(8 * h * p.Cp + kc), os = (unsigned)(8 * h * (p.Cp / 32) + (p.Cp ? k0 / 32 : 0));
     const unsigned turn = (8 * (k / 32 % 4) + 9) & 31;
-    F16 acc[2][4];
+    F16 acc[4][4];
 #pragma unroll
-    for (int i = 0; i < 2; i++)
+    for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int t = 0; t < 4; t++) acc[i][t] = zero16();
-    float dbs[2] = {0.f, 0.f};
+    float dbs[4] = {0.f, 0.f, 0.f, 0.f};
     Strip<T> q[D];
     // (never skipped -- past the end a strip is loaded again: behind a load that may or may not have been issued the compiler waits
     //  for everything in flight)
@@ -674,14 +685,14 @@ __global__ __launch_bounds__(2 * GW * 64, 2) void gg_k_lin8_wgrad(Wg p)
         gg_u32x4 fx[4][1];
         s.frag_x(fx, turn);
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < 4; i++) {
             gg_u32x4 fd[P];
             s.frag_dy(i, fd);
             mul<Ty<T>>(fd, fx, acc[i]);
         }
         if (first) {
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
+            for (int i = 0; i < 4; i++) {
                 float v = s.dyv(0, i);
 #pragma unroll
                 for (int e = 1; e < 8; e++) v += s.dyv(e, i);
@@ -713,16 +724,15 @@ __global__ __launch_bounds__(2 * GW * 64, 2) void gg_k_lin8_wgrad(Wg p)
         s.load_tail(p, g * 16 + 8 * h, n, k);
         use(s);
     }
-    // the sums of a half's waves, one of its two tiles of rows at a time
+    // the waves' sums: a quarter of the tile's rows at a time
     float *pt = p.part ? p.part + ((size_t)split * tiles + tile) * GT * GT : nullptr;
-    float *mine = ldsf + half * GW * 4 * 16 * 64;
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
+    for (int i = 0; i < 4; i++) {
         __syncthreads();
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int r = 0; r < 16; r++) mine[((wave * 4 + t) * 16 + r) * 64 + lane] = acc[i][t][r];
+            for (int r = 0; r < 16; r++) ldsf[((wave * 4 + t) * 16 + r) * 64 + lane] = acc[i][t][r];
         __syncthreads();
 #pragma unroll
         for (int e = 0; e < 16 / GW; e++) {
@@ -730,26 +740,25 @@ __global__ __launch_bounds__(2 * GW * 64, 2) void gg_k_lin8_wgrad(Wg p)
             float v[4];
 #pragma unroll
             for (int t = 0; t < 4; t++) {
-                v[t] = mine[(t * 16 + r) * 64 + lane];
+                v[t] = ldsf[(t * 16 + r) * 64 + lane];
 #pragma unroll
-                for (int o = 1; o < GW; o++) v[t] += mine[((o * 4 + t) * 16 + r) * 64 + lane];
+                for (int o = 1; o < GW; o++) v[t] += ldsf[((o * 4 + t) * 16 + r) * 64 + lane];
             }
-            const int nl = 64 * half + 2 * ggm_row(r, lane) + i;
+            const int nl = 4 * ggm_row(r, lane) + i;
             if (pt) *(float4 *)(pt + (size_t)nl * GT + 4 * j) = make_float4(v[0], v[1], v[2], v[3]);
             else if (p.dw && n0 + nl < p.N) put_row<T, 4>((T *)p.dw, n0 + nl, k, p.K, v);
         }
     }
-    if (!first || !p.db) return;
+    if (!first) return;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 2; i++) mine[(wave * 2 + i) * 64 + lane] = dbs[i];
+    for (int i = 0; i < 4; i++) ldsf[(wave * 4 + i) * 64 + lane] = dbs[i];
     __syncthreads();
     if ((int)threadIdx.x < GT) {
-        const int c = threadIdx.x % 64, jj = c / 2, i = c % 2;
-        const float *from = ldsf + (threadIdx.x / 64) * GW * 4 * 16 * 64;
+        const int jj = threadIdx.x / 4, i = threadIdx.x % 4;
         float v = 0.f;
 #pragma unroll
-        for (int o = 0; o < GW; o++) v += from[(o * 2 + i) * 64 + jj] + from[(o * 2 + i) * 64 + jj + 32];
+        for (int o = 0; o < GW; o++) v += ldsf[(o * 4 + i) * 64 + jj] + ldsf[(o * 4 + i) * 64 + jj + 32];
         const int nn = n0 + (int)threadIdx.x;
         if (p.part) p.dbpart[(size_t)split * p.tn * GT + nn] = v;
         else if (nn < p.N) GGRowT<T>::put((T *)p.db + nn, v);
@@ -842,14 +851,14 @@ size_t wgrad_bytes(long long R, unsigned tn, unsigned tk)
 template <class T> int launch_wgrad(Wg &p, hipStream_t st)
 {
     static GGDevOnce done;
-    constexpr int LDS = 2 * GW * 4 * 16 * 64 * 4;
+    constexpr int LDS = GW * 4 * 16 * 64 * 4;
     if (!done) {
         if (hipFuncSetAttribute((const void *)gg_k_lin8_wgrad<T>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS) != hipSuccess)
             return GRIDGCN_ELAUNCH;
         done = true;
     }
     const unsigned tiles = p.tn * p.tk;
-    gg_k_lin8_wgrad<T><<<(p.splits + 7) / 8 * 8 * tiles, 2 * GW * 64, LDS, st>>>(p);
+    gg_k_lin8_wgrad<T><<<(p.splits + 7) / 8 * 8 * tiles, GW * 64, LDS, st>>>(p);
     if (p.splits > 1) {
         const unsigned nw = p.dw ? tiles * (GT * GT / 128) : 0, nd = p.db ? p.tn : 0;
         gg_k_lin8_wsum<T><<<nw + nd, 256, 0, st>>>(p, nw);

@@ -616,6 +616,21 @@ static inline void simt_global_load_lds(const void *g, void *l, int size, int of
     memcpy((char *)l + off + simt_cur->lane * size, (const char *)g + off, size);
 }
 #define __builtin_amdgcn_global_load_lds simt_global_load_lds
+// v_cvt_scalef32_pk_{bf16,f16}_fp8: two codes of a half of the word times 2^(exponent of scale - 127)
+typedef __bf16 simt_bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 simt_f16x2 __attribute__((ext_vector_type(2)));
+static inline simt_bf16x2 simt_cvt_scalef32_pk_bf16_fp8(int w, float scale, bool high)
+{
+    const simt_f32x2 v = simt_cvt_pk_f32_fp8(w, high);
+    return simt_bf16x2{(__bf16)(v[0] * scale), (__bf16)(v[1] * scale)};
+}
+static inline simt_f16x2 simt_cvt_scalef32_pk_f16_fp8(int w, float scale, bool high)
+{
+    const simt_f32x2 v = simt_cvt_pk_f32_fp8(w, high);
+    return simt_f16x2{(_Float16)(v[0] * scale), (_Float16)(v[1] * scale)};
+}
+#define __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8 simt_cvt_scalef32_pk_bf16_fp8
+#define __builtin_amdgcn_cvt_scalef32_pk_f16_fp8 simt_cvt_scalef32_pk_f16_fp8
 static inline float simt_rcp(float x) { return 1.0f / x; }
 #define __builtin_amdgcn_rcpf simt_rcp
 static inline int simt_perm(unsigned a, unsigned b, unsigned sel)     // v_perm_b32: bytes 0-3 from b, 4-7 from a

@@ -49,6 +49,27 @@ def test_act8_every_code_and_scale():
 
 
 @pytest.mark.parametrize("dtype", cases.DTYPES)
+def test_linear_act8_every_code_and_scale(dtype):
+    """dW of unit rows of dy: row n of dW is the value of row n of the codes, whatever its scale"""
+    from grid_gcn_amd import act8
+    scale = torch.arange(10, 248) if dtype != torch.float16 else torch.arange(127 - 15, 127 + 8)     # (fp16: what packing fp16 gives)
+    R = len(scale)
+    codes = torch.arange(256, dtype=torch.uint8).view(1, 256).repeat(R, 1)
+    codes[(codes & 0x7f) == 0x7f] = 0                    # (NaN would reach every result of its column)
+    scales = scale.to(torch.uint8).view(R, 1).repeat(1, 8)
+    if dtype != torch.float16:
+        codes[scales.repeat_interleave(32, 1) > 246] &= 0xf7          # (2^128 and beyond)
+    values = codes.view(torch.float8_e4m3fn).double() * torch.exp2(scales.double() - 127).repeat_interleave(32, 1)
+    if dtype == torch.float16:
+        values = values.half().double()                  # (below 2^-24: not what packing gives)
+    dy = torch.eye(R, dtype=dtype, device=DEV)
+    w = torch.zeros(R, 256, dtype=dtype, device=DEV)
+    _, dw, _ = act8._linear_backward(dy, w, codes.to(DEV), scales.to(DEV), (R, 256), (False, True, False))
+    assert bool(torch.isfinite(values).all())
+    assert torch.equal(dw.cpu().double(), values.to(dtype).double())
+
+
+@pytest.mark.parametrize("dtype", cases.DTYPES)
 @pytest.mark.parametrize("case", cases.GN + [
     (4, 20000, 128, 32, "silu", False, False, 0), (3, 9000, 200, 8, "relu", True, True, 1), (32, 700, 64, 8, "gelu", True, True, 0),
     (1, 50000, 24, 3, "relu", False, False, 0), (300, 1, 512, 32, "relu", False, False, 0), (2, 300, 2048, 1, "none", False, True, 0)])
