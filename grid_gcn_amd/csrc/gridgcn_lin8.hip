@@ -150,6 +150,22 @@ template <class T> struct Block {
     // lane of the wave calls).  clean: as gg_a8_block_byte
     __device__ __forceinline__ unsigned byte(bool &clean) const
     {
+        if constexpr (CH == 32) {
+            // 16-bit rows: the largest of the bit patterns, two at a time
+            typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+            u16x2 m2 = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const unsigned u = w[i][j] & 0x7fff7fffu;
+                    m2 = __builtin_elementwise_max(m2, __builtin_bit_cast(u16x2, u));
+                }
+            const unsigned m = m2[0] > m2[1] ? m2[0] : m2[1];
+            constexpr bool BF = std::is_same<T, gg_bf16>::value;
+            clean = !__any(m >= (BF ? 0x7f80u : 0x7c00u));
+            if (clean) return gg_a8_byte(BF ? m << 16 : __float_as_uint(gg_f16of(m, 0)));
+        }
         auto top = [&](bool finite) {
             unsigned m = 0;
 #pragma unroll
@@ -168,19 +184,38 @@ template <class T> struct Block {
         if (!clean) m = top(true);
         return gg_a8_byte(m);
     }
+    // four values of 16 bits / scale as codes
+    static __device__ __forceinline__ unsigned enc(unsigned lo, unsigned hi, float scale)
+    {
+        typedef short s16x2 __attribute__((ext_vector_type(2)));
+        s16x2 r = {0, 0};
+        if constexpr (std::is_same<T, gg_f16>::value) {
+            r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(gg_f16x2, lo), scale, false);
+            r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r, __builtin_bit_cast(gg_f16x2, hi), scale, true);
+        } else {
+            r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(gg_bf16x2, lo), scale, false);
+            r = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r, __builtin_bit_cast(gg_bf16x2, hi), scale, true);
+        }
+        return __builtin_bit_cast(unsigned, r);
+    }
     // codes of channels 16 i .. 16 i + 15 of the lane's share
     __device__ __forceinline__ gg_u32x4 codes(int i, unsigned byte, bool clean) const
     {
-        Block b = *this;
-#pragma unroll
-        for (int j = 0; j < 4; j++) asm volatile("" : "+v"(b.w[j]));     // (16-bit rows: unpacked again, not held unpacked since byte())
         gg_u32x4 o;
+        if constexpr (CH == 32) {
+            if (clean) {                          // two values of 16 bits to two codes in one instruction
+                const float scale = gg_a8_scale(byte);
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[j] = enc(w[2 * i + j / 2][2 * (j & 1)], w[2 * i + j / 2][2 * (j & 1) + 1], scale);
+                return o;
+            }
+        }
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             float v[4];
             unsigned w[1];
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[e] = b.get(16 * i + 4 * j + e);
+            for (int e = 0; e < 4; e++) v[e] = get(16 * i + 4 * j + e);
             gg_a8_encode<4>(v, byte, clean, w);
             o[j] = w[0];
         }

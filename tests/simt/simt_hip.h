@@ -629,6 +629,15 @@ static inline simt_f16x2 simt_cvt_scalef32_pk_f16_fp8(int w, float scale, bool h
     const simt_f32x2 v = simt_cvt_pk_f32_fp8(w, high);
     return simt_f16x2{(_Float16)(v[0] * scale), (_Float16)(v[1] * scale)};
 }
+// v_cvt_scalef32_pk_fp8_{bf16,f16}: two values over 2^(exponent of scale - 127) to codes of a half of the word
+typedef short simt_s16x2 __attribute__((ext_vector_type(2)));
+template <class V> static inline simt_s16x2 simt_cvt_scalef32_pk_fp8(simt_s16x2 old, V v, float scale, bool high)
+{
+    old[high ? 1 : 0] = (short)(simt_f32_to_e4m3((float)v[0] / scale) | ((unsigned)simt_f32_to_e4m3((float)v[1] / scale) << 8));
+    return old;
+}
+#define __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16 simt_cvt_scalef32_pk_fp8
+#define __builtin_amdgcn_cvt_scalef32_pk_fp8_f16 simt_cvt_scalef32_pk_fp8
 #define __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8 simt_cvt_scalef32_pk_bf16_fp8
 #define __builtin_amdgcn_cvt_scalef32_pk_f16_fp8 simt_cvt_scalef32_pk_f16_fp8
 static inline float simt_rcp(float x) { return 1.0f / x; }

@@ -223,6 +223,30 @@ def test_linear_act8(case, dtype):
     check_linear(got, want, case)
 
 
+def check_codes(R, K, dtype, dev="cpu"):
+    """the 8-bit form that the linear layer writes is act8_pack's, special values among the rows"""
+    from grid_gcn_amd import act8
+    sp = cases.special_rows(dtype)
+    x = cases.rows((R,), K, dtype, 3)
+    rep = sp.repeat(1, -(-K // 32))[:, :K]
+    x[::max(1, R // len(rep))][:len(rep)] = rep[:len(x[::max(1, R // len(rep))])]
+    x = x.to(dev)
+    w = torch.zeros(3, K, dtype=dtype, device=dev)
+    _, codes, scales = act8._linear_forward(x, w, None, True)
+    c, s = ops.act8_pack(x)
+    assert torch.equal(scales, s)
+    assert torch.equal(codes & 0x7f, c & 0x7f)                    # (a NaN has no sign)
+    ok = (c & 0x7f) != 0x7f
+    assert torch.equal(codes[ok], c[ok])
+
+
+@pytest.mark.parametrize("dtype", cases.DTYPES)
+@pytest.mark.parametrize("R,K", [(40, 70), (90, 128)])
+def test_linear_act8_writes_the_same_codes(R, K, dtype):
+    with emu.emulated_gpu():
+        check_codes(R, K, dtype)
+
+
 def growing_rows(R, K, seed):
     """rows whose magnitude grows along them by 2^40, starts with zeros, falls off, or is far from 1 as a whole"""
     x = cases.rows((R,), K, torch.float32, seed)

@@ -87,6 +87,12 @@ def test_linear_act8(case, dtype):
     cpu.check_linear(got, want, case)
 
 
+@pytest.mark.parametrize("dtype", cases.DTYPES)
+@pytest.mark.parametrize("R,K", [(40, 70), (90, 128), (17000, 131), (20000, 512)])
+def test_linear_act8_writes_the_same_codes(R, K, dtype):
+    cpu.check_codes(R, K, dtype, DEV)
+
+
 def test_linear_act8_rows_and_columns_of_every_scale():
     cpu.run_scales(DEV)
 
