@@ -29,7 +29,6 @@ typedef unsigned gg_u32x2 __attribute__((ext_vector_type(2)));
 typedef gg_u32x4 gg_u32x4_a4 __attribute__((aligned(4)));
 typedef gg_u32x4 gg_u32x4_a2 __attribute__((aligned(2)));
 typedef gg_u32x2 gg_u32x2_a2 __attribute__((aligned(2)));
-typedef gg_u32x2 gg_u32x2_a4 __attribute__((aligned(4)));
 typedef unsigned gg_u32_a1 __attribute__((aligned(1)));
 typedef unsigned gg_u32_a2 __attribute__((aligned(2)));
 
@@ -52,82 +51,77 @@ __device__ __forceinline__ unsigned gg_cvt_f16(float a, float b)
 // (by value: __builtin_bit_cast of an ELEMENT of a vector takes element 0)
 __device__ __forceinline__ float gg_f16of(unsigned u, int i) { return (float)__builtin_bit_cast(gg_f16x2, u)[i]; }
 
+// Results that no cache can hold are stored around them (`past`): what an ordinary store leaves dirty is written back while the
+// next pass reads.  Forward and backward of a group normalisation, and a pass over its output, fp32 rows of 128:
+//   336 MB   518 -> 473 us, forward + scaling it 314 -> 308, + sum of it 286 -> 274;    268 MB   413 -> 376, 256 -> 248, 240 -> 222
+//   134 MB   203 -> 187,                         128 -> 123,             106 -> 114;     67 MB   104 -> 105,  61 ->  64,  61 ->  68
+// so the border is where the reader of the result would find little of it in the 256 MB of the last cache anyway.
+static inline bool gg_past_caches(long long rows, long long C, int dtype)
+{
+    return rows * C >= (192ll << 20) / (dtype == GG_T_F32 ? 4 : 2);
+}
+// one store of a 16- or 8-byte vector that is aligned to an element of T
+#define GG_STORE(TYPE)                                                                                              \
+    if (past) {                                                                                                     \
+        asm volatile("");              /* keep the two stores apart: merged, they are an ordinary one */            \
+        __builtin_nontemporal_store(v, (TYPE *)p);                                                                  \
+        asm volatile("");                                                                                           \
+    } else {                                                                                                        \
+        *(TYPE *)p = v;                                                                                             \
+    }
+template <class T> __device__ __forceinline__ void gg_st(T *p, gg_u32x4 v, bool past)
+{
+    if constexpr (sizeof(T) == 4) { GG_STORE(gg_u32x4_a4) }
+    else { GG_STORE(gg_u32x4_a2) }
+}
+template <class T> __device__ __forceinline__ void gg_st(T *p, gg_u32x2 v, bool past) { GG_STORE(gg_u32x2_a2) }
+#undef GG_STORE
+
 // ---- rows of T, 16 bytes at a time: V channels ----------------------------------------------------------------------
 template <class T> struct GGRowT;
 template <> struct GGRowT<float> {
     static constexpr int V = 4, id = GG_T_F32;
-    static __device__ __forceinline__ void ld(const float *p, float (&v)[4])
-    {
-        const gg_u32x4 u = *(const gg_u32x4_a4 *)p;
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = __uint_as_float(u[i]);
-    }
-    static __device__ __forceinline__ void st(float *p, const float (&v)[4])
+    static __device__ __forceinline__ void st(float *p, const float (&v)[4], bool past)
     {
         gg_u32x4 u;
 #pragma unroll
         for (int i = 0; i < 4; i++) u[i] = __float_as_uint(v[i]);
-        *(gg_u32x4_a4 *)p = u;
+        gg_st(p, u, past);
     }
     static __device__ __forceinline__ float get(const float *p) { return *p; }
     static __device__ __forceinline__ void put(float *p, float v) { *p = v; }
 };
 template <> struct GGRowT<gg_bf16> {
     static constexpr int V = 8, id = GG_T_BF16;
-    static __device__ __forceinline__ void ld(const gg_bf16 *p, float (&v)[8])
-    {
-        const gg_u32x4 u = *(const gg_u32x4_a2 *)p;
-#pragma unroll
-        for (int i = 0; i < 4; i++) { v[2 * i] = gg_lo16f(u[i]); v[2 * i + 1] = gg_hi16f(u[i]); }
-    }
-    static __device__ __forceinline__ void st(gg_bf16 *p, const float (&v)[8])
+    static __device__ __forceinline__ void st(gg_bf16 *p, const float (&v)[8], bool past)
     {
         gg_u32x4 u;
 #pragma unroll
         for (int i = 0; i < 4; i++) u[i] = gg_cvt_bf16(v[2 * i], v[2 * i + 1]);
-        *(gg_u32x4_a2 *)p = u;
+        gg_st(p, u, past);
     }
     static __device__ __forceinline__ float get(const gg_bf16 *p) { return __uint_as_float((unsigned)*(const unsigned short *)p << 16); }
     static __device__ __forceinline__ void put(gg_bf16 *p, float v) { *(unsigned short *)p = (unsigned short)gg_cvt_bf16(v, 0.f); }
 };
 template <> struct GGRowT<gg_f16> {
     static constexpr int V = 8, id = GG_T_F16;
-    static __device__ __forceinline__ void ld(const gg_f16 *p, float (&v)[8])
-    {
-        const gg_u32x4 u = *(const gg_u32x4_a2 *)p;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            v[2 * i] = gg_f16of(u[i], 0);
-            v[2 * i + 1] = gg_f16of(u[i], 1);
-        }
-    }
-    static __device__ __forceinline__ void st(gg_f16 *p, const float (&v)[8])
+    static __device__ __forceinline__ void st(gg_f16 *p, const float (&v)[8], bool past)
     {
         gg_u32x4 u;
 #pragma unroll
         for (int i = 0; i < 4; i++) u[i] = gg_cvt_f16(v[2 * i], v[2 * i + 1]);
-        *(gg_u32x4_a2 *)p = u;
+        gg_st(p, u, past);
     }
     static __device__ __forceinline__ float get(const gg_f16 *p) { return (float)*p; }
     static __device__ __forceinline__ void put(gg_f16 *p, float v) { *(unsigned short *)p = (unsigned short)gg_cvt_f16(v, 0.f); }
 };
 
-// V channels of a row from channel c on; zeros past C.  No lane crosses the row's end.
-template <class T> __device__ __forceinline__ void gg_ld_chunk(const T *row, int c, int C, float (&v)[GGRowT<T>::V])
+// V channels of a row from channel c on; what lies past C is left alone
+template <class T> __device__ __forceinline__ void gg_st_chunk(T *row, int c, int C, const float (&v)[GGRowT<T>::V], bool past)
 {
     constexpr int V = GGRowT<T>::V;
     if (c + V <= C) {
-        GGRowT<T>::ld(row + c, v);
-    } else {
-#pragma unroll
-        for (int i = 0; i < V; i++) v[i] = c + i < C ? GGRowT<T>::get(row + c + i) : 0.f;
-    }
-}
-template <class T> __device__ __forceinline__ void gg_st_chunk(T *row, int c, int C, const float (&v)[GGRowT<T>::V])
-{
-    constexpr int V = GGRowT<T>::V;
-    if (c + V <= C) {
-        GGRowT<T>::st(row + c, v);
+        GGRowT<T>::st(row + c, v, past);
     } else {
 #pragma unroll
         for (int i = 0; i < V; i++)
@@ -135,24 +129,56 @@ template <class T> __device__ __forceinline__ void gg_st_chunk(T *row, int c, in
     }
 }
 
-// the same chunk as it stands in memory: 4 registers until it is used
-template <class T> struct GGChunk {
-    gg_u32x4 w;
-    __device__ __forceinline__ void load(const T *row, int c, int C)
+// A thread's column: the V channels from c on.  It loads the V channels from `at` on, which end with the row at the latest, and
+// drops the first `drop` of them afterwards: the last chunk of a row costs no branch around its loads (a batch of loads with
+// branches between them goes out one by one).
+template <class T> struct GGCol {
+    int at, drop;
+    bool narrow;                              // rows shorter than a chunk: by element
+    __device__ __forceinline__ GGCol(int c, int C)
     {
         constexpr int V = GGRowT<T>::V;
-        if (c + V <= C) {
-            if constexpr (V == 4) w = *(const gg_u32x4_a4 *)(row + c);
-            else w = *(const gg_u32x4_a2 *)(row + c);
+        narrow = C < V;
+        at = narrow || c + V <= C ? c : C - V;
+        drop = c - at < V ? c - at : V;
+    }
+};
+
+// a chunk as it stands in memory: 4 registers until it is used
+template <class T> struct GGChunk {
+    gg_u32x4 w;
+    __device__ __forceinline__ void load(const T *row, const GGCol<T> &k, int C)
+    {
+        constexpr int V = GGRowT<T>::V;
+        if (!k.narrow) {
+            if constexpr (V == 4) w = *(const gg_u32x4_a4 *)(row + k.at);
+            else w = *(const gg_u32x4_a2 *)(row + k.at);
         } else {
             w = gg_u32x4{0u, 0u, 0u, 0u};
 #pragma unroll
-            for (int i = 0; i < V; i++) {
-                if (c + i >= C) continue;
-                if constexpr (V == 4) w[i] = ((const unsigned *)row)[c + i];
-                else w[i / 2] |= (unsigned)((const unsigned short *)row)[c + i] << (16 * (i & 1));
+            for (int i = 0; i < V - 1; i++) {
+                if (k.at + i >= C) continue;
+                if constexpr (V == 4) w[i] = ((const unsigned *)row)[k.at + i];
+                else w[i / 2] |= (unsigned)((const unsigned short *)row)[k.at + i] << (16 * (i & 1));
             }
         }
+    }
+    // what `load` read, from the column's first channel on; zeros past the row's end
+    __device__ __forceinline__ void align(const GGCol<T> &k)
+    {
+        constexpr int V = GGRowT<T>::V;
+        if (!k.drop) return;
+        int n = k.drop;
+        if constexpr (V == 8) {
+            if (n & 1) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) w[i] = (w[i] >> 16) | (i < 3 ? w[(i + 1) & 3] << 16 : 0u);
+            }
+            n >>= 1;
+        }
+        if (n & 1) w = gg_u32x4{w[1], w[2], w[3], 0u};
+        if (n & 2) w = gg_u32x4{w[2], w[3], 0u, 0u};
+        if (n & 4) w = gg_u32x4{0u, 0u, 0u, 0u};
     }
     __device__ __forceinline__ void zero() { w = gg_u32x4{0u, 0u, 0u, 0u}; }
     __device__ __forceinline__ void get(float (&v)[GGRowT<T>::V]) const

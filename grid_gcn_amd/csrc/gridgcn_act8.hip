@@ -27,19 +27,20 @@ __global__ __launch_bounds__(THREADS) void gg_k_act8_pack(const T *__restrict__ 
     const int Cp = gg_a8_cp(C), nb = Cp / GG_A8_BLOCK;
     const int tr = threadIdx.x / l.tpr, q = blockIdx.y * l.tpr + threadIdx.x % l.tpr, c = q * V;
     const bool on = tr < l.rpb && q < l.nq;     // (a chunk behind C: zeros)
+    const GGCol<T> col(on ? c : 0, C);
     const long long step = (long long)gridDim.x * l.rpb * UNROLL;
     for (long long r0 = (long long)blockIdx.x * l.rpb * UNROLL; r0 < R; r0 += step) {
         GGChunk<T> in[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) {
             const long long r = r0 + (long long)u * l.rpb + tr;
-            if (on && r < R) in[u].load(x + r * ldx, c, C);
-            else in[u].zero();
+            in[u].load(x + (r < R ? r : R - 1) * ldx, col, C);          // (rows past the end: encoded, not stored)
         }
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) {
             const long long r = r0 + (long long)u * l.rpb + tr;
             float v[V];
+            in[u].align(col);
             in[u].get(v);
             bool clean;
             const unsigned byte = gg_a8_block_byte<V>(v, clean);
@@ -55,7 +56,7 @@ __global__ __launch_bounds__(THREADS) void gg_k_act8_pack(const T *__restrict__ 
 
 template <class T>
 __global__ __launch_bounds__(THREADS) void gg_k_act8_unpack(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales,
-                                                            long long R, int C, Lay l, T *__restrict__ x, long long ldx)
+                                                            long long R, int C, Lay l, T *__restrict__ x, long long ldx, bool past)
 {
     constexpr int V = GGRowT<T>::V;
     const int Cp = gg_a8_cp(C), nb = Cp / GG_A8_BLOCK;
@@ -73,7 +74,7 @@ __global__ __launch_bounds__(THREADS) void gg_k_act8_unpack(const uint8_t *__res
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) {
             const long long r = r0 + (long long)u * l.rpb;
-            if (r < R) gg_st_chunk(x + r * ldx, c, C, v[u]);
+            if (r < R) gg_st_chunk(x + r * ldx, c, C, v[u], past);
         }
     }
 }
@@ -95,7 +96,8 @@ template <class T> void pack(const void *x, long long R, int C, long long ldx, u
 template <class T> void unpack(const uint8_t *codes, const uint8_t *scales, long long R, int C, void *x, long long ldx, hipStream_t st)
 {
     const Lay l = lay_of((C + GGRowT<T>::V - 1) / GGRowT<T>::V);
-    gg_k_act8_unpack<T><<<grid_of(R, l), THREADS, 0, st>>>(codes, scales, R, C, l, (T *)x, ldx);
+    gg_k_act8_unpack<T><<<grid_of(R, l), THREADS, 0, st>>>(codes, scales, R, C, l, (T *)x, ldx,
+                                                                 gg_past_caches(R, C, GGRowT<T>::id));
 }
 }  // namespace
 

@@ -14,8 +14,7 @@
 // Numerics.  Sums of the statistics run in 64 bits on x - x[first row, first channel of the group] (64-bit vector adds run at
 // the rate of 32-bit ones here, the passes wait for memory): the variance needs no second look at the data even when the mean is
 // large against it.  The mean is subtracted as two floats, so d is x - mean to 32 bits whatever the mean.  Sums of the backward:
-// 32 bits over UNROLL rows, then 64.  The sign of t decides a whole gradient under ReLU: where |t| is within the rounding of
-// its two terms, it is formed again in 64 bits.  No atomics: every sum has one order.
+// 32 bits over UNROLL rows, then 64.  No atomics: every sum has one order.
 #include "../../include/gridgcn.h"
 #include "gridgcn_act8.h"
 #include <type_traits>
@@ -26,6 +25,8 @@ constexpr int UNROLL = 4;
 constexpr int FEW = 512;                   // threads of the one-launch form, which keeps its values in registers
 template <class T> constexpr int KEEP = sizeof(T) == 4 ? 16 : 8;     // chunks a thread keeps
 constexpr float SQRT1_2 = 0.70710678118654752f, INV_SQRT_2PI = 0.39894228040143268f;
+
+typedef double f64x2 __attribute__((ext_vector_type(2)));
 
 struct Lay { int nq, tpr, rpb; };          // chunks of a slab row, threads per row, rows per step
 Lay lay_of(int nq, int threads = THREADS)
@@ -53,6 +54,7 @@ struct Args {
     double *tot;                           // [B, C, 2] sums of g and g * xh
     float2 *coef;                          // [B, G] rstd S1, rstd^2 S2
     long long rpc;                         // rows of a chunk
+    bool past;                             // y or dx around the caches
     int chunks;
 };
 
@@ -105,39 +107,54 @@ template <int ACT> __device__ __forceinline__ float act_grad(float t)
     return 1.f;
 }
 
+// the largest float that is not above v
+__device__ __forceinline__ float float_below(double v)
+{
+    const float f = (float)v;
+    if (!((double)f > v)) return f;                        // (NaN stays NaN)
+    const unsigned u = __float_as_uint(f);
+    return __uint_as_float(u == 0u ? 0x80000001u : (u >> 31 ? u + 1 : u - 1));
+}
+
 // constants of one channel
-struct Chan { float mh, ml, a, beta; };     // mean in two parts, rstd * gamma, beta
-__device__ __forceinline__ Chan chan_of(const Args &a, double mean, double rstd, int c)
+struct Chan {
+    float mh, ml, a;                        // mean in two parts, rstd * gamma
+    float beta;                             // forward, and the backward of the smooth activations
+    float thr;                              // ReLU backward: t > 0 exactly where `flip`ped x > thr
+    unsigned flip;
+};
+// The sign of t = (x - mean) rstd gamma + beta decides a whole gradient under ReLU, and 32 bits get it wrong where the two terms
+// cancel.  t > 0 is x > mean - beta / (rstd gamma), or < where gamma is negative: that border is formed once per channel in 64 bits
+// and rounded down to a float, which loses nothing against an x that is a float.
+template <int ACT, bool BACKWARD> __device__ __forceinline__ Chan chan_of(const Args &a, double mean, double rstd, int c)
 {
     Chan k;
     k.mh = (float)mean;
     k.ml = (float)(mean - (double)k.mh);
     k.beta = gg_ld_param(a.beta, a.ptype, c, 0.f);
-    k.a = (float)(rstd * (double)gg_ld_param(a.gamma, a.ptype, c, 1.f));
+    const double m = rstd * (double)gg_ld_param(a.gamma, a.ptype, c, 1.f);
+    k.a = (float)m;
+    k.thr = 0.f;
+    k.flip = 0u;
+    if constexpr (BACKWARD && ACT == GRIDGCN_ACT_RELU) {
+        const double t = mean - (double)k.beta / m;
+        k.flip = m < 0.0 ? 0x80000000u : 0u;
+        k.thr = float_below(m < 0.0 ? -t : t);
+        if (m == 0.0) k.thr = k.beta > 0.f ? -INFINITY : INFINITY;
+    }
     return k;
 }
 // ... of the V channels of a thread, from the statistics in memory
-template <int V, class P> __device__ __forceinline__ void chans(const Args &a, const P &p, Chan (&k)[V])
+template <int ACT, bool BACKWARD, int V, class P> __device__ __forceinline__ void chans(const Args &a, const P &p, Chan (&k)[V])
 {
 #pragma unroll
     for (int i = 0; i < V; i++) {
         const int c = p.c + i < a.C ? p.c + i : a.C - 1;
         const double *st = a.stats + ((size_t)p.b * a.G + c / a.cg) * 2;
-        k[i] = chan_of(a, st[0], st[1], c);
+        k[i] = chan_of<ACT, BACKWARD>(a, st[0], st[1], c);
     }
 }
 __device__ __forceinline__ float dev_of(const Chan &k, float x) { return (x - k.mh) - k.ml; }
-
-// ReLU: is t = d a + beta > 0?  The float value is off by less than 2^-21 of |beta| where the two terms cancel.
-__device__ __forceinline__ bool positive(const Chan &k, float t, float x, const double *stat, const Args &a, int c)
-{
-    if (__builtin_expect(fabsf(t) <= fabsf(k.beta) * 0x1p-20f, 0)) {
-        const double *st = stat + (c / a.cg) * 2;
-        const double t64 = ((double)x - st[0]) * st[1] * (double)gg_ld_param(a.gamma, a.ptype, c, 1.f) + (double)k.beta;
-        return t64 > 0.0;
-    }
-    return t > 0.f;
-}
 
 // where the workgroup's threads stand
 template <int V> struct Pos {
@@ -154,6 +171,8 @@ template <int V> struct Pos {
 };
 
 // Sums s[V][2] of the threads of a column over the workgroup's row lanes: LDS red[rpb][tpr * V][2]; afterwards red[0] holds them.
+// All threads take part: strips of rows first, then the strips (a thread per sum alone walks up to 512 rows of LDS one after
+// the other).
 template <int V, int NT> __device__ __forceinline__ void reduce_rows(double *red, const Lay &l, int tr, int qi, const double (&s)[V][2])
 {
     const int w = l.tpr * V * 2;
@@ -165,12 +184,34 @@ template <int V, int NT> __device__ __forceinline__ void reduce_rows(double *red
         }
     }
     __syncthreads();
+    const int strips = NT / w, per = strips > 1 ? (l.rpb + strips - 1) / strips : 1;
+    if (per > 1) {
+        const int k = (int)threadIdx.x / w, r0 = k * per, r1 = r0 + per < l.rpb ? r0 + per : l.rpb;
+        if (k < strips && r0 < r1) {
+            double *q = red + (size_t)threadIdx.x % w;
+            double v = q[(size_t)r0 * w];
+            for (int r = r0 + 1; r < r1; r++) v += q[(size_t)r * w];
+            q[(size_t)r0 * w] = v;         // (this thread's alone)
+        }
+        __syncthreads();
+    }
     for (int j = threadIdx.x; j < w; j += NT) {
         double v = red[j];
-        for (int r = 1; r < l.rpb; r++) v += red[(size_t)r * w + j];
+        for (int r = per; r < l.rpb; r += per) v += red[(size_t)r * w + j];
         red[j] = v;                        // (entry j of row 0 is this thread's alone)
     }
     __syncthreads();
+}
+
+// the values that the sums of a thread's channels are taken from: x[first row, first channel of the group]
+template <class T>
+__device__ __forceinline__ void base_of(const Args &a, const Pos<GGRowT<T>::V> &p, const T *x, double (&base)[GGRowT<T>::V])
+{
+    T w[GGRowT<T>::V];
+#pragma unroll
+    for (int i = 0; i < GGRowT<T>::V; i++) w[i] = x[((p.c + i < a.C ? p.c + i : a.C - 1) / a.cg) * a.cg];
+#pragma unroll
+    for (int i = 0; i < GGRowT<T>::V; i++) base[i] = (double)GGRowT<T>::get(w + i);
 }
 
 // first pass over the rows r0 <= n < r1 of cloud b: sums of x - base and its square per channel, and (SAVE8) the 8-bit form
@@ -181,26 +222,24 @@ __device__ __forceinline__ void rows_stats(const Args &a, const Lay &l, const Po
     constexpr int V = GGRowT<T>::V;
     const T *x = (const T *)a.x + (size_t)p.b * a.xb;
     const int Cp = gg_a8_cp(a.C), nb = Cp / GG_A8_BLOCK;
+    const GGCol<T> col(p.on ? p.c : 0, a.C);
+    base_of<T>(a, p, x, base);                             // (row 0 is valid where any row is)
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-        s[i][0] = s[i][1] = 0.0;
-        const int c = p.c + i < a.C ? p.c + i : a.C - 1;
-        base[i] = r1 > r0 ? (double)GGRowT<T>::get(x + (c / a.cg) * a.cg) : 0.0;      // (row 0 is valid where any row is)
-    }
+    for (int i = 0; i < V; i++) s[i][0] = s[i][1] = 0.0;
     constexpr int U = SAVE8 ? UNROLL : 2 * UNROLL;
     for (long long n0 = r0; n0 < r1; n0 += (long long)l.rpb * U) {
         GGChunk<T> r[U];
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const long long n = n0 + (long long)u * l.rpb + p.tr;
-            if (p.on && n < r1) r[u].load(x + (size_t)n * a.xn, p.c, a.C);
-            else r[u].zero();
+            r[u].load(x + (size_t)(n < r1 ? n : r1 - 1) * a.xn, col, a.C);        // (rows past the end: in no sum, not stored)
         }
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const long long n = n0 + (long long)u * l.rpb + p.tr;
             const bool in = p.on && n < r1;
             float v[V];
+            r[u].align(col);
             r[u].get(v);
             if (in) {
 #pragma unroll
@@ -245,6 +284,7 @@ __device__ __forceinline__ void rows_apply(const Args &a, const Lay &l, const Po
     const T *x = (const T *)a.x + (size_t)p.b * a.xb;
     T *y = (T *)a.y + (size_t)p.b * a.N * a.C;
     if (!p.on) return;
+    const GGCol<T> col(p.c, a.C);
     const long long rv = r1 < count ? r1 : count;          // rows with values
     long long n0 = r0 + p.tr;
     for (; n0 < rv; n0 += (long long)l.rpb * UNROLL) {
@@ -252,48 +292,52 @@ __device__ __forceinline__ void rows_apply(const Args &a, const Lay &l, const Po
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) {
             const long long n = n0 + (long long)u * l.rpb;
-            r[u].load(x + (size_t)(n < rv ? n : n0) * a.xn, p.c, a.C);
+            r[u].load(x + (size_t)(n < rv ? n : n0) * a.xn, col, a.C);
         }
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) {
             const long long n = n0 + (long long)u * l.rpb;
             if (n >= r1) continue;
             float v[V], o[V];
+            r[u].align(col);
             r[u].get(v);
 #pragma unroll
             for (int i = 0; i < V; i++) o[i] = n < rv ? act_of<ACT>(fmaf(dev_of(k[i], v[i]), k[i].a, k[i].beta)) : 0.f;
-            gg_st_chunk(y + (size_t)n * a.C, p.c, a.C, o);
+            gg_st_chunk(y + (size_t)n * a.C, p.c, a.C, o, a.past);
         }
     }
     float z[V];
 #pragma unroll
     for (int i = 0; i < V; i++) z[i] = 0.f;
-    for (; n0 < r1; n0 += l.rpb) gg_st_chunk(y + (size_t)n0 * a.C, p.c, a.C, z);
+    for (; n0 < r1; n0 += l.rpb) gg_st_chunk(y + (size_t)n0 * a.C, p.c, a.C, z, a.past);
 }
 
-// x^ of one chunk as it stands in memory: the input itself or its 8-bit form
+// x^ of one chunk as it stands in memory: the input itself or its 8-bit form (whose rows are whole chunks)
 template <class T, bool Q8> struct Xhat {
     typename std::conditional<Q8, GGCodes<GGRowT<T>::V>, GGChunk<T>>::type r;
-    __device__ __forceinline__ void load(const Args &a, const Pos<GGRowT<T>::V> &p, long long n)
+    __device__ __forceinline__ void load(const Args &a, const Pos<GGRowT<T>::V> &p, const GGCol<T> &col, long long n)
     {
         if constexpr (Q8) {
             const int Cp = gg_a8_cp(a.C);
             const size_t row = (size_t)p.b * a.N + n;
             r.load(a.codes + row * Cp + p.c, a.scales + row * (Cp / GG_A8_BLOCK) + p.c / GG_A8_BLOCK);
         } else {
-            r.load((const T *)a.x + (size_t)p.b * a.xb + (size_t)n * a.xn, p.c, a.C);
+            r.load((const T *)a.x + (size_t)p.b * a.xb + (size_t)n * a.xn, col, a.C);
         }
+    }
+    __device__ __forceinline__ void get(const GGCol<T> &col, float (&v)[GGRowT<T>::V])
+    {
+        if constexpr (!Q8) r.align(col);
+        r.get(v);
     }
 };
 
-// g = dy act'(t) of one value of channel c; stat: the cloud's statistics
-template <int ACT>
-__device__ __forceinline__ float gate(const Args &a, const Chan &k, float dy, float d, float x, const double *stat, int c)
+// g = dy act'(t) of one value
+template <int ACT> __device__ __forceinline__ float gate(const Chan &k, float dy, float d, float x)
 {
     if constexpr (ACT == GRIDGCN_ACT_NONE) return dy;
-    const float t = fmaf(d, k.a, k.beta);
-    if constexpr (ACT == GRIDGCN_ACT_RELU) return positive(k, t, x, stat, a, c < a.C ? c : a.C - 1) ? dy : 0.f;
-    return dy * act_grad<ACT>(t);
+    if constexpr (ACT == GRIDGCN_ACT_RELU) return __uint_as_float(__float_as_uint(x) ^ k.flip) > k.thr ? dy : 0.f;
+    return dy * act_grad<ACT>(fmaf(d, k.a, k.beta));
 }
 
 // backward, first pass over r0 <= n < r1 (all below count): s = sums of g and g * d per channel
@@ -303,18 +347,18 @@ __device__ __forceinline__ void rows_bwd_sums(const Args &a, const Lay &l, const
 {
     constexpr int V = GGRowT<T>::V;
     const T *dy = (const T *)a.dy + (size_t)p.b * a.gb;
-    const double *stat = a.stats + (size_t)p.b * a.G * 2;
 #pragma unroll
     for (int i = 0; i < V; i++) s[i][0] = s[i][1] = 0.0;
     if (!p.on) return;
+    const GGCol<T> col(p.c, a.C);
     for (long long n0 = r0 + p.tr; n0 < r1; n0 += (long long)l.rpb * UNROLL) {
         GGChunk<T> re[UNROLL];
         Xhat<T, Q8> rx[UNROLL];
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) {
             const long long n = n0 + (long long)u * l.rpb, nn = n < r1 ? n : n0;
-            re[u].load(dy + (size_t)nn * a.gn, p.c, a.C);
-            rx[u].load(a, p, nn);
+            re[u].load(dy + (size_t)nn * a.gn, col, a.C);
+            rx[u].load(a, p, col, nn);
         }
         float s0[V], s1[V];
 #pragma unroll
@@ -323,12 +367,13 @@ __device__ __forceinline__ void rows_bwd_sums(const Args &a, const Lay &l, const
         for (int u = 0; u < UNROLL; u++) {
             if (n0 + (long long)u * l.rpb >= r1) continue;
             float e[V], v[V];
+            re[u].align(col);
             re[u].get(e);
-            rx[u].r.get(v);
+            rx[u].get(col, v);
 #pragma unroll
             for (int i = 0; i < V; i++) {
                 const float d = dev_of(k[i], v[i]);
-                const float g = gate<ACT>(a, k[i], e[i], d, v[i], stat, p.c + i);
+                const float g = gate<ACT>(k[i], e[i], d, v[i]);
                 s0[i] += g;
                 s1[i] = fmaf(g, d, s1[i]);
             }
@@ -349,8 +394,8 @@ __device__ __forceinline__ void rows_bwd_dx(const Args &a, const Lay &l, const P
     constexpr int V = GGRowT<T>::V;
     const T *dy = (const T *)a.dy + (size_t)p.b * a.gb;
     T *dx = (T *)a.y + (size_t)p.b * a.N * a.C;
-    const double *stat = a.stats + (size_t)p.b * a.G * 2;
     if (!p.on) return;
+    const GGCol<T> col(p.c, a.C);
     const long long rv = r1 < count ? r1 : count;          // rows with values
     long long n0 = r0 + p.tr;
     for (; n0 < rv; n0 += (long long)l.rpb * UNROLL) {
@@ -359,29 +404,30 @@ __device__ __forceinline__ void rows_bwd_dx(const Args &a, const Lay &l, const P
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) {
             const long long n = n0 + (long long)u * l.rpb, nn = n < rv ? n : n0;
-            re[u].load(dy + (size_t)nn * a.gn, p.c, a.C);
-            rx[u].load(a, p, nn);
+            re[u].load(dy + (size_t)nn * a.gn, col, a.C);
+            rx[u].load(a, p, col, nn);
         }
 #pragma unroll
         for (int u = 0; u < UNROLL; u++) {
             const long long n = n0 + (long long)u * l.rpb;
             if (n >= r1) continue;
             float e[V], v[V], o[V];
+            re[u].align(col);
             re[u].get(e);
-            rx[u].r.get(v);
+            rx[u].get(col, v);
 #pragma unroll
             for (int i = 0; i < V; i++) {
                 const float d = dev_of(k[i], v[i]);
-                const float g = gate<ACT>(a, k[i], e[i], d, v[i], stat, p.c + i);
+                const float g = gate<ACT>(k[i], e[i], d, v[i]);
                 o[i] = n < rv ? fmaf(k[i].a, g, -fmaf(d, f[i].y, f[i].x)) : 0.f;
             }
-            gg_st_chunk(dx + (size_t)n * a.C, p.c, a.C, o);
+            gg_st_chunk(dx + (size_t)n * a.C, p.c, a.C, o, a.past);
         }
     }
     float z[V];
 #pragma unroll
     for (int i = 0; i < V; i++) z[i] = 0.f;
-    for (; n0 < r1; n0 += l.rpb) gg_st_chunk(dx + (size_t)n0 * a.C, p.c, a.C, z);
+    for (; n0 < r1; n0 += l.rpb) gg_st_chunk(dx + (size_t)n0 * a.C, p.c, a.C, z, a.past);
 }
 
 // ---- many rows: pass, small launch, pass ----------------------------------------------------------------------------
@@ -412,10 +458,18 @@ template <class F> __device__ __forceinline__ void sum_chunks(const Args &a, int
     for (int o = 0; o < n; o += cw) {
         double s0 = 0.0, s1 = 0.0;
         if (kl < nl && o + cl < n) {
-            const double *p = a.part + ((size_t)b * a.chunks * a.C + c0 + o + cl) * 2;
-            for (int k = kl; k < a.chunks; k += nl) {
-                s0 += p[(size_t)k * a.C * 2];
-                s1 += p[(size_t)k * a.C * 2 + 1];
+            const f64x2 *p = (const f64x2 *)a.part + (size_t)b * a.chunks * a.C + c0 + o + cl;
+            constexpr int U = 8;           // (loads in flight: with one at a time a group of 131 channels took 66 us, not 7)
+            for (int k = kl; k < a.chunks; k += nl * U) {
+                f64x2 v[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) v[u] = p[(size_t)(k + u * nl < a.chunks ? k + u * nl : k) * a.C];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    if (k + u * nl >= a.chunks) continue;
+                    s0 += v[u].x;
+                    s1 += v[u].y;
+                }
             }
         }
         red[threadIdx.x * 2] = s0;
@@ -502,12 +556,12 @@ __global__ __launch_bounds__(THREADS) void gg_k_gn_apply(Args a, Lay l)
     const long long r0 = (long long)(gridDim.x - 1 - blockIdx.x) * a.rpc;
     const long long r1 = r0 + a.rpc < a.N ? r0 + a.rpc : a.N;
     Chan k[V];
-    chans<V>(a, p, k);
+    chans<ACT, false, V>(a, p, k);
     rows_apply<T, ACT>(a, l, p, r0, r1, count_of(a, p.b), k);
 }
 
 template <class T, int ACT, bool Q8>
-__global__ __launch_bounds__(THREADS, 4) void gg_k_gn_bwd_sums(Args a, Lay l)
+__global__ __launch_bounds__(THREADS, sizeof(T) == 4 ? 4 : 3) void gg_k_gn_bwd_sums(Args a, Lay l)
 {
     constexpr int V = GGRowT<T>::V;
     __shared__ double red[THREADS * V * 2];
@@ -516,7 +570,7 @@ __global__ __launch_bounds__(THREADS, 4) void gg_k_gn_bwd_sums(Args a, Lay l)
     const long long r0 = (long long)blockIdx.x * a.rpc;
     const long long r1 = r0 + a.rpc < count ? r0 + a.rpc : count;
     Chan k[V];
-    chans<V>(a, p, k);
+    chans<ACT, true, V>(a, p, k);
     double s[V][2];
     rows_bwd_sums<T, ACT, Q8>(a, l, p, r0, r1, k, s);
     reduce_rows<V, THREADS>(red, l, p.tr, (int)threadIdx.x % l.tpr, s);
@@ -553,33 +607,50 @@ __global__ __launch_bounds__(THREADS) void gg_k_gn_bwd_fin(Args a)
     if (threadIdx.x == 0) a.coef[(size_t)b * a.G + g] = coef_of(a, b, g, s, q);
 }
 
-// dgamma, dbeta of a channel: the clouds' totals in order
-__device__ __forceinline__ void params_of(const Args &a, int c)
+// dgamma, dbeta of the channels c0 <= c < c1 (at most PAR of them): the clouds' totals, PARL lanes' strided sums, then the lanes.
+// red: LDS [THREADS * 2]; every thread calls.
+constexpr int PAR = 16, PARL = THREADS / PAR;
+__device__ __forceinline__ void params_of(const Args &a, int c0, int c1, double *red)
 {
+    const int c = c0 + (int)threadIdx.x % PAR, k0 = (int)threadIdx.x / PAR;
     double db = 0.0, dg = 0.0;
-    for (int b = 0; b < a.B; b++) {
-        const double *t = a.tot + ((size_t)b * a.C + c) * 2;
-        db += t[0];
-        dg += t[1];
+    if (c < c1) {
+        for (int b = k0; b < a.B; b += PARL) {
+            const double *t = a.tot + ((size_t)b * a.C + c) * 2;
+            db += t[0];
+            dg += t[1];
+        }
     }
-    if (a.dbeta) gg_st_param(a.dbeta, a.ptype, c, (float)db);
-    if (a.dgamma) gg_st_param(a.dgamma, a.ptype, c, (float)dg);
+    red[threadIdx.x * 2] = db;
+    red[threadIdx.x * 2 + 1] = dg;
+    __syncthreads();
+    if (k0 == 0 && c < c1) {
+        for (int k = 1; k < PARL; k++) {
+            db += red[(threadIdx.x + k * PAR) * 2];
+            dg += red[(threadIdx.x + k * PAR) * 2 + 1];
+        }
+        if (a.dbeta) gg_st_param(a.dbeta, a.ptype, c, (float)db);
+        if (a.dgamma) gg_st_param(a.dgamma, a.ptype, c, (float)dg);
+    }
+    __syncthreads();
 }
 
 template <class T, int ACT, bool Q8>
 __global__ __launch_bounds__(THREADS, 4) void gg_k_gn_bwd_dx(Args a, Lay l)
 {
     constexpr int V = GGRowT<T>::V;
-    if (blockIdx.x == 0 && blockIdx.z == 0) {
-        const int c0 = blockIdx.y * l.tpr * V, c1 = c0 + l.tpr * V < a.C ? c0 + l.tpr * V : a.C;
-        for (int c = c0 + threadIdx.x; c < c1; c += THREADS) params_of(a, c);
+    // (the workgroups take some channels' parameters along)
+    __shared__ double red[THREADS * 2];
+    if (a.dgamma || a.dbeta) {
+        const long long nth = ((long long)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
+        const long long all = (long long)gridDim.z * gridDim.y * gridDim.x;
+        for (long long c = nth * PAR; c < a.C; c += all * PAR) params_of(a, (int)c, c + PAR < a.C ? (int)c + PAR : a.C, red);
     }
-    if (!a.y) return;
     const Pos<V> p(l, blockIdx.y * l.tpr, a.B - 1 - (int)blockIdx.z);
     const long long r0 = (long long)(gridDim.x - 1 - blockIdx.x) * a.rpc;
     const long long r1 = r0 + a.rpc < a.N ? r0 + a.rpc : a.N;
     Chan k[V];
-    chans<V>(a, p, k);
+    chans<ACT, true, V>(a, p, k);
     float2 f[V];
 #pragma unroll
     for (int i = 0; i < V; i++) {
@@ -591,8 +662,9 @@ __global__ __launch_bounds__(THREADS, 4) void gg_k_gn_bwd_dx(Args a, Lay l)
 
 __global__ __launch_bounds__(THREADS) void gg_k_gn_params(Args a)
 {
-    const int c = blockIdx.x * THREADS + threadIdx.x;
-    if (c < a.C) params_of(a, c);
+    __shared__ double red[THREADS * 2];
+    const int c0 = blockIdx.x * PAR;
+    params_of(a, c0, c0 + PAR < a.C ? c0 + PAR : a.C, red);
 }
 
 // ---- few rows: one launch, a workgroup = whole groups of one cloud (l.nq chunks from channel slab * slab_c on), every value read
@@ -607,20 +679,18 @@ __global__ __launch_bounds__(FEW) void gg_k_gn_small(Args a, Lay l, int slab_c)
     p.on = p.tr < l.rpb && p.c < (SAVE8 && c1 == a.C ? gg_a8_cp(a.C) : c1);
     const long long count = count_of(a, p.b);
     const T *x = (const T *)a.x + (size_t)p.b * a.xb;
+    const GGCol<T> col(p.on ? p.c : 0, a.C);
     GGChunk<T> r[K];
 #pragma unroll
     for (int u = 0; u < K; u++) {
+        if ((long long)u * l.rpb >= a.N) continue;
         const long long n = (long long)u * l.rpb + p.tr;
-        if (p.on && n < count) r[u].load(x + (size_t)n * a.xn, p.c, a.C);
-        else r[u].zero();
+        r[u].load(x + (size_t)(n < count ? n : 0) * a.xn, col, a.C);               // (rows past the end: in no sum, not stored)
     }
     double s[V][2], base[V];
+    base_of<T>(a, p, x, base);
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-        s[i][0] = s[i][1] = 0.0;
-        const int c = p.c + i < a.C ? p.c + i : a.C - 1;
-        base[i] = count > 0 ? (double)GGRowT<T>::get(x + (c / a.cg) * a.cg) : 0.0;
-    }
+    for (int i = 0; i < V; i++) s[i][0] = s[i][1] = 0.0;
     const int Cp = gg_a8_cp(a.C), nb = Cp / GG_A8_BLOCK;
 #pragma unroll
     for (int u = 0; u < K; u++) {
@@ -628,6 +698,7 @@ __global__ __launch_bounds__(FEW) void gg_k_gn_small(Args a, Lay l, int slab_c)
         const bool in = p.on && n < count;
         if ((long long)u * l.rpb >= a.N) continue;
         float v[V];
+        r[u].align(col);
         r[u].get(v);
         if (in) {
 #pragma unroll
@@ -671,7 +742,7 @@ __global__ __launch_bounds__(FEW) void gg_k_gn_small(Args a, Lay l, int slab_c)
     for (int i = 0; i < V; i++) {
         const int c = p.c + i < c1 ? p.c + i : c1 - 1;
         const double *st = red + ((c - c0) / a.cg) * a.cg * 2;
-        k[i] = chan_of(a, st[0], st[1], c);
+        k[i] = chan_of<ACT, false>(a, st[0], st[1], c);
     }
     T *y = (T *)a.y + (size_t)p.b * a.N * a.C;
 #pragma unroll
@@ -682,7 +753,7 @@ __global__ __launch_bounds__(FEW) void gg_k_gn_small(Args a, Lay l, int slab_c)
         r[u].get(v);
 #pragma unroll
         for (int i = 0; i < V; i++) o[i] = n < count ? act_of<ACT>(fmaf(dev_of(k[i], v[i]), k[i].a, k[i].beta)) : 0.f;
-        gg_st_chunk(y + (size_t)n * a.C, p.c, a.C, o);
+        gg_st_chunk(y + (size_t)n * a.C, p.c, a.C, o, false);
     }
 }
 
@@ -697,24 +768,20 @@ __global__ __launch_bounds__(FEW) void gg_k_gn_small_bwd(Args a, Lay l, int slab
     const long long count = count_of(a, p.b);
     const T *dy = (const T *)a.dy + (size_t)p.b * a.gb;
     const double *stat = a.stats + (size_t)p.b * a.G * 2;
-    const int Cp = gg_a8_cp(a.C), nb = Cp / GG_A8_BLOCK;
+    Pos<V> at = p;
+    if (!p.on) at.c = c0;
+    const GGCol<T> col(at.c, a.C);
     GGChunk<T> rg[K];
-    typename std::conditional<Q8, GGCodes<V>, GGChunk<T>>::type rx[K];
+    Xhat<T, Q8> rx[K];
 #pragma unroll
     for (int u = 0; u < K; u++) {
-        const long long n = (long long)u * l.rpb + p.tr;
-        if (p.on && n < count) {
-            rg[u].load(dy + (size_t)n * a.gn, p.c, a.C);
-            const size_t row = (size_t)p.b * a.N + n;
-            if constexpr (Q8) rx[u].load(a.codes + row * Cp + p.c, a.scales + row * nb + p.c / GG_A8_BLOCK);
-            else rx[u].load((const T *)a.x + (size_t)p.b * a.xb + (size_t)n * a.xn, p.c, a.C);
-        } else {
-            rg[u].zero();
-            rx[u].zero();
-        }
+        if ((long long)u * l.rpb >= a.N) continue;
+        const long long n = (long long)u * l.rpb + p.tr, nn = n < count ? n : 0;    // (rows past the end: in no sum, not stored)
+        rg[u].load(dy + (size_t)nn * a.gn, col, a.C);
+        rx[u].load(a, at, col, nn);
     }
     Chan k[V];
-    chans<V>(a, p, k);
+    chans<ACT, true, V>(a, p, k);
     double s[V][2];
 #pragma unroll
     for (int i = 0; i < V; i++) s[i][0] = s[i][1] = 0.0;
@@ -722,12 +789,13 @@ __global__ __launch_bounds__(FEW) void gg_k_gn_small_bwd(Args a, Lay l, int slab
     for (int u = 0; u < K; u++) {
         if (!(p.on && (long long)u * l.rpb + p.tr < count)) continue;
         float e[V], v[V];
+        rg[u].align(col);
         rg[u].get(e);
-        rx[u].get(v);
+        rx[u].get(col, v);
 #pragma unroll
         for (int i = 0; i < V; i++) {
             const float d = dev_of(k[i], v[i]);
-            const float g = gate<ACT>(a, k[i], e[i], d, v[i], stat, p.c + i);
+            const float g = gate<ACT>(k[i], e[i], d, v[i]);
             s[i][0] += (double)g;
             s[i][1] = fma((double)g, (double)d, s[i][1]);
         }
@@ -772,14 +840,14 @@ __global__ __launch_bounds__(FEW) void gg_k_gn_small_bwd(Args a, Lay l, int slab
         if (n >= a.N) continue;
         float e[V], v[V], o[V];
         rg[u].get(e);
-        rx[u].get(v);
+        rx[u].r.get(v);
 #pragma unroll
         for (int i = 0; i < V; i++) {
             const float d = dev_of(k[i], v[i]);
-            const float g = gate<ACT>(a, k[i], e[i], d, v[i], stat, p.c + i);
+            const float g = gate<ACT>(k[i], e[i], d, v[i]);
             o[i] = n < count ? fmaf(k[i].a, g, -fmaf(d, f[i].y, f[i].x)) : 0.f;
         }
-        gg_st_chunk(dx + (size_t)n * a.C, p.c, a.C, o);
+        gg_st_chunk(dx + (size_t)n * a.C, p.c, a.C, o, false);
     }
 }
 
@@ -865,14 +933,14 @@ template <class T, int ACT, bool Q8> void launch_bwd(Args &a, const Plan &p, hip
 {
     if (p.small) {
         gg_k_gn_small_bwd<T, ACT, Q8><<<dim3(p.slabs, a.B), FEW, 0, st>>>(a, p.l, p.slab_c);
-        if (a.B > 1 && (a.dgamma || a.dbeta)) gg_k_gn_params<<<dim3((a.C + THREADS - 1) / THREADS), THREADS, 0, st>>>(a);
+        if (a.B > 1 && (a.dgamma || a.dbeta)) gg_k_gn_params<<<dim3((a.C + PAR - 1) / PAR), THREADS, 0, st>>>(a);
         return;
     }
     const unsigned slabs = (p.l.nq + p.l.tpr - 1) / p.l.tpr;
     gg_k_gn_bwd_sums<T, ACT, Q8><<<dim3(p.chunks, slabs, a.B), THREADS, 0, st>>>(a, p.l);
     gg_k_gn_bwd_fin<<<dim3(a.G, a.B), THREADS, 0, st>>>(a);
-    const unsigned gx = a.y ? (unsigned)p.chunks : 1u, gz = a.y ? (unsigned)a.B : 1u;
-    gg_k_gn_bwd_dx<T, ACT, Q8><<<dim3(gx, slabs, gz), THREADS, 0, st>>>(a, p.l);
+    if (a.y) gg_k_gn_bwd_dx<T, ACT, Q8><<<dim3(p.chunks, slabs, a.B), THREADS, 0, st>>>(a, p.l);
+    else gg_k_gn_params<<<dim3((a.C + PAR - 1) / PAR), THREADS, 0, st>>>(a);
 }
 
 template <class T, bool Q> void fwd_act(Args &a, const Plan &p, int act, hipStream_t st)
@@ -922,7 +990,7 @@ int gridgcn_group_norm_act_fwd(const void *x, int dtype, int B, long long N, int
     a.gamma = gamma; a.beta = beta; a.counts = counts; a.eps = eps; a.codes_out = codes; a.scales_out = scales;
     a.part = (double *)((char *)ws + p.off_part);
     a.stats = stats || p.small ? stats : (double *)((char *)ws + p.off_stats);
-    a.rpc = p.rpc; a.chunks = p.chunks;
+    a.rpc = p.rpc; a.chunks = p.chunks; a.past = gg_past_caches(B * N, C, dtype);
     const hipStream_t st = (hipStream_t)stream;
     const int rc = with_type(dtype, [&](auto *t) {
         typedef typename std::remove_pointer<decltype(t)>::type T;
@@ -952,7 +1020,7 @@ int gridgcn_group_norm_act_bwd(const void *dy, long long ldgb, long long ldgn, c
     a.part = (double *)((char *)ws + p.off_part);
     a.tot = (double *)((char *)ws + p.off_tot);
     a.coef = (float2 *)((char *)ws + p.off_coef);
-    a.rpc = p.rpc; a.chunks = p.chunks;
+    a.rpc = p.rpc; a.chunks = p.chunks; a.past = gg_past_caches(B * N, C, dtype);
     const hipStream_t st = (hipStream_t)stream;
     const int rc = with_type(dtype, [&](auto *t) {
         typedef typename std::remove_pointer<decltype(t)>::type T;

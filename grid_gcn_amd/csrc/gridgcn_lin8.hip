@@ -112,7 +112,11 @@ template <class T> struct Block {
         for (int i = 0; i < 4; i++) {
             GGChunk<T> c;
             c.zero();
-            if (k0 + i * VW < K) c.load(row, k0 + i * VW, K);
+            if (k0 + i * VW < K) {
+                const GGCol<T> col(k0 + i * VW, K);
+                c.load(row, col, K);
+                c.align(col);
+            }
             w[i] = c.w;
         }
     }
@@ -235,18 +239,30 @@ struct Mm {
     int K, N;
     unsigned ncol;             // column blocks
     unsigned nrow;             // row blocks
+    bool past;                 // many rows: y around the caches
+    bool spread;               // place()
 };
 
 // Workgroup -> (row block, column block): workgroups of consecutive numbers go to different XCDs; the column blocks of one row
-// block read the same rows, so they get numbers that are 8 apart and share an L2.
+// block read the same rows, so they get numbers that are 8 apart and share an L2.  With fewer than 64 row blocks, not a multiple
+// of 8, that would leave XCDs short of work (one row block: seven of eight idle): then one after the other.
 __device__ __forceinline__ bool place(const Mm &p, unsigned &row, unsigned &col)
 {
     const unsigned id = blockIdx.x, xcd = id & 7, slot = id >> 3;
-    col = slot % p.ncol;
-    row = (slot / p.ncol) * 8 + xcd;
+    if (p.spread) {
+        col = id % p.ncol;
+        row = id / p.ncol;
+    } else {
+        col = slot % p.ncol;
+        row = (slot / p.ncol) * 8 + xcd;
+    }
     return row < p.nrow;
 }
-unsigned place_grid(unsigned nrow, unsigned ncol) { return (nrow + 7) / 8 * 8 * ncol; }
+unsigned place_grid(Mm &p)
+{
+    p.spread = p.nrow < 64 && p.nrow % 8 != 0;
+    return (p.spread ? p.nrow : (p.nrow + 7) / 8 * 8) * p.ncol;
+}
 
 // ---- W in operand order, for many rows: [column block][step][tile of 32 columns][s][piece][lane], 16 bytes each; zeros behind K and N.
 // Tile nt of a column block holds its columns NT * j + nt: a lane's NT results of a row are then neighbours in memory.
@@ -326,16 +342,16 @@ template <class T, bool TRANS> __global__ __launch_bounds__(PT) void gg_k_lin8_p
 }
 
 // y of one row for M neighbouring columns
-template <class T, int M> __device__ __forceinline__ void put_row(T *y, long long row, int n, int N, const float (&v)[M])
+template <class T, int M> __device__ __forceinline__ void put_row(T *y, long long row, int n, int N, const float (&v)[M], bool past = false)
 {
     T *q = y + (size_t)row * N + n;
     if (M == 4 && n + 4 <= N) {
         if constexpr (sizeof(T) == 4) {
-            *(gg_u32x4_a4 *)q = gg_u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+            gg_st(q, gg_u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])}, past);
         } else if constexpr (std::is_same<T, gg_bf16>::value) {
-            *(gg_u32x2_a2 *)q = gg_u32x2{gg_cvt_bf16(v[0], v[1]), gg_cvt_bf16(v[2], v[3])};
+            gg_st(q, gg_u32x2{gg_cvt_bf16(v[0], v[1]), gg_cvt_bf16(v[2], v[3])}, past);
         } else {
-            *(gg_u32x2_a2 *)q = gg_u32x2{gg_cvt_f16(v[0], v[1]), gg_cvt_f16(v[2], v[3])};
+            gg_st(q, gg_u32x2{gg_cvt_f16(v[0], v[1]), gg_cvt_f16(v[2], v[3])}, past);
         }
     } else {
 #pragma unroll
@@ -484,7 +500,7 @@ __global__ __launch_bounds__(MW * 64, 3) void gg_k_lin8(Mm p)
         float v[NT];
 #pragma unroll
         for (int t = 0; t < NT; t++) v[t] = (P == 2 ? ldexpf(acc[t][i], rb + cb[t]) : acc[t][i]) + b[t];
-        put_row<T, NT>((T *)p.y, o, n, p.N, v);
+        put_row<T, NT>((T *)p.y, o, n, p.N, v, p.past);
     }
 }
 
@@ -576,7 +592,7 @@ struct Wg {
     float *part, *dbpart;         // splits > 1: [split][tile][128][128], [split][tiles_n * 128]
     long long R, ldy;
     int N, K, Cp;
-    unsigned tn, tk, splits;
+    unsigned tn, tk, splits, share;
 };
 
 template <class T> struct Strip {
@@ -686,10 +702,10 @@ __global__ __launch_bounds__(GW * 64, 1) void gg_k_lin8_wgrad(Wg p)
     constexpr int P = Ty<T>::P;
     constexpr int D = 3;                                            // strips in registers, one of them in use
     extern __shared__ __attribute__((aligned(16))) float ldsf[];    // [GW][4][16][64]
-    // (the tiles of one split read the same rows: same XCD, as in place())
-    const unsigned tiles = p.tn * p.tk, id = blockIdx.x, xcd = id & 7, slot = id >> 3;
-    const unsigned tile = slot % tiles, split = (slot / tiles) * 8 + xcd;
-    if (split >= p.splits) return;
+    // (the tiles of one split read the same rows: one XCD, or `share` of them)
+    const unsigned tiles = p.tn * p.tk, per = (tiles + p.share - 1) / p.share, id = blockIdx.x, slot = id >> 3;
+    const unsigned unit = (slot / per) * 8 + (id & 7), split = unit / p.share, tile = (unit % p.share) * per + slot % per;
+    if (split >= p.splits || tile >= tiles) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), h = lane >> 5, j = lane & 31;
     const int n0 = (int)(tile / p.tk) * GT, k0 = (int)(tile % p.tk) * GT, n = n0 + 4 * j, k = k0 + 4 * j;
     const bool first = tile % p.tk == 0 && p.db;
@@ -853,7 +869,7 @@ template <class T, bool TRANS, bool SAVE> void launch_mm(Mm &p, void *ws, hipStr
     if (!many(p.R, p.N)) {
         p.nrow = (unsigned)((p.R + 31) / 32);
         p.ncol = (unsigned)((p.N + 31) / 32);
-        gg_k_lin8_few<T, TRANS, SAVE><<<place_grid(p.nrow, p.ncol), SW * 64, 0, st>>>(p);
+        gg_k_lin8_few<T, TRANS, SAVE><<<place_grid(p), SW * 64, 0, st>>>(p);
         return;
     }
     p.nrow = (unsigned)((p.R + MW * 32 - 1) / (MW * 32));
@@ -865,16 +881,26 @@ template <class T, bool TRANS, bool SAVE> void launch_mm(Mm &p, void *ws, hipStr
     gg_k_lin8_pack<T, TRANS><<<p.ncol * NT, PT, 0, st>>>(k);
     p.wp = k.wp;
     p.wbyte = k.wbyte;
-    gg_k_lin8<T, SAVE><<<place_grid(p.nrow, p.ncol), MW * 64, 0, st>>>(p);
+    p.past = gg_past_caches(p.R, p.N, GGRowT<T>::id);
+    gg_k_lin8<T, SAVE><<<place_grid(p), MW * 64, 0, st>>>(p);
 }
 
+// Splits of the rows for dW: a multiple of 8 (an XCD each), or 1, 2, 4 of which 8, 4, 2 XCDs share the tiles.  A CU holds one workgroup,
+// an XCD 32: the fewest splits with the least time in (generations) x (strips of a wave + 6 for summing up), at least four strips
+// and at most two generations.  Measured, float32 dW: rows 32768, K = N = 1024 (64 tiles): 4 splits on four XCDs 363 us,
+// 8 splits 207;   rows 262144, K = 256, N = 128 (2 tiles): 64 splits 97, 128 splits 66, 256 splits 73.
 unsigned splits_of(long long R, unsigned tiles)
 {
-    // one generation of workgroups (one per CU: they use all its registers), at least four strips for each wave
-    long long s = 256 / tiles;
-    const long long most = (R + 16 * GW * 4 - 1) / (16 * GW * 4);
-    if (s > most) s = most;
-    return (unsigned)(s < 1 ? 1 : s);
+    const long long most = (R + 16 * GW * 4 - 1) / (16 * GW * 4), strips = R / (16 * GW);
+    unsigned best = 1;
+    long long least = -1;
+    for (unsigned s = 1; s <= 256 && s <= most; s = s < 8 ? s * 2 : s + 8) {
+        const long long load = s < 8 ? ((long long)tiles * s + 7) / 8 : (long long)(s / 8) * tiles, gens = (load + 31) / 32;
+        const long long time = gens * (strips / s + 6);
+        if (gens > 2 && s > 1) break;
+        if (least < 0 || time < least) { least = time; best = s; }
+    }
+    return best;
 }
 
 size_t wgrad_bytes(long long R, unsigned tn, unsigned tk)
@@ -893,7 +919,9 @@ template <class T> int launch_wgrad(Wg &p, hipStream_t st)
         done = true;
     }
     const unsigned tiles = p.tn * p.tk;
-    gg_k_lin8_wgrad<T><<<(p.splits + 7) / 8 * 8 * tiles, GW * 64, LDS, st>>>(p);
+    p.share = p.splits < 8 ? 8 / p.splits : 1;
+    const unsigned units = (p.splits * p.share + 7) / 8 * 8;
+    gg_k_lin8_wgrad<T><<<units * ((tiles + p.share - 1) / p.share), GW * 64, LDS, st>>>(p);
     if (p.splits > 1) {
         const unsigned nw = p.dw ? tiles * (GT * GT / 128) : 0, nd = p.db ? p.tn : 0;
         gg_k_lin8_wsum<T><<<nw + nd, 256, 0, st>>>(p, nw);
