@@ -854,8 +854,11 @@ __global__ __launch_bounds__(256) void gg_k_lin8_wsum(Wg p, unsigned nw)
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
-// Many rows where the larger workgroups fill at least half the CUs; below that, smaller ones, their waves on the contraction.
-bool many(long long R, int N) { return (R + MW * 32 - 1) / (MW * 32) * ((N + 32 * NT - 1) / (32 * NT)) >= 128; }
+// Many rows: more than one block of 128, and larger workgroups that fill at least half the CUs; below that smaller ones, their waves on
+// the contraction.  Measured (fp32 / bf16 forward, us; few | many):  8192 x 256 -> 128 (64 workgroups) 15 | 27 / 9 | 14;
+// 16384 (128) 27 | 27 / 17 | 15;  32768 50 | 29 / 31 | 17;  128 x 256 -> 16384 (one row block: W is laid out for it alone)
+// 21 | 36 / 14 | 19;  256 x 512 -> 8192 38 | 44 / 21 | 23.
+bool many(long long R, int N) { return R > MW * 32 && (R + MW * 32 - 1) / (MW * 32) * ((N + 32 * NT - 1) / (32 * NT)) >= 128; }
 size_t pack_bytes(long long R, int K, int N, int dtype)
 {
     if (!many(R, N)) return 0;

@@ -155,6 +155,36 @@ def test_group_norm_relu_gate_at_the_border():
     ref.check(dx, want["dx"], want["dx_tol"])
 
 
+def run_gate_of_any_gain(dtype, N, save8, dev="cpu"):
+    """gains of either sign, none, tiny and huge; shifts that put the border among the values, at them, and beyond them"""
+    C = 32
+    x = cases.rows((2, N), C, dtype, 12)
+    dy = cases.rows((2, N), C, dtype, 13, kind="grad")
+    w = torch.tensor([1.0, -1.0, 0.0, 0.0, 1e-30, -1e-30, 1e30, -1e30] * 4)
+    b = torch.tensor([0.3, 0.3, 0.5, -0.5, 1e-30, 1e-30, 0.0, 0.0] * 2 + [0.0] * 8 + [1e30, 1e30, 0.0, 1e-40, 1.0, -1.0, 1e30, -1e30])
+    want = ref.group_norm_act(x, w, b, 4, 1e-5, "relu", None, dy, save8)
+    t = [v.to(dev).requires_grad_() for v in (x, w, b)]
+    dx, dw, db = torch.autograd.grad(ops.group_norm_act(*t, 4, act="relu", save8=save8), t, dy.to(dev))
+    ref.check(db, want["db"], want["db_tol"], "db")
+    ref.check(dw, want["dw"], want["dw_tol"], "dw")
+    # what lies past the type's largest number by more than its bound and a step is infinite in it (float16 and a gain of 1e30)
+    lim = torch.finfo(dtype).max * (1 + torch.finfo(dtype).eps)
+    past = want["dx"].abs() - want["dx_tol"] > lim
+    got = dx.detach().cpu()
+    assert torch.equal(got[past].double(), want["dx"][past].sign() * float("inf"))
+    # (and may be where only its bound reaches past that)
+    keep = ~past & ~(got.isinf() & (want["dx"].abs() + want["dx_tol"] > lim))
+    ref.check(got[keep], want["dx"][keep], (want["dx_tol"] + torch.zeros_like(want["dx"]))[keep], "dx")
+
+
+@pytest.mark.parametrize("save8", [False, True])
+@pytest.mark.parametrize("dtype", cases.DTYPES)
+@pytest.mark.parametrize("N", [40, 600])
+def test_group_norm_relu_gate_of_any_gain(N, dtype, save8):
+    with emu.emulated_gpu():
+        run_gate_of_any_gain(dtype, N, save8)
+
+
 @pytest.mark.parametrize("act", ["none", "silu", "gelu"])
 def test_group_norm_formula_against_differences(act):
     """the oracle's gradients are the derivatives of its forward"""

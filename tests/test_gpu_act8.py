@@ -110,6 +110,48 @@ def test_group_norm_relu_gate_at_the_border():
     ref.check(dx, want["dx"], want["dx_tol"])
 
 
+@pytest.mark.parametrize("save8", [False, True])
+@pytest.mark.parametrize("dtype", cases.DTYPES)
+@pytest.mark.parametrize("N", [40, 5000])
+def test_group_norm_relu_gate_of_any_gain(N, dtype, save8):
+    cpu.run_gate_of_any_gain(dtype, N, save8, DEV)
+
+
+@pytest.mark.parametrize("dtype", cases.DTYPES)
+@pytest.mark.parametrize("case", [
+    # few rows against many columns, and the other way round: row blocks, splits and tiles that are no multiple of 8
+    (1, 96, 20000, True, 0), (3, 9000, 40, False, 0), (130, 64, 17000, True, 0), (300, 72, 5000, False, 0), (700, 1100, 1000, True, 0),
+    (2100, 900, 260, True, 0), (1300, 2000, 1900, False, 0), (9000, 130, 260, True, 0)])
+def test_linear_act8_wide(case, dtype):
+    got, want = cpu.run_linear(case, dtype, DEV)
+    cpu.check_linear(got, want, case)
+
+
+@pytest.mark.parametrize("dtype", cases.DTYPES)
+def test_results_larger_than_the_caches(dtype):
+    """more than 192 MB of output: every value as in a call on a part of the rows"""
+    R, C = (220 << 20) // (4 if dtype == torch.float32 else 2) // 99, 99
+    x = cases.rows((4096,), C, dtype, 7).to(DEV).repeat(R // 4096 + 1, 1)[:R]
+    codes, scales = ops.act8_pack(x)
+    back, part = ops.act8_unpack(codes, scales, C, dtype), ops.act8_unpack(codes[:4096], scales[:4096], C, dtype)
+    assert torch.equal(back, part.repeat(R // 4096 + 1, 1)[:R])
+    w = (torch.randn(C, C, generator=torch.Generator().manual_seed(2)) * 0.1).to(dtype).to(DEV)
+    with torch.no_grad():
+        y = ops.linear_act8(x, w)
+        assert torch.equal(y, ops.linear_act8(x[:4096 * 8], w)[:4096].repeat(R // 4096 + 1, 1)[:R])
+    B = R // 4096
+    x3, dy = x[:B * 4096].view(B, 4096, C).requires_grad_(), y[:B * 4096].view(B, 4096, C)
+    z = ops.group_norm_act(x3, None, None, 3, act="silu")
+    xs = x3[:1].detach().requires_grad_()
+    zs = ops.group_norm_act(xs, None, None, 3, act="silu")
+    n = x.new_zeros(1).float()
+    for a, b in ((z, zs), (torch.autograd.grad(z, x3, dy)[0], torch.autograd.grad(zs, xs, dy[:1])[0])):
+        # (the partial sums of a cloud are cut by the number of clouds: last bits of the statistics in 64 bits, a rounding of the result)
+        far = (a.detach().float() - b.detach().float()).abs() - torch.finfo(dtype).eps * 2 * b.detach().float().abs()
+        n = torch.maximum(n, far.max())
+    assert float(n) < 1e-5
+
+
 def _step(x, w, g, b, dy, counts, save8=True):
     z = ops.linear_act8(x, w)
     y = ops.group_norm_act(z, g, b, 8, act="relu", counts=counts, save8=save8)
