@@ -242,7 +242,8 @@ class _GroupNormAct(torch.autograd.Function):
 
 def group_norm_act(x, weight, bias, groups, eps=1e-5, act="relu", counts=None, save8=False):
     """y = act(group_norm(x) * weight + bias) on channels-last x [B, ..., C]; C in `groups` groups of consecutive channels,
-    statistics per (sample, group) over all positions in between ([B, C]: over the group's channels alone).
+    statistics per (sample, group) over all positions in between ([B, C]: over the group's channels alone).  At most
+    65535 samples and 8192 channels.
 
     weight, bias: [C] or None, float32 or x's type.  act: 'none' | 'relu' | 'silu' | 'gelu'.
     counts: int32 [B] or [B, 1] with x [B, N, C]: rows n >= counts[b] (an index operator's unused centres) are in no
