@@ -193,9 +193,11 @@ def make_step(net, opt, sync, loss_fn, inputs, target, use_graph):
             net.seed_dev = None
             if (sync is None or sync.world == 1) and "--eager" not in sys.argv:
                 # a failed stream capture leaves the HIP context of this process unusable
-                # ("operation failed due to a previous error during capture"): start over, eager
+                # ("operation failed due to a previous error during capture"): start over, eager, in a child process (a
+                # process that has initialised the GPU must not replace itself)
+                import subprocess
                 sys.stderr.flush()
-                os.execv(sys.executable, [sys.executable] + sys.argv + ["--eager"])
+                sys.exit(subprocess.call([sys.executable] + sys.argv + ["--eager"]))
     return eager, "eager"
 
 
