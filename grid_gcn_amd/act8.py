@@ -343,8 +343,9 @@ def linear_act8(x, weight, bias=None):
     """y = x W^T + bias on x [..., K], weight [N, K], bias [N] (all of one type: float32, bfloat16 or float16), keeping for the
     backward the 8-bit form of x (act8_pack) instead of x: 1.03 bytes a value, written in the forward's pass over x.
 
-    Sums are in float32.  A float32 operand enters the matrix instructions as a sum of 16-bit numbers; the error of a product is that
-    of a float32 product, but an operand that is infinite or beyond 3.39e38 gives NaN.
+    Sums are in float32.  A float32 operand enters the matrix instructions as a sum of three bfloat16 numbers, whatever stands
+    beside it in its row and however many rows there are; the error of a product is that of a float32 product, but an operand that is
+    infinite or beyond 3.39e38 gives NaN, and what of an operand lies below 2^-134 is dropped.
     Backward: dx = dy W and dbias as ever; dW = dy^T x^ with x^ the 8-bit values of x.  Not differentiable twice."""
     K, N = _check_linear(x, weight, bias)
     if x.numel() == 0:

@@ -5,15 +5,14 @@
 //
 // Rows are many (one per point or edge), K and N a few hundred: with 16-bit rows all three products wait for memory, with
 // 32-bit rows they would wait for the fp32 matrix instruction (1/16 of the bf16 rate).  So a 32-bit operand enters as a sum of
-// 16-bit numbers, to nearest each, and a product as the partial products that are above float32's own rounding:
-//   * y and dx, many rows: x * 2^-e = hi + lo in fp16 (11 + 11 bits and the sign of lo: all of float32's 24 but the last half
-//     step), e of a row of x and of a column of W, taken out of the sums as a power of two at the end; three partial products,
-//     what is dropped (lo lo) is below 2^-24 of the product;
-//   * few rows, and dW, where no common scale can leave the sum: x = hi + mid + lo in bf16, exactly; six partial products (dropped:
-//     below 2^-26) -- three in dW, as a value of the 8-bit form is exact in bf16 as it is.
+// three bf16 numbers, x = hi + mid + lo, to nearest each: 8 + 8 + 8 bits, all of float32's 24 for any finite x up to 3.39e38,
+// whatever stands beside it in its row.  A product is the six partial products that are above float32's own rounding (what is
+// dropped, mid lo + lo mid + lo lo, is below 2^-24 of it) -- three in dW, as a value of the 8-bit form is exact in bf16 as it is.
+// (Two fp16 numbers and three partial products under one power of two per row and column: 272 us for the y below, and what lies 2^-33
+// under the largest value of its row was gone, against a weight of zero too.)
 //
-// 655360 rows, 256 -> 128, fp32: y and codes 236 us (1.18 GB: 5.0 TB/s), dx 236 (1.0 GB: 4.3), dW 141 (0.5 GB, three products: 914
-// TFLOP/s), W laid out 4 - 11, dW's partial sums 5.   262144 rows, 256 -> 512, bf16: y and codes 167 (0.47 GB, 412 TFLOP/s), dx 123,
+// 655360 rows, 256 -> 128, fp32, average (least) of ten: y and codes 342 us (279; 1.18 GB: 3.5 TB/s, six products: 755 TFLOP/s), dx 344
+// (295; 1.0 GB), dW 175 (137; 0.5 GB, three products: 736 TFLOP/s), W laid out 5 - 11, dW's partial sums 5.   262144 rows, 256 -> 512, bf16: y and codes 167 (0.47 GB, 412 TFLOP/s), dx 123,
 // dW 100 (688 TFLOP/s): bound by issue, as vector and matrix instructions of a SIMD take turns.   Few rows: 32, 512 -> 256, fp32: y 7, dx 5, dW 11.
 #include "../../include/gridgcn.h"
 #include "gridgcn_act8.h"
@@ -42,12 +41,6 @@ template <> struct Ty<float> {
     static __device__ __forceinline__ F16 mfma(gg_u32x4 a, gg_u32x4 b, F16 c) { return Ty<gg_bf16>::mfma(a, b, c); }
 };
 
-// the operands of y and dx at many rows: 32-bit rows as two fp16 numbers
-template <class T> struct Mt {
-    static constexpr int P = sizeof(T) == 4 ? 2 : 1;
-    typedef typename std::conditional<std::is_same<T, gg_bf16>::value, Ty<gg_bf16>, Ty<gg_f16>>::type M;
-};
-
 __device__ __forceinline__ F16 zero16()
 {
     F16 z;
@@ -72,13 +65,6 @@ __device__ __forceinline__ void split2(float a, float b, unsigned &h, unsigned &
     l = gg_cvt_bf16(a, b);
 }
 
-// two floats as two fp16 pairs (of magnitudes that fp16 holds)
-__device__ __forceinline__ void halve2(float a, float b, unsigned &h, unsigned &l)
-{
-    h = gg_cvt_f16(a, b);
-    l = gg_cvt_f16(a - gg_f16of(h, 0), b - gg_f16of(h, 1));
-}
-
 // acc[t] += A B[t] from the pieces of both, the smallest partial products first; neighbouring instructions on different tiles
 template <class M, int TN, int PA, int PB>
 __device__ __forceinline__ void mul(const gg_u32x4 (&a)[PA], const gg_u32x4 (&b)[TN][PB], F16 (&c)[TN])
@@ -88,7 +74,6 @@ __device__ __forceinline__ void mul(const gg_u32x4 (&a)[PA], const gg_u32x4 (&b)
         for (int t = 0; t < TN; t++) c[t] = M::mfma(a[i], b[t][j], c[t]);
     };
     if constexpr (PA == 3 && PB == 3) { one(2, 0); one(1, 1); one(0, 2); one(1, 0); one(0, 1); }
-    else if constexpr (PA == 2) { one(1, 0); one(0, 1); }
     else if constexpr (PA == 3) { one(2, 0); one(1, 0); }
     one(0, 0);
 }
@@ -143,16 +128,6 @@ template <class T> struct Block {
         if constexpr (sizeof(T) == 4) return __uint_as_float(w[i / 4][i % 4]);
         else if constexpr (std::is_same<T, gg_bf16>::value) return (i & 1) ? gg_hi16f(w[i / 8][(i % 8) / 2]) : gg_lo16f(w[i / 8][(i % 8) / 2]);
         else return gg_f16of(w[i / 8][(i % 8) / 2], i & 1);
-    }
-    // channels 8 s .. of 32-bit rows, times `by`, as two fp16 numbers
-    __device__ __forceinline__ void frag2(int s, float by, gg_u32x4 (&f)[2]) const
-    {
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            unsigned h, l;
-            halve2(get(8 * s + 2 * j) * by, get(8 * s + 2 * j + 1) * by, h, l);
-            f[0][j] = h; f[1][j] = l;
-        }
     }
     // Scale byte of the 8-bit form: 16-bit rows, the lane holds a block of 32; 32-bit rows, the two halves hold one together (every
     // lane of the wave calls).  clean: as gg_a8_block_byte
@@ -234,8 +209,7 @@ template <class T> struct Block {
 struct Mm {
     const void *a;             // [R][K] rows, stride lda
     const void *w;             // few rows: TRANS ? [K][N] : [N][K], contiguous
-    const char *wp;            // many rows: W in operand order (gg_k_lin8_pack), and its columns' scale bytes
-    const int *wbyte;
+    const char *wp;            // many rows: W in operand order (gg_k_lin8_pack)
     const void *bias;
     void *y;                   // [R][N] contiguous
     uint8_t *codes, *scales;
@@ -270,13 +244,12 @@ unsigned place_grid(Mm &p)
 
 // ---- W in operand order, for many rows: [column block][step][tile of 32 columns][s][piece][lane], 16 bytes each; zeros behind K and N.
 // Tile nt of a column block holds its columns NT * j + nt: a lane's NT results of a row are then neighbours in memory.
-// 32-bit: two fp16 numbers of W * 2^(127 - byte), byte of a column as in the 8-bit form.  A workgroup = 32 columns. -------------
+// 32-bit: its three pieces.  A workgroup = 32 columns. -----------------------------------------------------------------
 constexpr int NT = 4, PT = 512;
-template <class T> constexpr int STEP = NT * SS<T> * Mt<T>::P * 1024;          // bytes of a step: 16 KB either way
+template <class T> constexpr int STEP = NT * SS<T> * Ty<T>::P * 1024;          // bytes of a step: 24 KB (32-bit), 16 KB
 struct Pk {
     const void *w;
     char *wp;
-    int *wbyte;
     int K, N, steps;
 };
 // 8 consecutive k of column n, zeros outside W (loaded from inside and dropped: eight loads in flight instead of eight branches)
@@ -300,41 +273,21 @@ template <class T, bool TRANS> __device__ __forceinline__ void ld8(const T *w, i
 }
 template <class T, bool TRANS> __global__ __launch_bounds__(PT) void gg_k_lin8_pack(Pk p)
 {
-    constexpr int S = SS<T>, P = Mt<T>::P, L = PT / 32;            // L lanes share a column
-    __shared__ unsigned red[32][L + 1];
+    constexpr int S = SS<T>, P = Ty<T>::P, L = PT / 32;            // L lanes share a column
     const int c = TRANS ? (int)threadIdx.x & 31 : (int)threadIdx.x / L, kl = TRANS ? (int)threadIdx.x >> 5 : (int)threadIdx.x % L;
     const int n = blockIdx.x * 32 + c, groups = p.steps * (KS<T> / 8);
-    unsigned byte = 0;
-    if constexpr (P == 2) {
-        unsigned m = 0;
-        for (int g = kl; g < groups; g += L) {
-            gg_u32x4 u[2];
-            ld8<T, TRANS>((const T *)p.w, n, 8 * g, p.K, p.N, u);
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const unsigned a = u[e / 4][e % 4] & 0x7fffffffu;
-                m = m > a ? m : a;
-            }
-        }
-        red[c][kl] = m;
-        __syncthreads();
-        for (int i = 0; i < L; i++) m = m > red[c][i] ? m : red[c][i];
-        byte = gg_a8_byte(m);
-        if (kl == 0) p.wbyte[n] = (int)byte;
-    }
     const int nl = n % (32 * NT), nt = nl % NT, j = nl / NT;
     char *base = p.wp + (size_t)(n / (32 * NT)) * p.steps * STEP<T>;
     for (int g = kl; g < groups; g += L) {
         const int st = g / (KS<T> / 8), gi = g % (KS<T> / 8), h = gi / S, s = gi % S;
         gg_u32x4 u[sizeof(T) / 2], f[P];
         ld8<T, TRANS>((const T *)p.w, n, 8 * g, p.K, p.N, u);
-        if constexpr (P == 2) {
-            const float by = gg_a8_unscale(byte);
+        if constexpr (P == 3) {
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                unsigned hi, lo;
-                halve2(__uint_as_float(u[e / 2][2 * (e & 1)]) * by, __uint_as_float(u[e / 2][2 * (e & 1) + 1]) * by, hi, lo);
-                f[0][e] = hi; f[1][e] = lo;
+                unsigned hi, mid, lo;
+                split2(__uint_as_float(u[e / 2][2 * (e & 1)]), __uint_as_float(u[e / 2][2 * (e & 1) + 1]), hi, mid, lo);
+                f[0][e] = hi; f[1][e] = mid; f[2][e] = lo;
             }
         } else {
             f[0] = u[0];
@@ -367,16 +320,13 @@ template <class T, int M> __device__ __forceinline__ void put_row(T *y, long lon
 // ---- many rows: a wave owns 32 rows and 32 NT columns, its rows straight from memory into registers (each row is read by one wave
 // only), W through LDS (copied there without passing registers), the next step of both in flight while this one is multiplied;
 // three workgroups per CU, so that one's barriers and stores are another's matrix instructions.
-// 32-bit rows: a row's scale is that of its first 32 channels, and grows (the sums are scaled down) where a later block is
-// more than 2^3 larger, which fp16's range allows for; smaller blocks keep 33 bits below the largest value of the row.
 // The 8-bit form is held back until 128 bytes of a row are complete: stored as they come, 16 bytes of a line per step, lines left the
 // L2 half written and the kernel moved a third more bytes.  The column blocks of one row block take turns at it. ----------------
 constexpr int MW = 4;             // waves
-constexpr int HEADROOM = 3;
 template <class T, bool SAVE>
 __global__ __launch_bounds__(MW * 64, 3) void gg_k_lin8(Mm p)
 {
-    constexpr int P = Mt<T>::P, S = SS<T>, PC = Block<T>::CH / 16, GROUP = 128 / KS<T>;      // GROUP steps make 128 codes of a row
+    constexpr int P = Ty<T>::P, S = SS<T>, PC = Block<T>::CH / 16, GROUP = 128 / KS<T>;      // GROUP steps make 128 codes of a row
     __shared__ __attribute__((aligned(16))) char lds[2][STEP<T>];
     unsigned brow, bcol;
     if (!place(p, brow, bcol)) return;
@@ -389,7 +339,6 @@ __global__ __launch_bounds__(MW * 64, 3) void gg_k_lin8(Mm p)
     F16 acc[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) acc[t] = zero16();
-    int rbyte = 0;                // scale byte of the row (32-bit rows)
     gg_u32x4 held[4];             // codes of the group so far, the last ones behind
     unsigned heldb = 0;           // ... scale bytes likewise
 
@@ -404,26 +353,10 @@ __global__ __launch_bounds__(MW * 64, 3) void gg_k_lin8(Mm p)
         __syncthreads();
     };
     auto step = [&](Block<T> &b, int st) {
-        bool clean = true;
-        unsigned byte = 0;
         const bool mine = SAVE && (unsigned)(st / GROUP) % p.ncol == bcol;
-        if (P == 2 || mine) byte = b.byte(clean);
-        float by = 1.f;
-        if constexpr (P == 2) {
-            if (st == 0) rbyte = (int)byte;
-            if (__any((int)byte > rbyte + HEADROOM)) {
-                const int up = (int)byte > rbyte + HEADROOM ? (int)byte : rbyte, d = rbyte - up;
-                rbyte = up;
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const int di = __shfl(d, ggm_row(i, lane));
-#pragma unroll
-                    for (int t = 0; t < NT; t++) acc[t][i] = ldexpf(acc[t][i], di);
-                }
-            }
-            by = gg_a8_unscale((unsigned)rbyte);
-        }
         if (mine) {
+            bool clean;
+            const unsigned byte = b.byte(clean);
 #pragma unroll
             for (int i = 0; i < 4 - PC; i++) held[i] = held[i + PC];
 #pragma unroll
@@ -458,8 +391,7 @@ __global__ __launch_bounds__(MW * 64, 3) void gg_k_lin8(Mm p)
 #pragma unroll
         for (int s = 0; s < S; s++) {
             gg_u32x4 fa[P];
-            if constexpr (P == 2) b.frag2(s, by, fa);
-            else b.frag(s, fa);
+            b.frag(s, fa);
 #pragma unroll
             for (int t = 0; t < NT; t += 2) {                     // (two tiles at a time: independent neighbours, few registers)
                 gg_u32x4 fb[2][P];
@@ -468,7 +400,7 @@ __global__ __launch_bounds__(MW * 64, 3) void gg_k_lin8(Mm p)
 #pragma unroll
                     for (int q = 0; q < P; q++) fb[u][q] = *(const gg_u32x4 *)(cur + (((t + u) * S + s) * P + q) * 1024 + lane * 16);
                 F16(&two)[2] = *(F16(*)[2])&acc[t];
-                mul<typename Mt<T>::M>(fa, fb, two);
+                mul<Ty<T>>(fa, fb, two);
             }
         }
     };
@@ -490,20 +422,15 @@ __global__ __launch_bounds__(MW * 64, 3) void gg_k_lin8(Mm p)
     }
     const int n = ((int)bcol * 32 + j) * NT;
     float b[NT];
-    int cb[NT];
 #pragma unroll
-    for (int t = 0; t < NT; t++) {
-        b[t] = n + t < p.N ? gg_ld_param(p.bias, GGRowT<T>::id, n + t, 0.f) : 0.f;
-        cb[t] = P == 2 ? p.wbyte[n + t] - 254 : 0;
-    }
+    for (int t = 0; t < NT; t++) b[t] = n + t < p.N ? gg_ld_param(p.bias, GGRowT<T>::id, n + t, 0.f) : 0.f;
 #pragma unroll
     for (int i = 0; i < 16; i++) {
         const long long o = m0 + ggm_row(i, lane);
-        const int rb = P == 2 ? __shfl(rbyte, ggm_row(i, lane)) : 0;
         if (o >= p.R) continue;
         float v[NT];
 #pragma unroll
-        for (int t = 0; t < NT; t++) v[t] = (P == 2 ? ldexpf(acc[t][i], rb + cb[t]) : acc[t][i]) + b[t];
+        for (int t = 0; t < NT; t++) v[t] = acc[t][i] + b[t];
         put_row<T, NT>((T *)p.y, o, n, p.N, v, p.past);
     }
 }
@@ -859,16 +786,17 @@ __global__ __launch_bounds__(256) void gg_k_lin8_wsum(Wg p, unsigned nw)
 
 // ---- host side ------------------------------------------------------------------------------------------------------
 // Many rows: more than one block of 128, and larger workgroups that fill at least half the CUs; below that smaller ones, their waves on
-// the contraction.  Measured (fp32 / bf16 forward, us; few | many):  8192 x 256 -> 128 (64 workgroups) 15 | 27 / 9 | 14;
-// 16384 (128) 27 | 27 / 17 | 15;  32768 50 | 29 / 31 | 17;  128 x 256 -> 16384 (one row block: W is laid out for it alone)
-// 21 | 36 / 14 | 19;  256 x 512 -> 8192 38 | 44 / 21 | 23.
+// the contraction.  Measured (fp32 / bf16 forward, us; few | many):  8192 x 256 -> 128 (64 workgroups) 15 | 28 / 10 | 15;
+// 16384 (128) 27 | 30 / 16 | 15;  32768 50 | 32 / 30 | 17;  128 x 256 -> 16384 (one row block: W is laid out for it alone)
+// 23 | 37 / 15 | 19;  256 x 512 -> 8192 40 | 48 / 22 | 23.
 bool many(long long R, int N) { return R > MW * 32 && (R + MW * 32 - 1) / (MW * 32) * ((N + 32 * NT - 1) / (32 * NT)) >= 128; }
 size_t pack_bytes(long long R, int K, int N, int dtype)
 {
     if (!many(R, N)) return 0;
-    const int ks = dtype == GRIDGCN_F32 ? KS<float> : KS<gg_bf16>;
+    const bool f32 = dtype == GRIDGCN_F32;
+    const int ks = f32 ? KS<float> : KS<gg_bf16>;
     const size_t ncol = (N + 32 * NT - 1) / (32 * NT), steps = (K + ks - 1) / ks;
-    return ncol * (steps * STEP<float> + 32 * NT * sizeof(int));
+    return ncol * steps * (f32 ? STEP<float> : STEP<gg_bf16>);
 }
 
 template <class T, bool TRANS, bool SAVE> void launch_mm(Mm &p, void *ws, hipStream_t st)
@@ -884,10 +812,8 @@ template <class T, bool TRANS, bool SAVE> void launch_mm(Mm &p, void *ws, hipStr
     Pk k = {};
     k.w = p.w; k.wp = (char *)ws; k.K = p.K; k.N = p.N;
     k.steps = (p.K + KS<T> - 1) / KS<T>;
-    k.wbyte = (int *)(k.wp + (size_t)p.ncol * k.steps * STEP<T>);
     gg_k_lin8_pack<T, TRANS><<<p.ncol * NT, PT, 0, st>>>(k);
     p.wp = k.wp;
-    p.wbyte = k.wbyte;
     p.past = gg_past_caches(p.R, p.N, GGRowT<T>::id);
     gg_k_lin8<T, SAVE><<<place_grid(p), MW * 64, 0, st>>>(p);
 }

@@ -853,8 +853,8 @@ int gridgcn_gridconv_forward(const float *src, const int32_t *nebidx, const floa
  *   the three may be NULL.  Rows n >= counts[b]: dx = 0, dy not read.
  *
  * gridgcn_linear_act8_fwd: y[R][N] = x[R][K] W[N][K]^T + bias[N] (bias may be NULL), all of one type, products summed in
- *   fp32 (float32 operands as sums of 16-bit numbers: the error of an fp32 product; an infinite operand gives NaN),
- *   and codes / scales (both or neither) the 8-bit form of x.
+ *   fp32 (float32 operands as sums of three bf16 numbers: the error of an fp32 product; an infinite operand gives NaN,
+ *   what lies below 2^-134 of one is dropped), and codes / scales (both or neither) the 8-bit form of x.
  * gridgcn_linear_act8_bwd: dx[R][K] = dy W;  dW[N][K] = dy^T x^ with x^ the values of codes / scales;  dbias[N] = sum of
  *   dy; any of them may be NULL (codes, scales only for dW; W only for dx).
  * *_workspace_bytes may answer 0: ws may then be NULL (group norm: stats = whether the call passes stats, save8 =

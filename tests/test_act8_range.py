@@ -1,0 +1,102 @@
+"""CPU tier: values of extreme magnitude, and calls off the usual path, of the batch-independent training layer
+(grid_gcn_amd/act8.py).  The functions that tests/test_gpu_act8_range.py runs on an MI355X take the device as `dev`."""
+import os
+import sys
+
+import pytest
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, os.path.join(os.path.dirname(os.path.abspath(__file__)), "simt"))
+
+import act8_cases as cases  # noqa: E402
+import test_act8 as base  # noqa: E402
+from oracle import act8_ref as ref  # noqa: E402
+from simt import emu  # noqa: E402
+from grid_gcn_amd import ops  # noqa: E402
+
+
+# ---- float32 products: the bound is that of a float32 sum of |x| |w|, whatever the range of a row or a column -----------
+def wide(R):
+    """columns: enough workgroups for the kernel of many rows where R goes there"""
+    return 5600 if R > 128 else 40
+
+
+def run_wide_rows(R, dev="cpu"):
+    """a value of each row far above the others, against a weight of zero: what is left is the sum of the others"""
+    K, N = 64, wide(R)
+    x, w = cases.rows((R,), K, torch.float32, 3), cases.rows((N,), K, torch.float32, 4)
+    x[:, 0] = torch.exp2(torch.arange(R) % 100 - 20.0)
+    w[:, 0] = 0
+    dy = cases.rows((R,), N, torch.float32, 5, kind="grad")
+    dy[:, 7] = torch.exp2(torch.arange(R) % 100 - 20.0)
+    w[7] = 0
+    xd, wd = x.to(dev).requires_grad_(), w.to(dev)
+    y = ops.linear_act8(xd, wd)
+    dx, = torch.autograd.grad(y, xd, dy.to(dev))
+    want = ref.linear_act8(x, w, None, dy)
+    ref.check(y, want["y"], want["y_tol"], "y")
+    ref.check(dx, want["dx"], want["dx_tol"], "dx")
+    dy[:, 7] = 0
+    ref.check_norm(y, want["y"], K, "y")
+    ref.check_norm(dx, want["dx"], N, "dx")
+
+
+def run_every_scale(R, dev="cpu"):
+    """rows that grow by 2^40, fall off, start with zeros or lie far from 1; columns of three scales"""
+    x, w, dy = base.growing_rows(R, 72, 3), cases.rows((wide(R),), 72, torch.float32, 4), base.growing_rows(R, wide(R), 5)
+    w[::3] *= 2.0 ** 20
+    w[1::3] *= 2.0 ** -30
+    w[:, ::5] *= 2.0 ** -25
+    xd, wd = x.to(dev).requires_grad_(), w.to(dev)
+    y = ops.linear_act8(xd, wd)
+    dx, = torch.autograd.grad(y, xd, dy.to(dev))
+    want = ref.linear_act8(x, w, None, dy)
+    ref.check(y, want["y"], want["y_tol"], "y")
+    ref.check(dx, want["dx"], want["dx_tol"], "dx")
+
+
+@pytest.mark.parametrize("R", [100, 260])                 # the kernel of few rows, and that of many
+def test_linear_act8_wide_rows(R):
+    with emu.emulated_gpu():
+        run_wide_rows(R)
+
+
+@pytest.mark.parametrize("R", [100, 260])
+def test_linear_act8_rows_of_every_scale(R):
+    with emu.emulated_gpu():
+        run_every_scale(R)
+
+
+def run_tiny(R, dev="cpu"):
+    """values whose lower pieces are subnormal bf16 numbers, against weights that bring the products back: what lies below
+    2^-134 (half of the smallest bf16 number) of a value may be gone"""
+    x, w = cases.rows((R,), 72, torch.float32, 3), cases.rows((wide(R),), 72, torch.float32, 4)
+    x[0::3] *= 2.0 ** -112
+    x[1::3] *= 2.0 ** -121
+    w = w * 2.0 ** 100
+    with torch.no_grad():
+        y = ops.linear_act8(x.to(dev), w.to(dev))
+    want = ref.linear_act8(x, w, None)
+    ref.check(y, want["y"], want["y_tol"] + 2.0 ** -134 * w.double().abs().sum(1), "y")
+
+
+@pytest.mark.parametrize("R", [100, 260])
+def test_linear_act8_tiny_values(R):
+    with emu.emulated_gpu():
+        run_tiny(R)
+
+
+def run_same_row_in_any_company(dev="cpu"):
+    """a row's result does not tell how many rows the call had, beyond the rounding of its sum"""
+    x, w = base.growing_rows(260, 72, 3), cases.rows((5600,), 72, torch.float32, 4)
+    with torch.no_grad():
+        many = ops.linear_act8(x.to(dev), w.to(dev)).cpu()[:40].double()
+        few = ops.linear_act8(x[:40].to(dev), w.to(dev)).cpu().double()
+    tol = ref.linear_act8(x[:40], w, None)["y_tol"]
+    assert bool(((many - few).abs() <= 2 * tol).all())
+
+
+def test_linear_act8_same_row_in_any_company():
+    with emu.emulated_gpu():
+        run_same_row_in_any_company()

@@ -1,0 +1,32 @@
+"""MI355X tier of tests/test_act8_range.py: extreme magnitudes and calls off the usual path, on the kernels themselves."""
+import os
+import sys
+
+import pytest
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+
+import test_act8_range as cpu  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.mark.parametrize("R", [100, 260, 4000])
+def test_linear_act8_wide_rows(R):
+    cpu.run_wide_rows(R, DEV)
+
+
+@pytest.mark.parametrize("R", [100, 260])
+def test_linear_act8_rows_of_every_scale(R):
+    cpu.run_every_scale(R, DEV)
+
+
+@pytest.mark.parametrize("R", [100, 260])
+def test_linear_act8_tiny_values(R):
+    cpu.run_tiny(R, DEV)
+
+
+def test_linear_act8_same_row_in_any_company():
+    cpu.run_same_row_in_any_company(DEV)
