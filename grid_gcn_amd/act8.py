@@ -96,7 +96,8 @@ def _new_act8(rows, C, dev):
 def act8_pack(x):
     """x [..., C] -> (codes uint8 [..., Cp], scales uint8 [..., Cp / 32]), Cp = C rounded up to 32: 32 consecutive channels
     share the smallest power of two 2^(scale - 127) >= max |x| / 448 (scale >= 10), a channel is the nearest e4m3 number of
-    x / 2^(scale - 127); infinities and NaN become NaN (and a magnitude above 3.29e38 rounds to 2^128, infinite).  Off by at most 2^-4 of the value, or 2^-10 of 2^(scale - 127)."""
+    x / 2^(scale - 127); infinities and NaN become NaN (and a magnitude above 3.29e38 rounds to 2^128, infinite; a float16 one
+    of 63488 or more to 65536, infinite as a float16).  Off by at most 2^-4 of the value, or 2^-10 of 2^(scale - 127)."""
     _check_rows(x, "x")
     C = x.shape[-1]
     _require(1 <= C <= ACT8_MAX_C, "x must have 1..%d channels" % ACT8_MAX_C)
@@ -114,7 +115,7 @@ def act8_pack(x):
 @torch.no_grad()
 def act8_unpack(codes, scales, C, dtype=torch.float32):
     """The values [..., C] that (codes, scales) of act8_pack stand for (exact in float32 and bfloat16; in float16 if
-    they were packed from float16)."""
+    they were packed from float16, but for 65536: infinite)."""
     C = int(C)
     _require(1 <= C <= ACT8_MAX_C, "C must be 1..%d" % ACT8_MAX_C)
     _check_codes(codes, scales, None, C)

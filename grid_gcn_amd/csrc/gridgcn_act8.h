@@ -7,7 +7,7 @@
 //     value, or 2^-10 * 2^E where the value is below 2^-6 * 2^E);
 //   * a value has 4 significant bits and (E >= -117) is never a subnormal float32: it is EXACT in bf16, and in fp16 when x
 //     was fp16 (x is a multiple of 2^-24, and so is its rounding to 4 bits) -- so it enters a bf16 / fp16 matrix instruction
-//     without a second rounding;
+//     without a second rounding.  One exception: an fp16 magnitude of 63488 or more rounds to 65536, infinite as an fp16;
 //   * infinities and NaN become NaN and do not take part in the maximum; a magnitude above 3.29e38 rounds to 2^128, which
 //     is infinite as a float32.
 // Layout: codes [rows][Cp], Cp = C rounded up to 32 (the padding holds zeros: rows start on 32 bytes whatever C is),

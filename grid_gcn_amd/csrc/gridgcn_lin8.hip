@@ -609,17 +609,40 @@ template <class T> struct Strip {
             return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((int)c, scale, false));
         }
     }
-    // the four columns of x^ as operands
-    __device__ __forceinline__ void frag_x(gg_u32x4 (&f)[4][1], unsigned turn) const
+    // bits of 2^E: the lane's byte turned to the exponent's place
+    static __device__ __forceinline__ unsigned scale_bits(unsigned w, unsigned turn)
     {
-        // (2^E: the lane's byte turned to the exponent's place)
-        auto scale = [&](unsigned w) { return __uint_as_float((unsigned)__builtin_amdgcn_alignbit(w, w, turn) & 0x7f800000u); };
+        return (unsigned)__builtin_amdgcn_alignbit(w, w, turn) & 0x7f800000u;
+    }
+    // fp16 rows: a magnitude of 63488 or more has the 8-bit value 65536 (E = 8), which fp16 does not hold.  Blocks of such a scale enter
+    // as two halves of x^ (exact: no value of theirs is below 2^-1 but 0).  big: a scale of the strip may be one (the bits of all together)
+    static constexpr unsigned BIG = 135u << 23;
+    __device__ __forceinline__ bool big(unsigned turn) const
+    {
+        unsigned o = s[0];
+#pragma unroll
+        for (int i = 1; i < 8; i++) o |= s[i];
+        return scale_bits(o, turn) >= BIG;
+    }
+    // the four columns of x^ as operands; `halve`: of BIG blocks the half.  REST: their other half alone
+    template <bool REST> __device__ __forceinline__ void frag_x(gg_u32x4 (&f)[4][1], unsigned turn, bool halve) const
+    {
+        unsigned sc[8], cc[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            sc[i] = scale_bits(s[i], turn);
+            cc[i] = REST && sc[i] < BIG ? 0u : c[i];
+        }
+        if (halve) {
+#pragma unroll
+            for (int i = 0; i < 8; i++) sc[i] -= sc[i] >= BIG ? 1u << 23 : 0u;
+        }
 #pragma unroll
         for (int q = 0; q < 4; q++) {
-            const float su = scale(s[2 * q]), sv = scale(s[2 * q + 1]);
+            const float su = __uint_as_float(sc[2 * q]), sv = __uint_as_float(sc[2 * q + 1]);
 #pragma unroll
             for (int t = 0; t < 4; t += 2) {
-                const unsigned u = two(c[2 * q], su, t != 0), v = two(c[2 * q + 1], sv, t != 0);
+                const unsigned u = two(cc[2 * q], su, t != 0), v = two(cc[2 * q + 1], sv, t != 0);
                 f[t][0][q] = gg_pair16(u, v, 0);
                 f[t + 1][0][q] = gg_pair16(u, v, 1);
             }
@@ -663,15 +686,24 @@ __global__ __launch_bounds__(GW * 64, 1) void gg_k_lin8_wgrad(Wg p)
         s.load_full(p, (const char *)p.dy + e * 16 * p.ldy * sizeof(T), (const char *)p.codes + e * 16 * p.Cp,
                     (const char *)p.scales + e * 16 * (p.Cp / 32), od, oc, os);
     };
-    auto use = [&](const Strip<T> &s) {
-        gg_u32x4 fx[4][1];
-        s.frag_x(fx, turn);
+    auto add = [&](const Strip<T> &s, const gg_u32x4 (&fx)[4][1]) {
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             gg_u32x4 fd[P];
             s.frag_dy(i, fd);
             mul<Ty<T>>(fd, fx, acc[i]);
         }
+    };
+    bool halved = false;
+    auto use = [&](const Strip<T> &s) {
+        gg_u32x4 fx[4][1];
+        bool halve = false;
+        if constexpr (std::is_same<T, gg_f16>::value) {
+            halve = __any(s.big(turn));
+            halved |= halve;
+        }
+        s.template frag_x<false>(fx, turn, halve);
+        add(s, fx);
         if (first) {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -705,6 +737,23 @@ __global__ __launch_bounds__(GW * 64, 1) void gg_k_lin8_wgrad(Wg p)
         Strip<T> s;
         s.load_tail(p, g * 16 + 8 * h, n, k);
         use(s);
+    }
+    if (halved) {             // (fp16: the strips with BIG blocks once more; 262144 rows, 256 -> 512: 128 us, one in 1000 rows BIG 225)
+        for (g = (long long)split * GW + wave; g < strips; g += stride) {
+            unsigned top = 0;                                     // (the scales alone: such strips are few)
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const long long r = g * 16 + 8 * h + i;
+                const unsigned e = r < p.R && k < p.Cp ? p.scales[(size_t)r * (p.Cp / 32) + k / 32] : 0u;
+                top = top > e ? top : e;
+            }
+            if (!__any(top >= Strip<T>::BIG >> 23)) continue;
+            Strip<T> s;
+            s.load_tail(p, g * 16 + 8 * h, n, k);
+            gg_u32x4 fx[4][1];
+            s.template frag_x<true>(fx, turn, true);
+            add(s, fx);
+        }
     }
     // the waves' sums: a quarter of the tile's rows at a time
     float *pt = p.part ? p.part + ((size_t)split * tiles + tile) * GT * GT : nullptr;

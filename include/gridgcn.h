@@ -839,7 +839,8 @@ int gridgcn_gridconv_forward(const float *src, const int32_t *nebidx, const floa
  *   32 consecutive channels share the power of two 2^(scale - 127), the smallest with max |x| <= 448 * 2^(scale - 127)
  *   (finite values only; scale >= 10); a channel is the e4m3 number nearest to x / 2^(scale - 127), ties to even.
  *   Infinities and NaN become NaN.  A value is exact in bf16, and in fp16 if x was fp16; a magnitude above 3.29e38
- *   rounds to 2^128, which float32 and bf16 read as infinite.
+ *   rounds to 2^128, which float32 and bf16 read as infinite, and an fp16 one of 63488 or more to 65536, which fp16 reads
+ *   as infinite (gridgcn_linear_act8_bwd takes it as 65536).
  * gridgcn_act8_pack / _unpack: x[R][ldx] -> codes[R][Cp], scales[R][Cp / 32], and back.  codes 16-byte aligned.
  *
  * gridgcn_group_norm_act_fwd: x[B][N][C] (strides ldb, ldn), G groups of C / G channels; per (b, group) mean and

@@ -100,3 +100,45 @@ def run_same_row_in_any_company(dev="cpu"):
 def test_linear_act8_same_row_in_any_company():
     with emu.emulated_gpu():
         run_same_row_in_any_company()
+
+
+# ---- the top of float16: a magnitude of 63488 or more becomes 65536 in the 8-bit form -----------------------------------
+def run_float16_top(dev="cpu"):
+    """one large activation, alone in its column: dW is dy times its 8-bit value, a finite number"""
+    x = torch.zeros(40, 40, dtype=torch.float16)
+    x[3, 5] = 65000.0
+    dy = cases.rows((40,), 4, torch.float16, 8, kind="grad")
+    dy[3] = torch.tensor([2.0 ** -10, 0.0, 0.0, 0.0])
+    w = torch.zeros(4, 40, dtype=torch.float16, device=dev, requires_grad=True)
+    dw, = torch.autograd.grad(ops.linear_act8(x.to(dev), w), w, dy.to(dev))
+    want = torch.zeros(4, 40)
+    want[0, 5] = 64.0
+    assert torch.equal(dw.cpu().float(), want)
+
+
+def run_float16_magnitudes(dev="cpu"):
+    """rows of every magnitude that float16 has, next to one another: row n of dW is the 8-bit value of row n of x times a power of two"""
+    k = torch.arange(-24, 16)
+    x = torch.exp2(k.double())[:, None] * torch.cat([torch.linspace(-1.99, 1.99, 47, dtype=torch.float64), torch.ones(1, dtype=torch.float64)])
+    top = torch.finfo(torch.float16).max
+    x = torch.cat([x, x.flip(0), torch.linspace(-top, top, 48, dtype=torch.float64)[None], torch.full((1, 48), -top, dtype=torch.float64)])
+    x = x.clamp(-top, top).half()
+    R = x.shape[0]
+    gain = torch.where(x.float().abs().amax(1) > 1000, 2.0 ** -4, 1.0)
+    dy = torch.diag(gain).half()
+    w = torch.zeros(R, 48, dtype=torch.float16, device=dev, requires_grad=True)
+    dw, = torch.autograd.grad(ops.linear_act8(x.to(dev), w), w, dy.to(dev))
+    want = ref.act8(x)[0] * gain.double()[:, None]
+    assert float(want.abs().max()) == 4096.0
+    # (the value times the gain is within float16 but for what it has below 2^-24)
+    ref.check(dw, want, torch.zeros_like(want), "dw")
+
+
+def test_linear_act8_float16_top():
+    with emu.emulated_gpu():
+        run_float16_top()
+
+
+def test_linear_act8_float16_magnitudes():
+    with emu.emulated_gpu():
+        run_float16_magnitudes()

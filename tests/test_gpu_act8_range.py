@@ -30,3 +30,11 @@ def test_linear_act8_tiny_values(R):
 
 def test_linear_act8_same_row_in_any_company():
     cpu.run_same_row_in_any_company(DEV)
+
+
+def test_linear_act8_float16_top():
+    cpu.run_float16_top(DEV)
+
+
+def test_linear_act8_float16_magnitudes():
+    cpu.run_float16_magnitudes(DEV)
