@@ -142,3 +142,34 @@ def test_linear_act8_float16_top():
 def test_linear_act8_float16_magnitudes():
     with emu.emulated_gpu():
         run_float16_magnitudes()
+
+
+# ---- group normalisation: standard deviations far from 1 ---------------------------------------------------------------
+GN_SCALES = [(2.0 ** 77, 0.0), (2.0 ** 115, 1e-5), (2.0 ** -80, 0.0), (2.0 ** -100, 0.0)]
+
+
+def run_gn_scale(scale, eps, N, act, dtype, save8, dev="cpu", dy_scale=1.0):
+    C, G = 32, 4
+    x = (cases.rows((2, N), C, torch.float32, 21) * scale).to(dtype)
+    dy = (cases.rows((2, N), C, torch.float32, 22, kind="grad") * dy_scale).to(dtype)
+    w = torch.rand(C, generator=torch.Generator().manual_seed(3)) + 0.5
+    b = torch.randn(C, generator=torch.Generator().manual_seed(4)) * 0.3
+    want = ref.group_norm_act(x, w, b, G, eps, act, None, dy, save8)
+    t = [v.to(dev).requires_grad_() for v in (x, w, b)]
+    y = ops.group_norm_act(*t, G, eps=eps, act=act, save8=save8)
+    dx, dw, db = torch.autograd.grad(y, t, dy.to(dev))
+    base.check_gn(dict(y=y, dx=dx, dw=dw, db=db), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,act,save8", [(40, "relu", False), (40, "silu", True), (2300, "gelu", False), (2300, "relu", True)])
+@pytest.mark.parametrize("scale,eps", GN_SCALES)
+def test_group_norm_act_far_from_one(scale, eps, N, act, save8, dtype):
+    with emu.emulated_gpu():
+        run_gn_scale(scale, eps, N, act, dtype, save8)
+
+
+@pytest.mark.parametrize("N", [40, 2300])
+def test_group_norm_act_small_values_and_gradients(N):
+    with emu.emulated_gpu():
+        run_gn_scale(2.0 ** -70, 0.0, N, "silu", torch.float32, False, dy_scale=2.0 ** -70)

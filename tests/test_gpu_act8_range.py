@@ -38,3 +38,15 @@ def test_linear_act8_float16_top():
 
 def test_linear_act8_float16_magnitudes():
     cpu.run_float16_magnitudes(DEV)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("N,act,save8", [(40, "relu", False), (40, "silu", True), (2300, "gelu", False), (2300, "relu", True)])
+@pytest.mark.parametrize("scale,eps", cpu.GN_SCALES)
+def test_group_norm_act_far_from_one(scale, eps, N, act, save8, dtype):
+    cpu.run_gn_scale(scale, eps, N, act, dtype, save8, DEV)
+
+
+@pytest.mark.parametrize("N", [40, 2300])
+def test_group_norm_act_small_values_and_gradients(N):
+    cpu.run_gn_scale(2.0 ** -70, 0.0, N, "silu", torch.float32, False, DEV, dy_scale=2.0 ** -70)
