@@ -57,7 +57,8 @@ class ConvGNAct(nn.Module):
     Training on the GPU keeps the conv's input and the normalisation's input in 8 bits (ops.linear_act8,
     ops.group_norm_act): 1.03 bytes a value instead of 4 between forward and backward.  On the CPU: stock PyTorch ops.
     groups: default = the largest power of two <= 32 that leaves groups of at least 4 channels (1 where none does).
-    counts (forward): int32 [B] or [B, 1], valid rows of x [B, N, cin]."""
+    counts (forward): int32 [B] or [B, 1], valid rows of x [B, N, cin]; the rows behind them are in no statistics and come out
+    as 0, whatever finite values they hold."""
 
     bn, use_relu = None, False          # (not a layer of the BatchNorm kernels: train/common.py: supported)
 
@@ -126,13 +127,17 @@ def _warn_stock_fallback(layers, x):
                       RuntimeWarning, stacklevel=3)
 
 
-def run_mlp(layers, x, mfma=True):
+def run_mlp(layers, x, mfma=True, counts=None):
     """A stack of ConvBNReLU layers.  Training on the GPU: one autograd op over the hand-written
-    kernels (tmlp.mlp_bn_relu_train); otherwise the stock PyTorch modules.  ConvGNAct layers have kernels of their own."""
+    kernels (tmlp.mlp_bn_relu_train); otherwise the stock PyTorch modules.  ConvGNAct layers have kernels of their own;
+    counts, for these: int32 [B, 1], the valid entries of x's second axis ([B, O, C] centres, [B, O, P, C] their edges)."""
     if layers and all(isinstance(l, ConvGNAct) for l in layers):
+        shape = x.shape
+        if counts is not None and x.dim() == 4:
+            x, counts = x.reshape(shape[0], -1, shape[3]), counts * shape[2]
         for l in layers:
-            x = l(x)
-        return x
+            x = l(x, counts)
+        return x.reshape(shape[:-1] + x.shape[-1:])
     if mfma and x.is_cuda and layers and layers[0].training and torch.is_grad_enabled():
         from .train import common as tcommon, evalpath as teval, mlp as tmlp
         if tcommon.supported(layers, x):
@@ -221,6 +226,7 @@ class SubGUpdate(nn.Module):
     center_in  : channels of center_ori_feats (None: down layer)
     center_dim / out_dim : centre MLP and update MLP dims (up layers)
     norm       : 'batch' or 'group' (every layer a ConvGNAct)
+    counts of the forward calls: with norm = 'group', int32 [B, 1] valid centres of each cloud (None: all)
     """
 
     def __init__(self, in_feats, pt_mlp, localfdim=0, relu=True, center_in=None, center_dim=(),
@@ -257,16 +263,19 @@ class SubGUpdate(nn.Module):
             nf = neighbors[..., 4:]
         return nf, att_vec
 
-    def forward(self, centers_xyz, neighbors, center_masks=None, center_ori_feats=None, tail=None):
+    def forward(self, centers_xyz, neighbors, center_masks=None, center_ori_feats=None, tail=None, counts=None):
         """centers_xyz [B,O,3], neighbors [B,O,P,4+C] (already gathered), center_masks [B,O]|None,
         center_ori_feats [B,O,Cc]|None  ->  [B,O,out_channels]."""
         nf, att_vec = self.edge_inputs(neighbors, centers_xyz)
-        pair = self.att2(self.att1(att_vec)) * self.pt_mlp(nf)             # :135-167
+        if counts is not None:
+            pair = run_mlp([self.att1[0], self.att2[0]], att_vec, counts=counts) * run_mlp(list(self.pt_mlp), nf, counts=counts)
+        else:
+            pair = self.att2(self.att1(att_vec)) * self.pt_mlp(nf)         # :135-167
         agg = pair.max(dim=2).values                                       # :57-59 (unmasked, F10)
-        return self.finish(agg, center_masks, center_ori_feats, tail=tail)
+        return self.finish(agg, center_masks, center_ori_feats, tail=tail, counts=counts)
 
     def forward_src(self, cent, src, nebidx, center_masks=None, center_ori_feats=None, tail=None,
-                    defer_mask=False):
+                    defer_mask=False, counts=None):
         """Training path on the GPU: the edge inputs (gather + geo features + concat) come from
         one HIP kernel (ops.edge_inputs, scatter-add backward); the MLPs with batch-statistics
         BatchNorm are stock PyTorch ops.  defer_mask: the caller multiplies by center_masks itself
@@ -309,10 +318,10 @@ class SubGUpdate(nn.Module):
             if tedge.edge_block_supported(pt_layers, att_layers, nf, nebidx.shape[2]):
                 agg = tedge.edge_block_train(nf, att_vec, pt_layers, att_layers)
                 return self.finish(agg, center_masks, center_ori_feats, tail=tail)
-        pair = run_mlp(att_layers, att_vec, self.mfma_train) * \
-            run_mlp(pt_layers, nf, self.mfma_train)
+        pair = run_mlp(att_layers, att_vec, self.mfma_train, counts) * \
+            run_mlp(pt_layers, nf, self.mfma_train, counts)
         agg = pair.max(dim=2).values
-        return self.finish(agg, center_masks, center_ori_feats, tail=tail)
+        return self.finish(agg, center_masks, center_ori_feats, tail=tail, counts=counts)
 
     def packed_layers(self):
         """BatchNorm-folded, padded weights for the fused kernel (cached; eval mode only)."""
@@ -373,7 +382,7 @@ class SubGUpdate(nn.Module):
                                    has_feats=self.has_feats, localfdim=self.localfdim)
         return self.finish(agg, center_masks, center_ori_feats, tail=tail)
 
-    def finish(self, agg, center_masks, center_ori_feats, buf=None, tail=None):
+    def finish(self, agg, center_masks, center_ori_feats, buf=None, tail=None, counts=None):
         link = None
         nonneg = False   # both halves of the concat are >= 0: update_func's ReLU is the identity
         if center_ori_feats is not None and buf is not None:
@@ -392,7 +401,7 @@ class SubGUpdate(nn.Module):
                                              out=tcommon.alias_columns(buf, 0, ccf), link=link)
             agg = tcommon._Cat2.apply(cf, agg, buf).reshape(B, O, buf.shape[1])
         elif center_ori_feats is not None:
-            cf = (run_mlp(list(self.center_mlp), center_ori_feats, self.mfma_train)
+            cf = (run_mlp(list(self.center_mlp), center_ori_feats, self.mfma_train, counts)
                   if self.center_mlp is not None else center_ori_feats)
             agg = torch.cat([cf, agg], dim=-1)                             # up_center_inte=concat
         if self.relu and not nonneg:
@@ -427,7 +436,7 @@ class SubGUpdate(nn.Module):
                 from .train import common as tcommon, evalpath as teval, head as thead, mlp as tmlp
                 agg = tmlp.mlp_bn_relu_train(agg, layers, prev=link)
             else:
-                agg = run_mlp(layers, agg, self.mfma_train)
+                agg = run_mlp(layers, agg, self.mfma_train, counts)
         if center_masks is not None:
             agg = agg * center_masks[..., None]                            # :284-285
         return agg

@@ -135,7 +135,8 @@ class GGCNSeg(nn.Module):
         # int64 GPU scalar added to every sampling / dropout seed inside the kernels (None: off).
         # graph.GraphedTrainStep sets and bumps it so that replays of ONE captured step still redraw
         self.seed_dev = None
-        # cfg["norm"] = "group": every conv of the net normalised per cloud (gridconv.ConvGNAct) instead of per batch
+        # cfg["norm"] = "group": every conv of the net normalised per cloud (gridconv.ConvGNAct) instead of per batch, over the
+        # cloud's own points and centres (what pads a batch is in no statistics)
         norm = self.norm = cfg.get("norm", "batch")
         g = cfg["grid"]
         nd = len(g["down"])
@@ -210,6 +211,7 @@ class GGCNSeg(nn.Module):
         feats = [data]                # center_locnfeat_alllayers: [B,n,4+C]
         feats_pad = [data_pad]        # (rows zero-padded to whole 32-byte pieces: the centre MLPs' input)
         masks, nums = [], [actual_centnum]
+        own = (lambda num: num) if self.norm == "group" else (lambda num: None)
         data_loc, data_layer = data, data
         fwd_no = self.forward_no
         if self.training:
@@ -236,10 +238,10 @@ class GGCNSeg(nn.Module):
                     self.jobs.append(("down%d" % i, layer, cent, data_layer, nebidx))
                 cf = layer.forward_fused(cent, data_layer, nebidx, centmsk)
             elif _is_hip(self.ix) and self.edge_kernel:
-                cf = layer.forward_src(cent, data_layer, nebidx, centmsk, defer_mask=glue)
+                cf = layer.forward_src(cent, data_layer, nebidx, centmsk, defer_mask=glue, counts=own(centnum))
             else:
                 neighbors = ix.batch_take_g(data_layer.contiguous(), nebidx, **self._take_kw)  # :172-173
-                cf = layer(cent[..., 0:3], neighbors, centmsk)                      # :185
+                cf = layer(cent[..., 0:3], neighbors, centmsk, counts=own(centnum)) # :185
             if glue:
                 data_layer, dl_pad = tcommon.cat_mask(cent, cf, centmsk, pad=i != nd - 1)   # :186
             else:
@@ -284,11 +286,11 @@ class GGCNSeg(nn.Module):
                                          tail=tail if i == nup - 1 else None)
             elif _is_hip(self.ix) and self.edge_kernel:
                 cf = layer.forward_src(upl, f_last, nebidx, cmask, center_ori_feats=f_this,
-                                       tail=tail if i == nup - 1 else None, defer_mask=glue)
+                                       tail=tail if i == nup - 1 else None, defer_mask=glue, counts=own(upnum))
             else:
                 neighbors = ix.batch_take_g(f_last.contiguous(), nebidx, **self._take_kw)  # :217-218
                 cf = layer(upl[..., 0:3], neighbors, cmask, center_ori_feats=f_this,
-                           tail=tail if i == nup - 1 else None)                       # :229
+                           tail=tail if i == nup - 1 else None, counts=own(upnum))    # :229
             if i != nup - 1:                      # (the last layer's features go to the head only)
                 if glue:
                     f_last = tcommon.cat_mask(upl, cf, cmask)[0]                  # :231
@@ -297,7 +299,7 @@ class GGCNSeg(nn.Module):
         self.last_tail_done = tail.done           # (introspection only: which head path ran)
         if tail.done == 2:                        # fc1, dropout and fc2 ran inside the last up layer
             return cf
-        net = cf if tail.done else run_mlp([self.fc1], cf)
+        net = cf if tail.done else run_mlp([self.fc1], cf, counts=own(actual_centnum))
         net = F.dropout(net, self.cfg["dropout"], self.training)
         if HEAD_KERNELS and self.training and torch.is_grad_enabled() and _is_hip(self.ix):
             from .train import common as tcommon, head as thead

@@ -13,7 +13,7 @@ import act8_cases as cases  # noqa: E402
 import test_act8 as base  # noqa: E402
 from oracle import act8_ref as ref  # noqa: E402
 from simt import emu  # noqa: E402
-from grid_gcn_amd import ops  # noqa: E402
+from grid_gcn_amd import gridconv, model, ops, synth  # noqa: E402
 
 
 # ---- float32 products: the bound is that of a float32 sum of |x| |w|, whatever the range of a row or a column -----------
@@ -173,3 +173,74 @@ def test_group_norm_act_far_from_one(scale, eps, N, act, save8, dtype):
 def test_group_norm_act_small_values_and_gradients(N):
     with emu.emulated_gpu():
         run_gn_scale(2.0 ** -70, 0.0, N, "silu", torch.float32, False, dy_scale=2.0 ** -70)
+
+
+# ---- counts through the framework's own layers ---------------------------------------------------------------------------
+def run_padded_layers(dev="cpu"):
+    """what pads a cloud changes nothing of its own results: rows of centres, and edges of centres"""
+    torch.manual_seed(4)
+    net = gridconv.mlp(10, [24, 32], norm="group").to(dev)
+    for shape in ((1, 100, 10), (1, 30, 5, 10)):
+        x = torch.randn(shape)
+        pad = torch.cat([x, torch.zeros((1, 50) + shape[2:])], 1)
+        both = torch.cat([pad, torch.randn(pad.shape)]).to(dev)
+        n = torch.tensor([[shape[1]], [both.shape[1]]], dtype=torch.int32, device=dev)
+        alone = gridconv.run_mlp(list(net), x.to(dev), counts=n[:1])
+        g1 = torch.autograd.grad(alone.square().sum(), list(net.parameters()))
+        got = gridconv.run_mlp(list(net), both, counts=n)
+        g2 = torch.autograd.grad(got[:1, :shape[1]].square().sum(), list(net.parameters()))
+        # (the same values on the same weights: float32 sums in another order at most, each worth 2^-20 of the norm)
+        assert float((got[:1, :shape[1]] - alone).norm() / alone.norm()) < 2.0 ** -18
+        assert float(got[0, shape[1]:].abs().max()) == 0.0
+        assert all(float((a - b).norm()) <= 2.0 ** -8 * float(a.norm()) + 1e-4 for a, b in zip(g1, g2))
+
+
+def test_padded_layers():
+    run_padded_layers()                                    # stock operations
+    with emu.emulated_gpu():
+        run_padded_layers()
+
+
+def _small_group_net():
+    import copy
+    cfg = copy.deepcopy(model.SEG_8192)
+    cfg["norm"] = "group"
+    for lv, (P, O) in zip(cfg["grid"]["down"], ((8, 24), (4, 12), (4, 6))):
+        lv["max_p_grid"], lv["max_o_grid"] = P, O
+    for lv, O in zip(cfg["grid"]["up"], (12, 24, 64)):
+        lv["max_o_grid"] = O
+    cfg.update(pt_ele_dim=[[16, 32]] + [[32, 32]] * 2, inputDim=[0, 32, 32], up_inputDim=[32] * 3, up_center_dim=[[32]] * 3,
+               up_pt_ele_dim=[[32]] * 3, up_gcn_outDim=[[32]] * 3, dropout=0.0)
+    return cfg
+
+
+def run_cloud_in_any_company(index_ops, dev="cpu"):
+    """a cloud of 40 points: its logits and the gradients of its loss, alone and in front of a cloud of 64"""
+    torch.manual_seed(0)
+    net = model.GGCNSeg(_small_group_net(), index_ops=index_ops, fixed_seed=True).to(dev).train()
+    data, npn = synth.make_batch(2, 64, "planes")
+    x = torch.from_numpy(data[..., :3].copy())
+    n = torch.tensor([[40], [64]], dtype=torch.int32)
+    lab = torch.randint(1, 21, (2, 64))
+    lab[0, 40:] = 0
+    lab[1] = 0                                             # (the ignored label)
+    res = []
+    for clouds, length in ((1, 40), (2, 64)):
+        net.zero_grad()
+        out = net(x[:clouds, :length].contiguous().to(dev), n[:clouds].to(dev))
+        model.seg_loss(out, lab[:clouds, :length].contiguous().to(dev)).backward()
+        res.append((out[0, :40].detach().cpu(), {k: p.grad.cpu().clone() for k, p in net.named_parameters()}))
+    (a, ga), (b, gb) = res
+    assert float((a - b).norm() / a.norm()) < 2.0 ** -16
+    va, vb = (torch.cat([g[k].reshape(-1) for k in ga]) for g in (ga, gb))
+    assert float((va - vb).norm() / va.norm()) < 2.0 ** -8, float((va - vb).norm() / va.norm())
+
+
+def test_cloud_in_any_company_stock_operations():
+    from oracle.torch_index_ops import OracleIndexOps
+    run_cloud_in_any_company(OracleIndexOps)
+
+
+def test_cloud_in_any_company_kernels():
+    with emu.emulated_gpu():
+        run_cloud_in_any_company(model.HipIndexOps)

@@ -8,6 +8,7 @@ import torch
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 
 import test_act8_range as cpu  # noqa: E402
+from grid_gcn_amd import model  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -50,3 +51,11 @@ def test_group_norm_act_far_from_one(scale, eps, N, act, save8, dtype):
 @pytest.mark.parametrize("N", [40, 2300])
 def test_group_norm_act_small_values_and_gradients(N):
     cpu.run_gn_scale(2.0 ** -70, 0.0, N, "silu", torch.float32, False, DEV, dy_scale=2.0 ** -70)
+
+
+def test_padded_layers():
+    cpu.run_padded_layers(DEV)
+
+
+def test_cloud_in_any_company():
+    cpu.run_cloud_in_any_company(model.HipIndexOps, DEV)
