@@ -13,6 +13,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -58,6 +59,12 @@ def _check_rows(t, name, min_dim=1):
     _require(t.is_cuda, "%s must live on the GPU (there is no CPU path)" % name)
     _require(t.dtype in _DTYPES, "%s must be float32, bfloat16 or float16" % name)
     _require(t.dim() >= min_dim, "%s should have at least %d dimensions" % (name, min_dim))
+
+
+def _no_tangents(name, *ts):
+    if forward_ad._current_level >= 0:
+        for t in ts:
+            _require(t is None or forward_ad.unpack_dual(t).tangent is None, "%s has no forward-mode derivative" % name)
 
 
 def _rows2(t):
@@ -251,9 +258,10 @@ def group_norm_act(x, weight, bias, groups, eps=1e-5, act="relu", counts=None, s
     statistics; their output and gradient are 0 and what they hold is never read.
     save8: keep x for the backward in 8 bits (act8_pack) instead of x itself: 1.03 bytes a value.  The gradients are then those of
     the formulas at the 8-bit values of x, with the statistics of x.
-    Not differentiable twice."""
+    Not differentiable twice, nor in forward mode."""
     eps = float(eps)
     C, groups, ptype = _check_gn(x, weight, bias, groups, eps, act, counts)
+    _no_tangents("group_norm_act", x, weight, bias)
     if x.numel() == 0:
         y = x * 0
         for t in (weight, bias):
@@ -347,8 +355,9 @@ def linear_act8(x, weight, bias=None):
     Sums are in float32.  A float32 operand enters the matrix instructions as a sum of three bfloat16 numbers, whatever stands
     beside it in its row and however many rows there are; the error of a product is that of a float32 product, but an operand that is
     infinite or beyond 3.39e38 gives NaN, and what of an operand lies below 2^-134 is dropped.
-    Backward: dx = dy W and dbias as ever; dW = dy^T x^ with x^ the 8-bit values of x.  Not differentiable twice."""
+    Backward: dx = dy W and dbias as ever; dW = dy^T x^ with x^ the 8-bit values of x.  Not differentiable twice, nor in forward mode."""
     K, N = _check_linear(x, weight, bias)
+    _no_tangents("linear_act8", x, weight, bias)
     if x.numel() == 0:
         return torch.nn.functional.linear(x, weight, bias)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):

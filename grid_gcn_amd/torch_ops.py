@@ -215,6 +215,7 @@ def group_norm_act(x: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], 
                    save8: bool = False) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
     _, groups, ptype = act8._check_gn(x, weight, bias, groups, eps, act, counts)
     act8._require(x.numel() > 0, "x must not be empty")
+    act8._no_tangents("group_norm_act", x, weight, bias)
     y, _, st, codes, scales = act8._gn_forward(x, weight, bias, groups, ptype, eps, act, counts, save8, True)
     if not save8:
         codes, scales = (torch.empty(0, dtype=torch.uint8, device=x.device) for _ in range(2))
@@ -274,6 +275,7 @@ group_norm_act.register_autograd(_gn_bwd, setup_context=_gn_setup)
 def linear_act8(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
     act8._check_linear(x, weight, bias)
     act8._require(x.numel() > 0, "x must not be empty")
+    act8._no_tangents("linear_act8", x, weight, bias)
     return act8._linear_forward(x, weight, bias, True)
 
 

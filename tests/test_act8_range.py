@@ -244,3 +244,27 @@ def test_cloud_in_any_company_stock_operations():
 def test_cloud_in_any_company_kernels():
     with emu.emulated_gpu():
         run_cloud_in_any_company(model.HipIndexOps)
+
+
+# ---- forward-mode differentiation: refused, not dropped ------------------------------------------------------------------
+def run_tangents_refused(dev="cpu"):
+    import torch.autograd.forward_ad as fwd
+    x, w, v = torch.randn(2, 6, 8, device=dev), torch.randn(4, 8, device=dev), torch.ones(8, device=dev)
+    gn = lambda x, v: ops.group_norm_act(x, v, v, 2)                      # noqa: E731
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))             # noqa: E731
+        for call in (lambda: gn(dual(x), v), lambda: gn(x, dual(v)), lambda: ops.linear_act8(dual(x), w),
+                     lambda: ops.linear_act8(x, dual(w)), lambda: ops.linear_act8(x, w, dual(v[:4].clone())),
+                     lambda: ops.linear_act8(dual(x[:0]), w), lambda: gn(dual(x[:0]), v)):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(RuntimeError):
+                    call()
+        assert ops.linear_act8(x, w).shape == (2, 6, 4) and gn(x, v).shape == x.shape       # (a level without tangents)
+    for f, t in ((lambda x: gn(x, v), x), (lambda x: ops.linear_act8(x, w), x)):
+        with pytest.raises(RuntimeError):
+            torch.func.jvp(f, (t,), (torch.ones_like(t),))
+
+
+def test_tangents_refused():
+    with emu.emulated_gpu():
+        run_tangents_refused()

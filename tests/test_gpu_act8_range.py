@@ -59,3 +59,52 @@ def test_padded_layers():
 
 def test_cloud_in_any_company():
     cpu.run_cloud_in_any_company(model.HipIndexOps, DEV)
+
+
+def test_tangents_refused():
+    cpu.run_tangents_refused(DEV)
+
+
+@pytest.mark.parametrize("need", [False, True])
+def test_tangents_refused_by_the_registered_operators(need):
+    import torch.autograd.forward_ad as fwd
+    x, w, v = torch.randn(2, 6, 8, device=DEV, requires_grad=need), torch.randn(4, 8, device=DEV), torch.ones(8, device=DEV)
+    g = torch.ops.gridgcn
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))             # noqa: E731
+        for call in (lambda: g.group_norm_act(dual(x), v, v, 2), lambda: g.group_norm_act(x, dual(v), v, 2),
+                     lambda: g.linear_act8(dual(x), w), lambda: g.linear_act8(x, dual(w))):
+            with pytest.raises(RuntimeError):
+                call()
+
+
+def test_captured_step_of_the_group_norm_net_follows_the_counts():
+    """replays of one captured training step, with other clouds, counts and eager work in between, against eager steps"""
+    import copy
+    from grid_gcn_amd import graph, synth
+    torch.manual_seed(0)
+    net = model.GGCNSeg(cpu._small_group_net(), fixed_seed=True).to(DEV).train()
+    twin = copy.deepcopy(net)
+    data, _ = synth.make_batch(4, 64, "planes")
+    clouds = torch.from_numpy(data[..., :3].copy()).to(DEV)
+    x, n = clouds[:2].clone(), torch.tensor([[64], [40]], dtype=torch.int32, device=DEV)
+    lab = torch.randint(1, 21, (2, 64), device=DEV)
+    adam = lambda m: torch.optim.Adam(m.parameters(), lr=1e-3, fused=True, capturable=True)          # noqa: E731
+    opt, opt2 = adam(net), adam(twin)
+    step = graph.GraphedTrainStep(net, opt, model.seg_loss, (x, n), lab, warmup=1)
+
+    def eager():
+        opt2.zero_grad(set_to_none=True)
+        loss = model.seg_loss(twin(x, n), lab)
+        loss.backward()
+        opt2.step()
+        return float(loss)
+
+    eager()                                               # (the warm-up step)
+    for i, counts in enumerate(((64, 40), (17, 64), (64, 64), (33, 50))):
+        x.copy_(clouds[[i, (i + 1) % 4]])
+        n.copy_(torch.tensor(counts, dtype=torch.int32)[:, None])
+        got, want = float(step()), eager()
+        torch.cuda.synchronize()
+        # (the same kernels on the same values; only the gathers' gradient sums may come in another order)
+        assert abs(got - want) < 1e-4 * abs(want), (i, got, want)
