@@ -252,7 +252,8 @@ def group_norm_act_backward(dy: Tensor, x: Optional[Tensor], codes: Optional[Ten
 @group_norm_act_backward.register_fake
 def _(dy, x, codes, scales, stats, weight, bias, groups, act, counts=None):
     return (torch.empty_like(dy, memory_format=torch.contiguous_format),
-            dy.new_empty(0) if weight is None else torch.empty_like(weight), dy.new_empty(0) if bias is None else torch.empty_like(bias))
+            dy.new_empty(0) if weight is None else weight.new_empty(tuple(weight.shape)),
+            dy.new_empty(0) if bias is None else bias.new_empty(tuple(bias.shape)))
 
 
 def _gn_setup(ctx, inputs, output):
@@ -298,7 +299,7 @@ def linear_act8_backward(dy: Tensor, weight: Tensor, codes: Tensor, scales: Tens
 
 @linear_act8_backward.register_fake
 def _(dy, weight, codes, scales):
-    return (dy.new_empty(tuple(dy.shape[:-1]) + (weight.shape[1],)), torch.empty_like(weight), dy.new_empty(weight.shape[0]))
+    return (dy.new_empty(tuple(dy.shape[:-1]) + (weight.shape[1],)), dy.new_empty(tuple(weight.shape)), dy.new_empty(weight.shape[0]))
 
 
 def _lin8_setup(ctx, inputs, output):

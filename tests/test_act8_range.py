@@ -268,3 +268,26 @@ def run_tangents_refused(dev="cpu"):
 def test_tangents_refused():
     with emu.emulated_gpu():
         run_tangents_refused()
+
+
+# ---- the registered operators on fake tensors: what a compiled graph plans with --------------------------------------------
+def _layouts(ts):
+    return [(tuple(t.shape), t.stride(), t.dtype) for t in ts]
+
+
+def test_fake_backwards_have_the_layouts_of_the_kernels():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    import grid_gcn_amd  # noqa: F401
+    bf, g = torch.bfloat16, torch.ops.gridgcn
+    with FakeTensorMode():
+        w = torch.empty((33, 7), device="cuda", dtype=bf).t()                     # a transposed weight
+        dy = torch.empty((7, 100, 2), device="cuda", dtype=bf).permute(2, 1, 0)
+        codes, scales = torch.empty((200, 64), device="cuda", dtype=torch.uint8), torch.empty((200, 2), device="cuda", dtype=torch.uint8)
+        assert _layouts(g.linear_act8_backward(dy, w, codes, scales)) == [
+            ((2, 100, 33), (3300, 33, 1), bf), ((7, 33), (33, 1), bf), ((7,), (1,), bf)]
+        gamma = torch.empty(66, device="cuda")[::2]
+        beta = torch.empty(1, device="cuda").expand(33)
+        dy = torch.empty((33, 100, 2), device="cuda", dtype=bf).permute(2, 1, 0)
+        st = torch.empty((2, 3, 2), device="cuda", dtype=torch.float64)
+        assert _layouts(g.group_norm_act_backward(dy, None, codes, scales, st, gamma, beta, 3, "silu")) == [
+            ((2, 100, 33), (3300, 33, 1), bf), ((33,), (1,), torch.float32), ((33,), (1,), torch.float32)]
