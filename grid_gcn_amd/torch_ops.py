@@ -185,7 +185,8 @@ batch_take.register_autograd(_take_bwd, setup_context=_take_setup)
 #     torch.ops.gridgcn.act8_unpack(codes, scales, C, dtype) -> x
 #     torch.ops.gridgcn.group_norm_act(x, weight, bias, groups, eps=1e-5, act="relu", counts=None, save8=False)
 #         -> (y, stats, codes, scales)         differentiable w.r.t. x, weight, bias through y; stats [B, groups, 2] f64
-#                                              (mean, rstd); codes, scales: empty without save8, rows >= counts unwritten
+#                                              (mean, rstd), not differentiable; codes, scales: empty without save8, rows >= counts
+#                                              unwritten
 #     torch.ops.gridgcn.linear_act8(x, weight, bias=None) -> (y, codes, scales)        differentiable through y
 @_lib_def("gridgcn::act8_pack", mutates_args=(), device_types="cuda")
 def act8_pack(x: Tensor) -> Tuple[Tensor, Tensor]:
@@ -259,6 +260,7 @@ def _(dy, x, codes, scales, stats, weight, bias, groups, act, counts=None):
 def _gn_setup(ctx, inputs, output):
     x, weight, bias, groups, eps, act, counts, save8 = inputs
     _, st, codes, scales = output
+    ctx.mark_non_differentiable(st)
     ctx.save_for_backward(None if save8 else x, codes if save8 else None, scales if save8 else None, st, weight, bias, counts)
     ctx.gn = (groups, act)
 

@@ -291,3 +291,13 @@ def test_fake_backwards_have_the_layouts_of_the_kernels():
         st = torch.empty((2, 3, 2), device="cuda", dtype=torch.float64)
         assert _layouts(g.group_norm_act_backward(dy, None, codes, scales, st, gamma, beta, 3, "silu")) == [
             ((2, 100, 33), (3300, 33, 1), bf), ((33,), (1,), torch.float32), ((33,), (1,), torch.float32)]
+
+
+def test_statistics_of_the_registered_operator_are_not_differentiable():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    import grid_gcn_amd  # noqa: F401
+    with FakeTensorMode():
+        x = torch.empty((2, 100, 33), device="cuda", requires_grad=True)
+        for save8 in (False, True):
+            y, st, codes, scales = torch.ops.gridgcn.group_norm_act(x, None, None, 3, save8=save8)
+            assert y.requires_grad and not st.requires_grad and not codes.requires_grad and not scales.requires_grad
