@@ -234,8 +234,9 @@ def _(x, weight, bias, groups, eps=1e-5, act="relu", counts=None, save8=False):
 @_lib_def("gridgcn::group_norm_act_backward", mutates_args=(), device_types="cuda")
 def group_norm_act_backward(dy: Tensor, x: Optional[Tensor], codes: Optional[Tensor], scales: Optional[Tensor],
                             stats: Tensor, weight: Optional[Tensor], bias: Optional[Tensor], groups: int, act: str,
-                            counts: Optional[Tensor] = None) -> Tuple[Tensor, Tensor, Tensor]:
-    """(dx, dweight, dbias); the last two are empty where the parameter is None"""
+                            counts: Optional[Tensor] = None, need_dx: bool = True, need_dw: bool = True,
+                            need_db: bool = True) -> Tuple[Tensor, Tensor, Tensor]:
+    """(dx, dweight, dbias); empty and not computed: what is not needed, and the gradient of a parameter that is None"""
     _, groups, ptype = act8._check_gn(dy, weight, bias, groups, 0.0, act, counts)
     B, C = dy.shape[0], dy.shape[-1]
     act8._require(stats.dtype == torch.float64 and stats.is_contiguous() and tuple(stats.shape) == (B, groups, 2),
@@ -246,15 +247,15 @@ def group_norm_act_backward(dy: Tensor, x: Optional[Tensor], codes: Optional[Ten
         act8._require(x is not None and x.shape == dy.shape and x.dtype == dy.dtype, "x must have dy's shape and type")
         x = act8._rows3(x, B)[0]
     dx, dw, db = act8._gn_backward(dy, x, codes, scales, stats, weight, bias, tuple(dy.shape), groups, ptype, act, counts,
-                                   (True, weight is not None, bias is not None))
-    return dx, dy.new_empty(0) if dw is None else dw, dy.new_empty(0) if db is None else db
+                                   (need_dx, need_dw and weight is not None, need_db and bias is not None))
+    return tuple(dy.new_empty(0) if t is None else t for t in (dx, dw, db))
 
 
 @group_norm_act_backward.register_fake
-def _(dy, x, codes, scales, stats, weight, bias, groups, act, counts=None):
-    return (torch.empty_like(dy, memory_format=torch.contiguous_format),
-            dy.new_empty(0) if weight is None else weight.new_empty(tuple(weight.shape)),
-            dy.new_empty(0) if bias is None else bias.new_empty(tuple(bias.shape)))
+def _(dy, x, codes, scales, stats, weight, bias, groups, act, counts=None, need_dx=True, need_dw=True, need_db=True):
+    return (torch.empty_like(dy, memory_format=torch.contiguous_format) if need_dx else dy.new_empty(0),
+            weight.new_empty(tuple(weight.shape)) if need_dw and weight is not None else dy.new_empty(0),
+            bias.new_empty(tuple(bias.shape)) if need_db and bias is not None else dy.new_empty(0))
 
 
 def _gn_setup(ctx, inputs, output):
@@ -267,8 +268,9 @@ def _gn_setup(ctx, inputs, output):
 
 def _gn_bwd(ctx, dy, *_):
     x, codes, scales, st, weight, bias, counts = ctx.saved_tensors
-    dx, dw, db = torch.ops.gridgcn.group_norm_act_backward(dy, x, codes, scales, st, weight, bias, *ctx.gn, counts)
-    return dx, None if weight is None else dw, None if bias is None else db, None, None, None, None, None
+    need = ctx.needs_input_grad[:3]
+    grads = torch.ops.gridgcn.group_norm_act_backward(dy, x, codes, scales, st, weight, bias, *ctx.gn, counts, *need)
+    return tuple(t if n else None for t, n in zip(grads, need)) + (None,) * 5
 
 
 group_norm_act.register_autograd(_gn_bwd, setup_context=_gn_setup)
@@ -290,31 +292,34 @@ def _(x, weight, bias=None):
 
 
 @_lib_def("gridgcn::linear_act8_backward", mutates_args=(), device_types="cuda")
-def linear_act8_backward(dy: Tensor, weight: Tensor, codes: Tensor, scales: Tensor) -> Tuple[Tensor, Tensor, Tensor]:
-    """(dx, dweight, dbias)"""
+def linear_act8_backward(dy: Tensor, weight: Tensor, codes: Tensor, scales: Tensor, need_dx: bool = True,
+                         need_dw: bool = True, need_db: bool = True) -> Tuple[Tensor, Tensor, Tensor]:
+    """(dx, dweight, dbias); empty and not computed: what is not needed"""
     act8._check_rows(dy, "dy")
     N, K = weight.shape
     act8._require(weight.dtype == dy.dtype and weight.device == dy.device and dy.shape[-1] == N, "weight should be [%d, K] of dy's type" % dy.shape[-1])
     act8._check_codes(codes, scales, dy.numel() // N, K)
-    return act8._linear_backward(dy, weight, codes, scales, tuple(dy.shape[:-1]) + (K,), (True, True, True))
+    grads = act8._linear_backward(dy, weight, codes, scales, tuple(dy.shape[:-1]) + (K,), (need_dx, need_dw, need_db))
+    return tuple(dy.new_empty(0) if t is None else t for t in grads)
 
 
 @linear_act8_backward.register_fake
-def _(dy, weight, codes, scales):
-    return (dy.new_empty(tuple(dy.shape[:-1]) + (weight.shape[1],)), dy.new_empty(tuple(weight.shape)), dy.new_empty(weight.shape[0]))
+def _(dy, weight, codes, scales, need_dx=True, need_dw=True, need_db=True):
+    return (dy.new_empty(tuple(dy.shape[:-1]) + (weight.shape[1],) if need_dx else 0),
+            dy.new_empty(tuple(weight.shape) if need_dw else 0), dy.new_empty(weight.shape[0] if need_db else 0))
 
 
 def _lin8_setup(ctx, inputs, output):
     x, weight, bias = inputs
     _, codes, scales = output
     ctx.save_for_backward(weight, codes, scales)
-    ctx.has_bias = bias is not None
 
 
 def _lin8_bwd(ctx, dy, *_):
     weight, codes, scales = ctx.saved_tensors
-    dx, dw, db = torch.ops.gridgcn.linear_act8_backward(dy, weight, codes, scales)
-    return dx, dw, db if ctx.has_bias else None
+    need = ctx.needs_input_grad
+    grads = torch.ops.gridgcn.linear_act8_backward(dy, weight, codes, scales, *need)
+    return tuple(t if n else None for t, n in zip(grads, need))
 
 
 linear_act8.register_autograd(_lin8_bwd, setup_context=_lin8_setup)

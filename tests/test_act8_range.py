@@ -301,3 +301,25 @@ def test_statistics_of_the_registered_operator_are_not_differentiable():
         for save8 in (False, True):
             y, st, codes, scales = torch.ops.gridgcn.group_norm_act(x, None, None, 3, save8=save8)
             assert y.requires_grad and not st.requires_grad and not codes.requires_grad and not scales.requires_grad
+
+
+def test_registered_backwards_leave_out_what_is_not_needed():
+    from types import SimpleNamespace
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from grid_gcn_amd import torch_ops
+    with FakeTensorMode():
+        e = lambda *s: torch.empty(s, device="cuda")                      # noqa: E731
+        codes, scales = (torch.empty(s, device="cuda", dtype=torch.uint8) for s in ((18, 32), (18, 1)))
+        w, v, st = e(5, 32), e(32), torch.empty((2, 4, 2), device="cuda", dtype=torch.float64)
+        for need in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 1)):
+            sizes = lambda shapes: [s if n else (0,) for s, n in zip(shapes, need)]       # noqa: E731
+            need = tuple(bool(n) for n in need)
+            got = torch.ops.gridgcn.linear_act8_backward(e(2, 9, 5), w, codes, scales, *need)
+            assert [tuple(t.shape) for t in got] == sizes(((2, 9, 32), (5, 32), (5,)))
+            got = torch_ops._lin8_bwd(SimpleNamespace(saved_tensors=(w, codes, scales), needs_input_grad=need), e(2, 9, 5), None, None)
+            assert [t is not None for t in got] == list(need)
+            got = torch.ops.gridgcn.group_norm_act_backward(e(2, 9, 32), None, codes, scales, st, v, v, 4, "relu", None, *need)
+            assert [tuple(t.shape) for t in got] == sizes(((2, 9, 32), (32,), (32,)))
+            ctx = SimpleNamespace(saved_tensors=(None, codes, scales, st, v, v, None), needs_input_grad=need + (False,) * 5, gn=(4, "relu"))
+            got = torch_ops._gn_bwd(ctx, e(2, 9, 32), None, None, None)
+            assert len(got) == 8 and [t is not None for t in got[:3]] == list(need)

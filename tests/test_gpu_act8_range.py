@@ -108,3 +108,21 @@ def test_captured_step_of_the_group_norm_net_follows_the_counts():
         torch.cuda.synchronize()
         # (the same kernels on the same values; only the gathers' gradient sums may come in another order)
         assert abs(got - want) < 1e-4 * abs(want), (i, got, want)
+
+
+def test_registered_backwards_leave_out_what_is_not_needed():
+    g = torch.ops.gridgcn
+    x, w, b, v = (torch.randn(s, device=DEV) for s in ((40, 32), (5, 32), (5,), (32,)))
+    _, codes, scales = g.linear_act8(x, w, b)
+    y, st, c8, s8 = g.group_norm_act(x, v, v, 4, save8=True)
+    dy = torch.randn(40, 5, device=DEV)
+    full = g.linear_act8_backward(dy, w, codes, scales), g.group_norm_act_backward(x, None, c8, s8, st, v, v, 4, "relu")
+    for need in ((1, 0, 0), (0, 1, 0), (0, 0, 1)):
+        need = tuple(bool(n) for n in need)
+        part = g.linear_act8_backward(dy, w, codes, scales, *need), g.group_norm_act_backward(x, None, c8, s8, st, v, v, 4, "relu", None, *need)
+        for f, p in zip(full, part):
+            assert all(torch.equal(a, q) if n else q.numel() == 0 for a, q, n in zip(f, p, need))
+        leaves = [t.clone().requires_grad_(n) for t, n in zip((x, w, b), need)]
+        y = g.linear_act8(*leaves)[0]
+        y.backward(dy)
+        assert all((t.grad is not None) == n and (not n or torch.equal(t.grad, a)) for t, n, a in zip(leaves, need, full[0]))
