@@ -65,35 +65,52 @@ __device__ __forceinline__ long long count_of(const Args &a, int b)
     return n < 0 ? 0 : (n < a.N ? n : a.N);
 }
 
-// Phi(t) = (1 + erf(t / sqrt 2)) / 2 and e = exp(-t^2 / 2), which its derivative wants as well.  erf by the rational
-// approximation 7.1.26 of Abramowitz and Stegun, whose one exponential is that same e: |error of Phi| < 7.5e-8, about half a step
-// of float32 at 1 (half the instructions of erff plus an exponential: a forward + backward of 67 M bf16 values by erff was
-// bound by arithmetic).
-__device__ __forceinline__ float normal_cdf(float t, float &e)
+// Phi(t) = (1 + erf(t / sqrt 2)) / 2 and e = exp(-t^2 / 2), which its derivative wants as well.  Phi(-a) = e R(a), and R falls slowly,
+// from 1/2 as 1 / (a sqrt(2 pi)): a polynomial in k = 1 / (1 + p a), fitted for the least relative error over 0 <= a <= 14.5 (beyond,
+// e is 0).
+//   32-bit rows: R = k Q(1 - k), Q of degree 9, error 2e-9: t Phi(t) is off by 3.5e-8 of its norm for normal t (0.5 t (1 + erf), erf
+//   to a step: 3.7e-8) and keeps its digits where Phi(t) is small (4e-6 of the value at t = -9, the exponential's);
+//   16-bit rows: degree 6 in k, error 1e-7 at 0, growing to 2e-4 (half of fp16's half step) from |t| = 5 on.  (Degree 9 for them too:
+//   backward of 16 x 65536 x 64 bf16 from codes 159 us, not 146.)
+template <class T> __device__ __forceinline__ float normal_cdf(float t, float &e)
 {
-    const float a = fabsf(t), k = __builtin_amdgcn_rcpf(fmaf(a, 0.3275911f * SQRT1_2, 1.f));
-    e = __expf(-0.5f * t * t);
-    float q = fmaf(k, 1.061405429f, -1.453152027f);
-    q = fmaf(k, q, 1.421413741f);
-    q = fmaf(k, q, -0.284496736f);
-    q = fmaf(k, q, 0.254829592f);
-    q *= 0.5f * k * e;                      // Phi(-|t|): no cancellation on the side where it is small
-    return t < 0.f ? q : 1.f - q;
+    e = __builtin_amdgcn_exp2f(t * t * -0.72134752f);
+    float q;
+    if constexpr (GGRowT<T>::id == GG_T_F32) {
+        const float pa = 0.2375f * fminf(fabsf(t), 16.f), k = __builtin_amdgcn_rcpf(1.f + pa), m = pa * k;      // m = 1 - k
+        q = fmaf(m, -0.0271149112f, 0.105926423f);
+        q = fmaf(m, q, -0.114639388f);
+        q = fmaf(m, q, -0.0758714394f);
+        q = fmaf(m, q, 0.169976482f);
+        q = fmaf(m, q, 0.313199016f);
+        q = fmaf(m, q, -1.1696099f);
+        q = fmaf(m, q, 1.57263014f);
+        q = fmaf(m, q, -1.17975722f);
+        q = fmaf(m, q, 0.500000001f) * (k * e);
+    } else {
+        const float k = __builtin_amdgcn_rcpf(fmaf(fabsf(t), 0.2875f, 1.f));
+        q = fmaf(k, -0.0921373988f, 0.305879399f);
+        q = fmaf(k, q, -0.11953044f);
+        q = fmaf(k, q, 0.19386526f);
+        q = fmaf(k, q, 0.0956545484f);
+        q = fmaf(k, q, 0.116268678f) * (k * e);
+    }
+    return t < 0.f ? q : 1.f - q;           // (q = Phi(-|t|): no cancellation on the side where it is small)
 }
 // (the reciprocal instruction is good to one step: far below the activation's own rounding budget)
 __device__ __forceinline__ float sigmoid(float t) { return __builtin_amdgcn_rcpf(1.f + __expf(-t)); }
 
-template <int ACT> __device__ __forceinline__ float act_of(float t)
+template <int ACT, class T> __device__ __forceinline__ float act_of(float t)
 {
     if constexpr (ACT == GRIDGCN_ACT_RELU) return t > 0.f ? t : (t != t ? t : 0.f);     // (NaN stays NaN)
     if constexpr (ACT == GRIDGCN_ACT_SILU) return t * sigmoid(t);
     if constexpr (ACT == GRIDGCN_ACT_GELU) {
         float e;
-        return t * normal_cdf(t, e);
+        return t * normal_cdf<T>(t, e);
     }
     return t;
 }
-template <int ACT> __device__ __forceinline__ float act_grad(float t)
+template <int ACT, class T> __device__ __forceinline__ float act_grad(float t)
 {
     if constexpr (ACT == GRIDGCN_ACT_SILU) {
         const float s = sigmoid(t);
@@ -101,7 +118,7 @@ template <int ACT> __device__ __forceinline__ float act_grad(float t)
     }
     if constexpr (ACT == GRIDGCN_ACT_GELU) {
         float e;
-        const float c = normal_cdf(t, e);
+        const float c = normal_cdf<T>(t, e);
         return fmaf(t * INV_SQRT_2PI, e, c);
     }
     return 1.f;
@@ -304,7 +321,7 @@ __device__ __forceinline__ void rows_apply(const Args &a, const Lay &l, const Po
             r[u].align(col);
             r[u].get(v);
 #pragma unroll
-            for (int i = 0; i < V; i++) o[i] = n < rv ? act_of<ACT>(fmaf(dev_of(k[i], v[i]), k[i].a, k[i].beta)) : 0.f;
+            for (int i = 0; i < V; i++) o[i] = n < rv ? act_of<ACT, T>(fmaf(dev_of(k[i], v[i]), k[i].a, k[i].beta)) : 0.f;
             gg_st_chunk(y + (size_t)n * a.C, p.c, a.C, o, a.past);
         }
     }
@@ -335,11 +352,11 @@ template <class T, bool Q8> struct Xhat {
 };
 
 // g = dy act'(t) of one value
-template <int ACT> __device__ __forceinline__ float gate(const Chan &k, float dy, float d, float x)
+template <int ACT, class T> __device__ __forceinline__ float gate(const Chan &k, float dy, float d, float x)
 {
     if constexpr (ACT == GRIDGCN_ACT_NONE) return dy;
     if constexpr (ACT == GRIDGCN_ACT_RELU) return __uint_as_float(__float_as_uint(x) ^ k.flip) > k.thr ? dy : 0.f;
-    return dy * act_grad<ACT>(fmaf(d, k.a, k.beta));
+    return dy * act_grad<ACT, T>(fmaf(d, k.a, k.beta));
 }
 
 // backward, first pass over r0 <= n < r1 (all below count): s = sums of g and g * xh per channel
@@ -375,7 +392,7 @@ __device__ __forceinline__ void rows_bwd_sums(const Args &a, const Lay &l, const
 #pragma unroll
             for (int i = 0; i < V; i++) {
                 const float d = dev_of(k[i], v[i]);
-                const float g = gate<ACT>(k[i], e[i], d, v[i]);
+                const float g = gate<ACT, T>(k[i], e[i], d, v[i]);
                 s0[i] += g;
                 s1[i] = fmaf(g, d * k[i].rstd, s1[i]);
             }
@@ -420,7 +437,7 @@ __device__ __forceinline__ void rows_bwd_dx(const Args &a, const Lay &l, const P
 #pragma unroll
             for (int i = 0; i < V; i++) {
                 const float d = dev_of(k[i], v[i]);
-                const float g = gate<ACT>(k[i], e[i], d, v[i]);
+                const float g = gate<ACT, T>(k[i], e[i], d, v[i]);
                 o[i] = n < rv ? fmaf(k[i].a, g, -fmaf(d * k[i].rstd, f[i].y, f[i].x)) : 0.f;
             }
             gg_st_chunk(dx + (size_t)n * a.C, p.c, a.C, o, a.past);
@@ -760,7 +777,7 @@ __global__ __launch_bounds__(FEW) void gg_k_gn_small(Args a, Lay l, int slab_c)
         float v[V], o[V];
         r[u].get(v);
 #pragma unroll
-        for (int i = 0; i < V; i++) o[i] = n < count ? act_of<ACT>(fmaf(dev_of(k[i], v[i]), k[i].a, k[i].beta)) : 0.f;
+        for (int i = 0; i < V; i++) o[i] = n < count ? act_of<ACT, T>(fmaf(dev_of(k[i], v[i]), k[i].a, k[i].beta)) : 0.f;
         gg_st_chunk(y + (size_t)n * a.C, p.c, a.C, o, false);
     }
 }
@@ -802,7 +819,7 @@ __global__ __launch_bounds__(FEW) void gg_k_gn_small_bwd(Args a, Lay l, int slab
 #pragma unroll
         for (int i = 0; i < V; i++) {
             const float d = dev_of(k[i], v[i]);
-            const float g = gate<ACT>(k[i], e[i], d, v[i]);
+            const float g = gate<ACT, T>(k[i], e[i], d, v[i]);
             s[i][0] += (double)g;
             s[i][1] = fma((double)g, (double)(d * k[i].rstd), s[i][1]);
         }
@@ -851,7 +868,7 @@ __global__ __launch_bounds__(FEW) void gg_k_gn_small_bwd(Args a, Lay l, int slab
 #pragma unroll
         for (int i = 0; i < V; i++) {
             const float d = dev_of(k[i], v[i]);
-            const float g = gate<ACT>(k[i], e[i], d, v[i]);
+            const float g = gate<ACT, T>(k[i], e[i], d, v[i]);
             o[i] = n < count ? fmaf(k[i].a, g, -fmaf(d * k[i].rstd, f[i].y, f[i].x)) : 0.f;
         }
         gg_st_chunk(dx + (size_t)n * a.C, p.c, a.C, o, false);

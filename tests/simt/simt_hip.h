@@ -642,6 +642,8 @@ template <class V> static inline simt_s16x2 simt_cvt_scalef32_pk_fp8(simt_s16x2 
 #define __builtin_amdgcn_cvt_scalef32_pk_f16_fp8 simt_cvt_scalef32_pk_f16_fp8
 static inline float simt_rcp(float x) { return 1.0f / x; }
 #define __builtin_amdgcn_rcpf simt_rcp
+static inline float simt_exp2(float x) { return __builtin_exp2f(x); }
+#define __builtin_amdgcn_exp2f simt_exp2
 static inline int simt_perm(unsigned a, unsigned b, unsigned sel)     // v_perm_b32: bytes 0-3 from b, 4-7 from a
 {
     const uint64_t v = ((uint64_t)a << 32) | b;

@@ -323,3 +323,54 @@ def test_registered_backwards_leave_out_what_is_not_needed():
             ctx = SimpleNamespace(saved_tensors=(None, codes, scales, st, v, v, None), needs_input_grad=need + (False,) * 5, gn=(4, "relu"))
             got = torch_ops._gn_bwd(ctx, e(2, 9, 32), None, None, None)
             assert len(got) == 8 and [t is not None for t in got[:3]] == list(need)
+
+
+# ---- GELU: as many digits as float32's own 0.5 t (1 + erf), and where Phi is small -----------------------------------------
+def run_gelu_digits(dev="cpu"):
+    """Norms of the error, in units of U = 2^-24.  A rounding is uniform within half a step: 0.42 U of a value, root mean square.  t has four
+    (x - mean, rstd, rstd weight, the product), which t f'/f <= 1.3 carries into f = t Phi(t): 1.1 U; Phi: 1 U (an erf good to a
+    step), the last product 0.42 U: 1.6 U together.  Between -1.5 and -0.5 |t f'/f| <= 1.2 and 1 + erf is a difference of up to three
+    times its size: 1 U, 2 U, 0.42 U: 2.3 U."""
+    import math
+    x = torch.randn(8, 4096, 16, generator=torch.Generator().manual_seed(5))
+    with torch.no_grad():
+        y = ops.group_norm_act(x.to(dev), None, None, 2, act="gelu").cpu().double()
+        wide = ops.group_norm_act(x.to(dev), torch.full((16,), 2.0, device=dev), None, 2, act="gelu").cpu().double()
+    t = ref.group_norm_act(x, None, None, 2, 1e-5, "none")["y"]
+    f = lambda t: t * 0.5 * torch.special.erfc(-t / math.sqrt(2))          # noqa: E731
+    for lo, hi, lim in ((-9.0, 9.0, 1.6), (-1.5, -0.5, 2.3)):
+        at = (t > lo) & (t < hi)
+        off = float((y - f(t))[at].norm() / f(t)[at].norm())
+        assert off <= lim * ref.U, (lo, hi, off / ref.U)
+    # value by value: t is off by 4 U of itself, f' / f is |t| + 1 / |t| at most; exponential and product as in the oracle's bound
+    t = 2 * t
+    off = ((wide - f(t)) / f(t)).abs()
+    at = (t < -0.1) & (t > -8.0)
+    assert int((t[at] < -6).sum()) > 20
+    assert bool((off <= ref.U * (4 * t * t + 4 + 8 * (1 + t.abs()) + 2))[at].all())
+
+
+def run_gelu_tail_of_16_bits(dtype, dev="cpu"):
+    """half a step of the type, and what the coarser fit may add (1e-7 exp(1.5 |t|), at most 2e-4)"""
+    import math
+    x = torch.randn(8, 4096, 16, generator=torch.Generator().manual_seed(6)).to(dtype)
+    with torch.no_grad():
+        y = ops.group_norm_act(x.to(dev), torch.full((16,), 2.0, device=dev), None, 2, act="gelu").cpu().double()
+    t = 2 * ref.group_norm_act(x, None, None, 2, 1e-5, "none")["y"]
+    want = t * 0.5 * torch.special.erfc(-t / math.sqrt(2))
+    at = (t < -0.1) & (want.abs() > torch.finfo(dtype).tiny)
+    assert int((t[at] < -3.5).sum()) > 100
+    fit = torch.clamp(1e-7 * torch.exp(1.5 * t.abs()), max=2e-4)
+    u = ref.U * (4 * t * t + 4 + 8 * (1 + t.abs()) + 2)
+    assert bool((((y - want) / want).abs() <= ref.half_step(dtype) * (1 + fit + u) + fit + u)[at].all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gelu_tail_of_16_bits(dtype):
+    with emu.emulated_gpu():
+        run_gelu_tail_of_16_bits(dtype)
+
+
+def test_gelu_digits():
+    with emu.emulated_gpu():
+        run_gelu_digits()

@@ -126,3 +126,12 @@ def test_registered_backwards_leave_out_what_is_not_needed():
         y = g.linear_act8(*leaves)[0]
         y.backward(dy)
         assert all((t.grad is not None) == n and (not n or torch.equal(t.grad, a)) for t, n, a in zip(leaves, need, full[0]))
+
+
+def test_gelu_digits():
+    cpu.run_gelu_digits(DEV)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gelu_tail_of_16_bits(dtype):
+    cpu.run_gelu_tail_of_16_bits(dtype, DEV)
