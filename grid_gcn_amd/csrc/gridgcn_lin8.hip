@@ -520,7 +520,8 @@ struct Wg {
     const void *dy;               // [R][N], stride ldy
     const uint8_t *codes, *scales; // without dw (tk = 1): any four readable bytes, Cp = 0
     void *dw, *db;                // [N][K], [N]
-    float *part, *dbpart;         // splits > 1: [split][tile][128][128], [split][tiles_n * 128]
+    float *part;                  // splits > 1: [split][tile][128][128]
+    double *dbpart;               // ... [split][tiles_n * 128]
     long long R, ldy;
     int N, K, Cp;
     unsigned tn, tk, splits, share;
@@ -677,7 +678,7 @@ __global__ __launch_bounds__(GW * 64, 1) void gg_k_lin8_wgrad(Wg p)
     for (int i = 0; i < 4; i++)
 #pragma unroll
         for (int t = 0; t < 4; t++) acc[i][t] = zero16();
-    float dbs[4] = {0.f, 0.f, 0.f, 0.f};
+    double dbs[4] = {0.0, 0.0, 0.0, 0.0};                          // (a lane's column over thousands of strips: 64 bits)
     Strip<T> q[D];
     // (never skipped -- past the end a strip is loaded again: behind a load that may or may not have been issued the compiler waits
     //  for everything in flight)
@@ -710,7 +711,7 @@ __global__ __launch_bounds__(GW * 64, 1) void gg_k_lin8_wgrad(Wg p)
                 float v = s.dyv(0, i);
 #pragma unroll
                 for (int e = 1; e < 8; e++) v += s.dyv(e, i);
-                dbs[i] += v;
+                dbs[i] += (double)v;
             }
         }
     };
@@ -782,31 +783,45 @@ __global__ __launch_bounds__(GW * 64, 1) void gg_k_lin8_wgrad(Wg p)
     }
     if (!first) return;
     __syncthreads();
+    double *ldsd = (double *)ldsf;
 #pragma unroll
-    for (int i = 0; i < 4; i++) ldsf[(wave * 4 + i) * 64 + lane] = dbs[i];
+    for (int i = 0; i < 4; i++) ldsd[(wave * 4 + i) * 64 + lane] = dbs[i];
     __syncthreads();
     if ((int)threadIdx.x < GT) {
         const int jj = threadIdx.x / 4, i = threadIdx.x % 4;
-        float v = 0.f;
+        double v = 0.0;
 #pragma unroll
-        for (int o = 0; o < GW; o++) v += ldsf[(o * 4 + i) * 64 + jj] + ldsf[(o * 4 + i) * 64 + jj + 32];
+        for (int o = 0; o < GW; o++) v += ldsd[(o * 4 + i) * 64 + jj] + ldsd[(o * 4 + i) * 64 + jj + 32];
         const int nn = n0 + (int)threadIdx.x;
         if (p.part) p.dbpart[(size_t)split * p.tn * GT + nn] = v;
-        else if (nn < p.N) GGRowT<T>::put((T *)p.db + nn, v);
+        else if (nn < p.N) GGRowT<T>::put((T *)p.db + nn, (float)v);
     }
 }
 
-// sums of the splits: a workgroup = 32 groups of 4 results x 8 lanes over the splits
+// sums of the splits: a workgroup = 32 groups of 4 results (db: 32 results, in 64 bits) x 8 lanes over the splits
 template <class T>
 __global__ __launch_bounds__(256) void gg_k_lin8_wsum(Wg p, unsigned nw)
 {
     __shared__ float4 red[8][32];
     const unsigned tiles = p.tn * p.tk;
     const int e = threadIdx.x & 31, l = threadIdx.x >> 5;
-    const bool isdb = blockIdx.x >= nw;
-    const size_t at = ((size_t)(isdb ? blockIdx.x - nw : blockIdx.x) * 32 + e) * 4;
-    const size_t stride = isdb ? (size_t)p.tn * GT : (size_t)tiles * GT * GT;
-    const float *src = (isdb ? p.dbpart : p.part) + at;
+    if (blockIdx.x >= nw) {
+        __shared__ double redd[8][32];
+        const size_t nn = (size_t)(blockIdx.x - nw) * 32 + e;
+        double v = 0.0;
+#pragma unroll 8
+        for (unsigned q = l; q < p.splits; q += 8) v += p.dbpart[q * (size_t)p.tn * GT + nn];
+        redd[l][e] = v;
+        __syncthreads();
+        if (l || nn >= (size_t)p.N) return;
+#pragma unroll
+        for (int q = 1; q < 8; q++) v += redd[q][e];
+        GGRowT<T>::put((T *)p.db + nn, (float)v);
+        return;
+    }
+    const size_t at = ((size_t)blockIdx.x * 32 + e) * 4;
+    const size_t stride = (size_t)tiles * GT * GT;
+    const float *src = p.part + at;
     float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 8
     for (unsigned q = l; q < p.splits; q += 8) {
@@ -822,15 +837,9 @@ __global__ __launch_bounds__(256) void gg_k_lin8_wsum(Wg p, unsigned nw)
         s.x += v.x; s.y += v.y; s.z += v.z; s.w += v.w;
     }
     const float v[4] = {s.x, s.y, s.z, s.w};
-    if (isdb) {
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-            if ((int)at + t < p.N) GGRowT<T>::put((T *)p.db + at + t, v[t]);
-    } else {
-        const unsigned tile = (unsigned)(at / (GT * GT));
-        const int rem = (int)(at % (GT * GT)), n = (int)(tile / p.tk) * GT + rem / GT, k = (int)(tile % p.tk) * GT + rem % GT;
-        if (n < p.N) put_row<T, 4>((T *)p.dw, n, k, p.K, v);
-    }
+    const unsigned tile = (unsigned)(at / (GT * GT));
+    const int rem = (int)(at % (GT * GT)), n = (int)(tile / p.tk) * GT + rem / GT, k = (int)(tile % p.tk) * GT + rem % GT;
+    if (n < p.N) put_row<T, 4>((T *)p.dw, n, k, p.K, v);
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
@@ -888,7 +897,7 @@ unsigned splits_of(long long R, unsigned tiles)
 size_t wgrad_bytes(long long R, unsigned tn, unsigned tk)
 {
     const unsigned s = splits_of(R, tn * tk);
-    return s > 1 ? (size_t)s * ((size_t)tn * tk * GT * GT + (size_t)tn * GT) * 4 : 0;
+    return s > 1 ? (size_t)s * ((size_t)tn * tk * GT * GT * sizeof(float) + (size_t)tn * GT * sizeof(double)) : 0;
 }
 
 template <class T> int launch_wgrad(Wg &p, hipStream_t st)
@@ -905,7 +914,7 @@ template <class T> int launch_wgrad(Wg &p, hipStream_t st)
     const unsigned units = (p.splits * p.share + 7) / 8 * 8;
     gg_k_lin8_wgrad<T><<<units * ((tiles + p.share - 1) / p.share), GW * 64, LDS, st>>>(p);
     if (p.splits > 1) {
-        const unsigned nw = p.dw ? tiles * (GT * GT / 128) : 0, nd = p.db ? p.tn : 0;
+        const unsigned nw = p.dw ? tiles * (GT * GT / 128) : 0, nd = p.db ? p.tn * (GT / 32) : 0;
         gg_k_lin8_wsum<T><<<nw + nd, 256, 0, st>>>(p, nw);
     }
     return 0;
@@ -984,7 +993,7 @@ int gridgcn_linear_act8_bwd(const void *dy, int dtype, long long R, int N, long 
     if (need && (!ws || ws_bytes < need || ((uintptr_t)ws & 15))) return GRIDGCN_EWORKSPACE;
     if (g.splits > 1) {
         g.part = (float *)ws;
-        g.dbpart = g.part + (size_t)g.splits * g.tn * g.tk * GT * GT;
+        g.dbpart = (double *)(g.part + (size_t)g.splits * g.tn * g.tk * GT * GT);
     }
     const hipStream_t st = (hipStream_t)stream;
     const int rc = with_type(dtype, [&](auto *t) {

@@ -135,3 +135,19 @@ def test_gelu_digits():
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_gelu_tail_of_16_bits(dtype):
     cpu.run_gelu_tail_of_16_bits(dtype, DEV)
+
+
+@pytest.mark.parametrize("R,N,K", [(65536, 2048, 2048), (1048576, 64, 3)])
+def test_linear_act8_db_of_many_rows(R, N, K):
+    """The sums run in float32 over eight rows, then in 64 bits.  The roundings of the first are independent and, over R / 8 sums, 0.02
+    U of the result; what is left is the last rounding, half a step: 1 U = 2^-24 (a chain of float32 sums: 2 U and more)."""
+    g = torch.Generator().manual_seed(3)
+    dy = 1 + torch.rand(R, N, generator=g)
+    x = torch.randn(64, K, generator=g).to(DEV).repeat(R // 64, 1)
+    w, b = torch.zeros(N, K, device=DEV), torch.zeros(N, device=DEV, requires_grad=True)
+    db, = torch.autograd.grad(cpu.ops.linear_act8(x, w.requires_grad_(), b), b, dy.to(DEV))
+    want = dy.double().sum(0)
+    assert float(((db.cpu().double() - want) / want).abs().max()) <= 1.05 * 2.0 ** -24
+    # ... in the call that forms dW too
+    db = torch.autograd.grad(cpu.ops.linear_act8(x, w, b), (w, b), dy.to(DEV))[1]
+    assert float(((db.cpu().double() - want) / want).abs().max()) <= 1.05 * 2.0 ** -24
