@@ -1011,7 +1011,7 @@ int gridgcn_group_norm_act_fwd(const void *x, int dtype, int B, long long N, int
         !(eps >= 0.f) || act < GRIDGCN_ACT_NONE || act > GRIDGCN_ACT_GELU || !codes != !scales || ((uintptr_t)codes & 15))
         return GRIDGCN_EINVAL;
     const Plan p = plan_of(B, N, C, G, dtype, codes != nullptr, stats != nullptr, false);
-    if (p.bytes && (!ws || ws_bytes < p.bytes)) return GRIDGCN_EWORKSPACE;
+    if (p.bytes && (!ws || ws_bytes < p.bytes || ((uintptr_t)ws & 15))) return GRIDGCN_EWORKSPACE;
     Args a = {};
     a.x = x; a.y = y; a.N = N; a.xb = ldb; a.xn = ldn; a.B = B; a.C = C; a.G = G; a.cg = C / G; a.ptype = ptype;
     a.gamma = gamma; a.beta = beta; a.counts = counts; a.eps = eps; a.codes_out = codes; a.scales_out = scales;
@@ -1039,7 +1039,7 @@ int gridgcn_group_norm_act_bwd(const void *dy, long long ldgb, long long ldgn, c
         return GRIDGCN_EINVAL;
     if (!dx && !dgamma && !dbeta) return GRIDGCN_OK;
     const Plan p = plan_of(B, N, C, G, dtype, false, true, true);
-    if (p.bytes && (!ws || ws_bytes < p.bytes)) return GRIDGCN_EWORKSPACE;
+    if (p.bytes && (!ws || ws_bytes < p.bytes || ((uintptr_t)ws & 15))) return GRIDGCN_EWORKSPACE;
     Args a = {};
     a.dy = dy; a.gb = ldgb; a.gn = ldgn; a.x = x; a.xb = ldb; a.xn = ldn; a.codes = codes; a.scales = scales;
     a.y = dx; a.N = N; a.B = B; a.C = C; a.G = G; a.cg = C / G; a.ptype = ptype; a.gamma = gamma; a.beta = beta;

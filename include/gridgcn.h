@@ -858,7 +858,7 @@ int gridgcn_gridconv_forward(const float *src, const int32_t *nebidx, const floa
  *   what lies below 2^-134 of one is dropped), and codes / scales (both or neither) the 8-bit form of x.
  * gridgcn_linear_act8_bwd: dx[R][K] = dy W;  dW[N][K] = dy^T x^ with x^ the values of codes / scales;  dbias[N] = sum of
  *   dy; any of them may be NULL (codes, scales only for dW; W only for dx).
- * *_workspace_bytes may answer 0: ws may then be NULL (group norm: stats = whether the call passes stats, save8 =
+ * *_workspace_bytes may answer 0: ws may then be NULL; else it is 16-byte aligned (group norm: stats = whether the call passes stats, save8 =
  *   whether it passes codes to write; both ignored with backward).  Row strides of at most GRIDGCN_MAX_LD elements.
  * Sums have one order: the same call gives the same bits. */
 #define GRIDGCN_F32 0

@@ -374,3 +374,17 @@ def test_gelu_tail_of_16_bits(dtype):
 def test_gelu_digits():
     with emu.emulated_gpu():
         run_gelu_digits()
+
+
+def test_c_entries_refuse_a_workspace_off_its_alignment():
+    import ctypes
+    from grid_gcn_amd import _lib, build
+    build.build()
+    lib = _lib.load()
+    a = (ctypes.cast((ctypes.c_float * 256)(), ctypes.c_void_p).value + 15) & ~15
+    EWORKSPACE = 2
+    for ws in (a + 4, a + 8):
+        assert lib.gridgcn_group_norm_act_fwd(a, 0, 2, 100000, 8, 800000, 8, 2, a, a, 0, None, 1e-5, 1, a, None, None, None, ws, 1 << 30,
+                                              None) == EWORKSPACE
+        assert lib.gridgcn_group_norm_act_bwd(a, 800000, 8, a, 800000, 8, None, None, 0, 2, 100000, 8, 2, a, a, a, 0, None, 1, a, a, a,
+                                              ws, 1 << 30, None) == EWORKSPACE
