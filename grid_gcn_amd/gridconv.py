@@ -36,7 +36,13 @@ class ConvBNReLU(nn.Module):
         y = self.lin(x)
         if self.bn is not None:
             shp = y.shape
-            y = self.bn(y.reshape(-1, shp[-1])).reshape(shp)
+            y = y.reshape(-1, shp[-1])
+            if self.bn.training and y.dtype == torch.float32 and not y.is_cuda:
+                # [1, C, rows]: the CPU sums a channel in 64 bits; of [rows, C] it sums the rows of a thread in 32, and the
+                # fewer threads, the fewer digits (one thread, 60000 rows: 4e-6 of the norm)
+                y = self.bn(y.t().contiguous()[None])[0].t().reshape(shp)
+            else:
+                y = self.bn(y).reshape(shp)
         return F.relu(y) if self.use_relu else y
 
     def folded(self):

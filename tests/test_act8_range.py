@@ -388,3 +388,37 @@ def test_c_entries_refuse_a_workspace_off_its_alignment():
                                               None) == EWORKSPACE
         assert lib.gridgcn_group_norm_act_bwd(a, 800000, 8, a, 800000, 8, None, None, 0, 2, 100000, 8, 2, a, a, a, 0, None, 1, a, a, a,
                                               ws, 1 << 30, None) == EWORKSPACE
+
+
+# ---- ConvBNReLU on the CPU: statistics that do not depend on the number of threads -------------------------------------------
+def test_batch_statistics_on_the_cpu_keep_their_digits():
+    """y, dx, dgamma, dbeta of 300000 rows against float64, on one thread and on all.  A dozen roundings per value, U = 2^-24 each at
+    most, of terms up to twice the result: 24 U of the norm -- of dgamma and dbeta, whose terms
+    cancel (3e5 of magnitude 0.8 leave 1e4), of the norm of the sums of their terms' magnitudes.  (A float32 sum over the rows of a thread: 70 U and more.  The
+    linear layer's own weight gradient is a float32 product over the rows, not looked at here.)"""
+    g = torch.Generator().manual_seed(7)
+    x, dy = torch.randn(300000, 4, generator=g), torch.randn(300000, 6, generator=g) + 1
+    torch.manual_seed(0)
+    layer = gridconv.ConvBNReLU(4, 6).train()
+    with torch.no_grad():
+        layer.lin.bias.uniform_(-2, 2)
+        layer.bn.bias.uniform_(2, 3)                       # (mostly open gates: a gate that flips is no rounding)
+    xd, w = x.double().requires_grad_(), {k: v.detach().double().requires_grad_() for k, v in layer.named_parameters()}
+    z = xd @ w["lin.weight"].t() + w["lin.bias"]
+    t = (z - z.mean(0)) / torch.sqrt(z.var(0, unbiased=False) + layer.bn.eps) * w["bn.weight"] + w["bn.bias"]
+    keep = (t.detach().abs() > 1e-4).double()
+    want = torch.autograd.grad((torch.relu(t) * keep * dy).sum(), [xd, w["bn.weight"], w["bn.bias"]])
+    g = (keep * (t > 0) * dy).detach()
+    xh = ((t - w["bn.bias"]) / w["bn.weight"]).detach()
+    size = [torch.relu(t), want[0], (g * xh).abs().sum(0), g.abs().sum(0)]
+    threads = torch.get_num_threads()
+    try:
+        for n in {1, threads}:
+            torch.set_num_threads(n)
+            xr = x.clone().requires_grad_()
+            y = layer(xr)
+            got = torch.autograd.grad((y * keep.float() * dy).sum(), [xr, layer.bn.weight, layer.bn.bias])
+            for a, b, s in zip((y,) + got, (torch.relu(t),) + want, size):
+                assert float((a.double() - b).norm() / s.norm()) <= 24 * ref.U, n
+    finally:
+        torch.set_num_threads(threads)
