@@ -172,6 +172,28 @@ def geo_features(neighbors, centers_xyz):
     return geo_vec, geo_dist, att_vec
 
 
+class _PairMax(torch.autograd.Function):
+    """(a * b).max(dim=2).values of [B, O, P, C] edges, keeping for the backward the two factors of each maximum [B, O, C] in place of
+    both factors of every edge (which layers with 8-bit checkpoints do not hold otherwise)"""
+
+    @staticmethod
+    def forward(ctx, a, b):
+        agg, at = (a * b).max(dim=2, keepdim=True)
+        ctx.save_for_backward(a.gather(2, at), b.gather(2, at), at)
+        ctx.edges = a.shape[2]
+        return agg.squeeze(2)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        a, b, at = ctx.saved_tensors
+        shape = a.shape[:2] + (ctx.edges,) + a.shape[3:]
+        g = g.unsqueeze(2)
+        da, db = (g.new_zeros(shape).scatter_(2, at, g * other) if need else None
+                  for other, need in zip((b, a), ctx.needs_input_grad))
+        return da, db
+
+
 class Tail:
     """What directly follows a GridConv block in the CALLER (the segmentation head behind the last
     up layer): conv+BN+ReLU `layers` that may join the block's update chain, and optionally the
@@ -324,9 +346,12 @@ class SubGUpdate(nn.Module):
             if tedge.edge_block_supported(pt_layers, att_layers, nf, nebidx.shape[2]):
                 agg = tedge.edge_block_train(nf, att_vec, pt_layers, att_layers)
                 return self.finish(agg, center_masks, center_ori_feats, tail=tail)
-        pair = run_mlp(att_layers, att_vec, self.mfma_train, counts) * \
-            run_mlp(pt_layers, nf, self.mfma_train, counts)
-        agg = pair.max(dim=2).values
+        att, pt = run_mlp(att_layers, att_vec, self.mfma_train, counts), run_mlp(pt_layers, nf, self.mfma_train, counts)
+        if isinstance(pt_layers[0], ConvGNAct) and torch.is_grad_enabled():
+            agg = _PairMax.apply(att, pt)
+        else:
+            agg = (att * pt).max(dim=2).values
+        del att, pt
         return self.finish(agg, center_masks, center_ori_feats, tail=tail, counts=counts)
 
     def packed_layers(self):

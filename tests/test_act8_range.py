@@ -422,3 +422,41 @@ def test_batch_statistics_on_the_cpu_keep_their_digits():
                 assert float((a.double() - b).norm() / s.norm()) <= 24 * ref.U, n
     finally:
         torch.set_num_threads(threads)
+
+
+# ---- what an edge block with 8-bit checkpoints holds between forward and backward -------------------------------------------
+def run_edge_block_holds(dev="cpu"):
+    B, O, P, C = 1, 40, 8, 64
+    torch.manual_seed(3)
+    layer = gridconv.SubGUpdate(16, [32, C], localfdim=3, norm="group").to(dev).train()
+    src = torch.randn(B, 50, 4 + 16).to(dev).requires_grad_()
+    cent = torch.randn(B, O, 4).to(dev)
+    idx = torch.randint(0, 50, (B, O, P), dtype=torch.int32).to(dev)
+    held = {}
+
+    def pack(t):
+        held[t.untyped_storage().data_ptr()] = (t.untyped_storage().nbytes(), t.dtype)
+        return t
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+        out = layer.forward_src(cent, src, idx)
+    # the widest edge tensors as codes (of both products' inputs and both norms'), none of them in float32
+    assert not [h for h in held.values() if h[0] >= B * O * P * C * 4 and h[1] == torch.float32], held
+    edges = [c for l in (layer.att1, layer.att2, layer.pt_mlp) for c in l]
+    codes = sum(-(-c // 32) * 33 for l in edges for c in (l.lin.in_features, l.lin.out_features))
+    assert sum(h[0] for h in held.values()) <= B * O * P * codes + 4 * B * O * C * 8 + 100000
+    dy = torch.randn(out.shape).to(dev)
+    got = torch.autograd.grad(out, [src] + list(layer.parameters()), dy)
+    # against the stock product and maximum on the same layers
+    nf, att = ops.edge_inputs(src, idx, cent, has_feats=True, localfdim=3)
+    pair = gridconv.run_mlp([layer.att1[0], layer.att2[0]], att) * gridconv.run_mlp(list(layer.pt_mlp), nf)
+    want = layer.finish(pair.max(dim=2).values, None, None)
+    assert torch.equal(out, want)
+    for a, b in zip(got, torch.autograd.grad(want, [src] + list(layer.parameters()), dy)):
+        # (the same values; the gather's gradient sums may come in another order)
+        assert float((a - b).norm()) <= 2.0 ** -20 * float(b.norm())
+
+
+def test_edge_block_holds_no_float32_edges():
+    with emu.emulated_gpu():
+        run_edge_block_holds()

@@ -151,3 +151,7 @@ def test_linear_act8_db_of_many_rows(R, N, K):
     # ... in the call that forms dW too
     db = torch.autograd.grad(cpu.ops.linear_act8(x, w, b), (w, b), dy.to(DEV))[1]
     assert float(((db.cpu().double() - want) / want).abs().max()) <= 1.05 * 2.0 ** -24
+
+
+def test_edge_block_holds_no_float32_edges():
+    cpu.run_edge_block_holds(DEV)
