@@ -1,7 +1,7 @@
 // gridgcn_act8.hip -- rows to and from the 8-bit form of gridgcn_act8.h.  Bound by memory: T + 1.03 bytes per value.
 // A thread keeps ONE column chunk of 16 bytes and walks rows: no division in the loop, whole lines per wave; the 8 (fp32)
 // or 4 (16-bit) neighbouring lanes of a 32-channel block find its maximum with cross-lane moves.
-// 655360 rows of fp32: C = 128 pack 80 us (5.3 TB/s), unpack 62 (6.8); C = 131 (rows that start anywhere, codes of 160) 89 (5.1), 108 (4.2).
+// 655360 rows of fp32: C = 128 pack 80 us (5.3 TB/s), unpack 62 (6.8); C = 131 (rows that start anywhere, codes of 160) 86 (5.2), 111 (4.1).
 #include "../../include/gridgcn.h"
 #include "gridgcn_act8.h"
 

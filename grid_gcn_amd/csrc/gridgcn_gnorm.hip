@@ -449,9 +449,10 @@ __device__ __forceinline__ void rows_bwd_dx(const Args &a, const Lay &l, const P
     for (; n0 < r1; n0 += l.rpb) gg_st_chunk(dx + (size_t)n0 * a.C, p.c, a.C, z, a.past);
 }
 
-// Bound by memory.  8 x 81920 x 128 fp32 (336 MB a tensor), SiLU: stats 61 us (5.5 TB/s), apply 115 (5.8), backward sums 113 (5.9),
-// dx 176 (5.7): the forward reads x twice, the backward x and dy twice.  16 x 65536 x 64 bf16, GELU, x kept in 8 bits:
-// stats 46 (with the codes written), apply 55, sums 71, dx 70.
+// Average (least) of ten calls, us.  8 x 81920 x 128 fp32 (336 MB a tensor), SiLU: stats 67 (60), apply 117 (114), backward sums 116 (112), dx
+// 180 (176): memory, at 5.0 - 5.8 TB/s; the forward reads x twice, the backward x and dy twice.  16 x 65536 x 64 bf16, GELU, x kept in 8
+// bits: stats 48 (46, the codes written), apply 55 (53), sums 78 (74), dx 76 (73): the last three bound by arithmetic (GELU and the codes
+// keep the vector pipes busy all the time).
 // ---- many rows: pass, small launch, pass ----------------------------------------------------------------------------
 template <class T, bool SAVE8>
 __global__ __launch_bounds__(THREADS, 4) void gg_k_gn_stats(Args a, Lay l)
@@ -693,7 +694,7 @@ __global__ __launch_bounds__(THREADS) void gg_k_gn_params(Args a)
 
 // ---- few rows: one launch, a workgroup = whole groups of one cloud (l.nq chunks from channel slab * slab_c on), every value read
 // once and kept in registers: the time is one trip to memory, a reduction and the stores: 16 ragged clouds of 1024 rows, 128
-// channels, fp32: forward 10 us, backward 13; 32 rows of 512: 7 and 9 --------------------------------------
+// channels, fp32, average (least) of ten: forward with the codes 19 us (17), backward 15 (14); 32 rows of 512: 8 (7) and 10 (9) --------
 template <class T, int ACT, bool SAVE8>
 __global__ __launch_bounds__(FEW) void gg_k_gn_small(Args a, Lay l, int slab_c)
 {

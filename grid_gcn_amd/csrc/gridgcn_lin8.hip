@@ -11,9 +11,12 @@
 // (Two fp16 numbers and three partial products under one power of two per row and column: 272 us for the y below, and what lies 2^-33
 // under the largest value of its row was gone, against a weight of zero too.)
 //
-// 655360 rows, 256 -> 128, fp32, average (least) of ten: y and codes 342 us (279; 1.18 GB: 3.5 TB/s, six products: 755 TFLOP/s), dx 344
-// (295; 1.0 GB), dW 175 (137; 0.5 GB, three products: 736 TFLOP/s), W laid out 5 - 11, dW's partial sums 5.   262144 rows, 256 -> 512, bf16: y and codes 167 (0.47 GB, 412 TFLOP/s), dx 123,
-// dW 100 (688 TFLOP/s): bound by issue, as vector and matrix instructions of a SIMD take turns.   Few rows: 32, 512 -> 256, fp32: y 7, dx 5, dW 11.
+// Average (least) of ten calls, us.  655360 rows, 256 -> 128, fp32: y and codes 352 (288; 1.18 GB: 3.4 TB/s, six products: 732 TFLOP/s), dx
+// 357 (295; 1.0 GB), dW 180 (139; 0.5 GB, three products: 716 TFLOP/s), W laid out 5 - 11, dW's partial sums 5: matrix pipe busy 43 - 48 %
+// of the cycles, vector 26 - 41.
+// 262144 rows, 256 -> 512, bf16: y and codes 178 (166; 0.47 GB, 386 TFLOP/s), dx 133 (123), dW 106 (96; 648 TFLOP/s): matrix 18, 26, 36 %,
+// vector 23, 15, 33 %; what is left of y and dx are waits (a step of K ends at a barrier and at all of its loads).
+// Few rows: 32, 512 -> 256, fp32: y 9 (7), dx 5 (5), dW 12 (11).
 #include "../../include/gridgcn.h"
 #include "gridgcn_act8.h"
 #include "gridgcn_mma.h"
